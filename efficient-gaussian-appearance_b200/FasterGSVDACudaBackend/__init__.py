@@ -4,12 +4,13 @@ initialize_residual_mlp, FusedAdam, update_3d_filter, relocation_adjustment and 
 (hand-written sm_100a CUDA behind a C ABI)."""
 from .rasterization import diff_rasterize, rasterize, update_pruning_scores, RasterizerSettings, initialize_appearance, initialize_residual_mlp
 from .adam import FusedAdam
+from .adamw import FusedAdamW
 from .filter3d import update_3d_filter
 from .densification import relocation_adjustment, add_noise
 
 __all__ = [
     'diff_rasterize', 'rasterize', 'update_pruning_scores', 'RasterizerSettings', 'initialize_appearance', 'initialize_residual_mlp',
-    'FusedAdam',
+    'FusedAdam', 'FusedAdamW',
     'update_3d_filter',
     'relocation_adjustment', 'add_noise',
 ]

@@ -58,6 +58,16 @@ class AdamSegment(ctypes.Structure):
                 ('n_learning_rates', c_int32), ('beta1', c_double), ('beta2', c_double), ('eps', c_double)]
 
 
+class AdamwHyper(ctypes.Structure):
+    _fields_ = [('learning_rates', c_double * 7), ('n_learning_rates', c_int32), ('reserved', c_int32), ('beta1', c_double), ('beta2', c_double),
+                ('eps', c_double), ('weight_decay', c_double), ('step', c_int64)]
+
+
+class AdamwTensors(ctypes.Structure):
+    _fields_ = [('count', c_int64)] + [(name, c_void_p) for name in (
+        'param', 'grad', 'exp_avg', 'exp_avg_sq', 'exp_avg_exponent', 'exp_avg_sq_exponent', 'master', 'n_elements', 'hyper')]
+
+
 class PeerBuffers(ctypes.Structure):
     _fields_ = [('n_ranks', c_int), ('grads', c_void_p * 8), ('params', c_void_p * 8), ('local_params', c_void_p),
                 ('multicast_grads', c_void_p), ('multicast_params', c_void_p)]
@@ -94,6 +104,10 @@ PROTOTYPES = {
     'fgs_update_3d_filter': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_float, c_float, c_float, c_float, c_float,
                                      c_float, c_float, c_float, c_void_p]),
     'fgs_adam_step': (c_int, [_P(AdamSegment), c_int, c_void_p]),
+    'fgs_adamw_step': (c_int, [_P(AdamwTensors), _P(AdamwHyper), c_int, c_int, c_int, c_void_p, c_int, c_double, c_void_p, c_void_p]),
+    'fgs_grad_squares_capacity': (c_int, [c_int64, _P(c_int)]),
+    'fgs_grad_squares': (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, _P(c_int), c_void_p]),
+    'fgs_adamw_read_moments': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p]),
     'fgs_profile_enable': (c_int, [c_int]),
     'fgs_inference_noalloc': (c_int, [c_void_p, _P(Primitives), _P(Settings), c_void_p, c_int, c_int, c_void_p, _P(c_int64), _P(c_int64)]),
     'fgs_profile_collect': (c_int, [ctypes.c_char_p, c_size_t, _P(c_double), c_int, _P(c_int)]),

@@ -1,7 +1,8 @@
-"""Builds libfgs_b200.so (all CUDA sources of csrc/) for sm_100a with nvcc, in parallel, in-tree.
+"""Builds libfgs_b200.so (all CUDA sources of csrc/) for sm_100a with nvcc, in parallel, in-tree, and the Python module
+_fgs_host (csrc/host.cpp, the host side of the many-tensor operators) with the C++ compiler against torch.
 
-Usage: python build.py [--force]. The shared library lands in FasterGSVDACudaBackend/lib/ so that it
-travels with the source tree; objects go to _build/ next to this file.
+Usage: python build.py [--force]. The shared libraries land in FasterGSVDACudaBackend/lib/ so that they
+travel with the source tree; objects go to _build/ next to this file.
 """
 import concurrent.futures
 import hashlib
@@ -14,6 +15,8 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / 'csrc'
 BUILD = HERE / '_build'
 LIB = HERE / 'FasterGSVDACudaBackend' / 'lib' / 'libfgs_b200.so'
+HOST_LIB = LIB.with_name('_fgs_host.so')
+CXX = os.environ.get('CXX', 'g++')
 NVCC = os.environ.get('NVCC', '/usr/local/cuda/bin/nvcc')
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
 # Default for the remaining sources (sort, adam, densification, the C ABI): -fmad=false, no implicit contraction of
@@ -60,6 +63,27 @@ def _compile(src: Path, headers_digest: str) -> Path:
     return obj
 
 
+def _compile_host() -> Path:
+    """The torch-facing host module: compiled against the headers and libraries of the installed torch."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    src = CSRC / 'host.cpp'
+    stamp = BUILD / 'host.stamp'
+    key = torch.__version__ + sys.version + hashlib.sha256(src.read_bytes()).hexdigest()
+    if HOST_LIB.exists() and stamp.exists() and stamp.read_text() == key:
+        return HOST_LIB
+    libs = [p for p in cpp_extension.library_paths() if Path(p).exists()]
+    cmd = [CXX, '-O2', '-std=c++17', '-fPIC', '-shared', f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}',
+           *[f'-I{p}' for p in cpp_extension.include_paths()], f"-I{sysconfig.get_paths()['include']}", str(src), '-o', str(HOST_LIB),
+           *[f'-L{p}' for p in libs], '-lc10', '-ltorch_cpu', '-ltorch_python']
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f'{CXX} failed for {src.name}:\n{res.stdout}\n{res.stderr}')
+    stamp.write_text(key)
+    return HOST_LIB
+
+
 def build(force: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     LIB.parent.mkdir(parents=True, exist_ok=True)
@@ -70,7 +94,9 @@ def build(force: bool = False) -> Path:
         for f in BUILD.glob('*.stamp'):
             f.unlink()
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        host = ex.submit(_compile_host)
         objs = list(ex.map(lambda s: _compile(s, hd), sources))
+    host.result()
     cmd = [NVCC, *ARCH, '-shared', '-o', str(LIB), *map(str, objs), '-lcudart']
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:

@@ -4,6 +4,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -729,6 +730,98 @@ int fgs_adam_step(const fgs_adam_segment* segs, int n, void* stream) {
     if (k < 0) return FGS_ERR_INVALID_ARGUMENT;
     ProfScope p_("adam", static_cast<cudaStream_t>(stream));
     FGS_CUDA(fgs::launch_adam(S, k, static_cast<cudaStream_t>(stream)), "adam");
+    return FGS_OK;
+}
+
+int fgs_adamw_step(const fgs_adamw_tensors* t, const fgs_adamw_hyper* hypers, int n_hypers, int dtype, int state_bits, const double* partials,
+                   int n_partials, double max_norm, float* grad_norm, void* stream) {
+    static_assert(FGS_ADAMW_BLOCK == fgs::kAdamwBlock && FGS_DTYPE_F32 == fgs::kDtypeF32 && FGS_DTYPE_BF16 == fgs::kDtypeBf16 &&
+                      FGS_DTYPE_F16 == fgs::kDtypeF16,
+                  "C ABI constants");
+    if (!t || t->count < 0 || t->count > 0x7FFFFFFF) return fail(FGS_ERR_INVALID_ARGUMENT, "bad tensor list");
+    if (dtype < FGS_DTYPE_F32 || dtype > FGS_DTYPE_F16) return fail(FGS_ERR_INVALID_ARGUMENT, "unknown dtype");
+    if (state_bits != 8 && state_bits != 32) return fail(FGS_ERR_INVALID_ARGUMENT, "state_bits must be 8 or 32");
+    if (t->count == 0) return FGS_OK;
+    const bool eight = state_bits == 8, master = t->master != nullptr;
+    if (!t->param || !t->grad || !t->exp_avg || !t->exp_avg_sq || !t->n_elements || !t->hyper || !hypers || n_hypers < 1)
+        return fail(FGS_ERR_INVALID_ARGUMENT, "NULL argument");
+    if (eight && (!t->exp_avg_exponent || !t->exp_avg_sq_exponent)) return fail(FGS_ERR_INVALID_ARGUMENT, "8-bit moments need their exponents");
+    if (master && dtype == FGS_DTYPE_F32) return fail(FGS_ERR_INVALID_ARGUMENT, "master weights are for half-precision parameters");
+    if (partials && (n_partials < 0 || !grad_norm || !(max_norm > 0.0))) return fail(FGS_ERR_INVALID_ARGUMENT, "clipping needs max_norm > 0 and grad_norm");
+    try {
+        std::vector<fgs::AdamwHyper> H(static_cast<size_t>(n_hypers));
+        for (int i = 0; i < n_hypers; i++) {
+            const fgs_adamw_hyper& a = hypers[i];
+            if (a.n_learning_rates < 1 || a.n_learning_rates > 7) return fail(FGS_ERR_INVALID_ARGUMENT, "between 1 and 7 learning rates are supported");
+            if (a.step < 1) return fail(FGS_ERR_INVALID_ARGUMENT, "step must be >= 1");
+            if (!(a.beta1 >= 0.0 && a.beta1 < 1.0 && a.beta2 >= 0.0 && a.beta2 < 1.0)) return fail(FGS_ERR_INVALID_ARGUMENT, "betas must be in [0, 1)");
+            if (!(a.eps >= 0.0)) return fail(FGS_ERR_INVALID_ARGUMENT, "eps must not be negative");
+            fgs::AdamwHyper& h = H[static_cast<size_t>(i)];
+            const double bc1 = 1.0 / (1.0 - std::pow(a.beta1, static_cast<double>(a.step)));
+            for (int j = 0; j < 7; j++) {
+                const double lr = j < a.n_learning_rates ? a.learning_rates[j] : 0.0;
+                h.lr[j] = static_cast<float>(lr * bc1);
+                h.decay[j] = static_cast<float>(1.0 - lr * a.weight_decay);
+            }
+            h.n_lr = a.n_learning_rates;
+            h.beta1 = static_cast<float>(a.beta1);
+            h.rest1 = static_cast<float>(1.0 - a.beta1);
+            h.beta2 = static_cast<float>(a.beta2);
+            h.rest2 = static_cast<float>(1.0 - a.beta2);
+            h.eps = static_cast<float>(a.eps);
+            h.root_rcp = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(a.beta2, static_cast<double>(a.step))));
+            h.step = static_cast<uint32_t>(a.step);
+        }
+        for (int64_t i = 0; i < t->count; i++) {
+            if (t->n_elements[i] <= 0) continue;
+            if (!t->param[i] || !t->grad[i] || !t->exp_avg[i] || !t->exp_avg_sq[i] || (master && !t->master[i]) ||
+                (eight && (!t->exp_avg_exponent[i] || !t->exp_avg_sq_exponent[i])))
+                return fail(FGS_ERR_INVALID_ARGUMENT, "tensor pointer is NULL");
+            if (t->hyper[i] < 0 || t->hyper[i] >= n_hypers) return fail(FGS_ERR_INVALID_ARGUMENT, "hyperparameter index out of range");
+        }
+        const fgs::AdamwTensors A{static_cast<int>(t->count), t->param, t->grad, t->exp_avg, t->exp_avg_sq, t->exp_avg_exponent,
+                                  t->exp_avg_sq_exponent, t->master, t->n_elements, t->hyper};
+        const fgs::AdamwClip clip{partials, n_partials, max_norm, grad_norm};
+        ProfScope p_("adamw", static_cast<cudaStream_t>(stream));
+        FGS_CUDA(fgs::launch_adamw(A, H.data(), dtype, eight, master, clip, static_cast<cudaStream_t>(stream)), "adamw");
+    } catch (const std::exception& e) {
+        return fail(FGS_ERR_INVALID_ARGUMENT, e.what());
+    }
+    return FGS_OK;
+}
+
+int fgs_grad_squares_capacity(int64_t count, int* out) {
+    if (!out || count < 0 || count > 0x7FFFFF) return fail(FGS_ERR_INVALID_ARGUMENT, "bad argument");
+    *out = fgs::grad_squares_launches(static_cast<int>(count)) * fgs::kNormPartials;
+    return FGS_OK;
+}
+
+int fgs_grad_squares(const void* const* grads, const int64_t* n_elements, const uint8_t* dtypes, int64_t count, double* partials, int capacity,
+                     int* n_partials, void* stream) {
+    int need = 0;
+    const int rc = fgs_grad_squares_capacity(count, &need);
+    if (rc != FGS_OK) return rc;
+    if (!n_partials || (count > 0 && (!grads || !n_elements || !dtypes || !partials))) return fail(FGS_ERR_INVALID_ARGUMENT, "NULL argument");
+    if (capacity < need) return fail(FGS_ERR_WORKSPACE, "too few partial sums");
+    for (int64_t i = 0; i < count; i++) {
+        if (dtypes[i] > FGS_DTYPE_F16) return fail(FGS_ERR_INVALID_ARGUMENT, "unknown dtype");
+        if (n_elements[i] > 0 && !grads[i]) return fail(FGS_ERR_INVALID_ARGUMENT, "gradient pointer is NULL");
+    }
+    ProfScope p_("grad_norm", static_cast<cudaStream_t>(stream));
+    FGS_CUDA(fgs::launch_grad_squares(grads, n_elements, dtypes, static_cast<int>(count), partials, n_partials, static_cast<cudaStream_t>(stream)),
+             "gradient norm");
+    return FGS_OK;
+}
+
+int fgs_adamw_read_moments(const uint8_t* const* codes, const uint8_t* const* exponents, const uint8_t* is_signed, const int64_t* n_elements,
+                           int64_t count, void* const* out, int dtype, void* stream) {
+    if (count < 0 || count > 0x7FFFFFFF) return fail(FGS_ERR_INVALID_ARGUMENT, "bad tensor list");
+    if (dtype != FGS_DTYPE_F32 && dtype != FGS_DTYPE_BF16) return fail(FGS_ERR_INVALID_ARGUMENT, "moments are read as fp32 or bf16");
+    if (count > 0 && (!codes || !exponents || !is_signed || !n_elements || !out)) return fail(FGS_ERR_INVALID_ARGUMENT, "NULL argument");
+    for (int64_t i = 0; i < count; i++)
+        if (n_elements[i] > 0 && (!codes[i] || !exponents[i] || !out[i])) return fail(FGS_ERR_INVALID_ARGUMENT, "tensor pointer is NULL");
+    FGS_CUDA(fgs::launch_read_moments(codes, exponents, is_signed, n_elements, static_cast<int>(count), out, dtype, static_cast<cudaStream_t>(stream)),
+             "read moments");
     return FGS_OK;
 }
 

@@ -112,6 +112,35 @@ cudaError_t launch_adam(const AdamSegment* segs, int n_segs, cudaStream_t s);
 cudaError_t launch_dp_shard_adam(const AdamSegment* segs, int n_segs, const float* const* grads, float* const* params, int n_ranks,
                                  const float* local_params, const float* mc_grads, float* mc_params, cudaStream_t s);
 
+// adamw.cu
+enum { kDtypeF32 = 0, kDtypeBf16 = 1, kDtypeF16 = 2 };
+constexpr int kAdamwBlock = 256;     // elements of a tensor that share one exponent byte (8-bit moments)
+constexpr int kMaxAdamwHypers = 8;   // different (group, step) pairs of one launch
+constexpr int kNormPartials = 592;   // partial sums of one gradient-norm launch
+struct AdamwHyper {
+    float lr[7], decay[7];  // lr / (1 - b1^t) and 1 - lr wd per column
+    int n_lr;
+    float beta1, rest1, beta2, rest2, eps, root_rcp;
+    uint32_t step;
+};
+struct AdamwTensors {
+    int count;
+    void* const* param; const void* const* grad; void* const* m; void* const* v;
+    uint8_t* const* m_exp; uint8_t* const* v_exp; float* const* master;
+    const int64_t* n_elements; const int32_t* hyper;
+};
+struct AdamwClip {
+    const double* partials; int n_partials;  // partials == nullptr: no clipping
+    double max_norm;
+    float* norm_out;
+};
+cudaError_t launch_adamw(const AdamwTensors& A, const AdamwHyper* hypers, int dtype, bool eight, bool master, const AdamwClip& clip, cudaStream_t s);
+int grad_squares_launches(int count);
+cudaError_t launch_grad_squares(const void* const* grads, const int64_t* n_elements, const uint8_t* dtypes, int count, double* partials,
+                                int* n_partials, cudaStream_t s);
+cudaError_t launch_read_moments(const uint8_t* const* codes, const uint8_t* const* exps, const uint8_t* is_signed, const int64_t* n_elements, int count,
+                                void* const* out, int dtype, cudaStream_t s);
+
 // densification.cu
 cudaError_t launch_relocation(const float* old_opacity, const float* old_scale, const int64_t* n_samples, float* new_opacity, float* new_scale,
                               uint32_t n, cudaStream_t s);

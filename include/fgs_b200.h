@@ -194,6 +194,47 @@ int fgs_pruning_scores(const fgs_settings* settings, const fgs_frame* frame, voi
 /* fused Adam over up to 12 segments in one launch (adam/src/adam.cu:18-42 per element) */
 int fgs_adam_step(const fgs_adam_segment* segments, int n_segments, void* stream);
 
+/* AdamW with decoupled weight decay over any number of tensors of one type (no reference counterpart; its optimizer is
+ * the fused Adam above): one launch per 384 tensors (and per 8 different hyperparameter sets). Per element of tensor i:
+ *   g <- c g;  m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g g;
+ *   p <- p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+ * in fp32; c = min(1, max_norm / (norm + 1e-6)) with the norm from fgs_grad_squares, or 1. The arrays of the struct
+ * hold one entry per tensor. */
+enum { FGS_DTYPE_F32 = 0, FGS_DTYPE_BF16 = 1, FGS_DTYPE_F16 = 2 };
+#define FGS_ADAMW_BLOCK 256 /* elements that share one exponent byte where the moments are held in 8 bits */
+typedef struct {
+    double learning_rates[7];  /* cycled per element of a tensor, as fgs_adam_segment */
+    int32_t n_learning_rates;  /* 1..7 */
+    int32_t reserved;
+    double beta1, beta2, eps, weight_decay;
+    int64_t step;              /* step count after this update (>= 1) */
+} fgs_adamw_hyper;
+typedef struct {
+    int64_t count;
+    void* const* param;
+    const void* const* grad;        /* of the parameters' type */
+    void* const* exp_avg;           /* fp32, or one code byte per element */
+    void* const* exp_avg_sq;
+    uint8_t* const* exp_avg_exponent;    /* 8-bit moments: one byte per 256 elements (rounded up); NULL for 32 bits */
+    uint8_t* const* exp_avg_sq_exponent;
+    float* const* master;           /* fp32 copy of half-precision parameters, or NULL: it is updated, param gets its rounding */
+    const int64_t* n_elements;
+    const int32_t* hyper;           /* index into the hyperparameter sets */
+} fgs_adamw_tensors;
+/* `partials`: the n_partials values of fgs_grad_squares (any number of its calls, one after another in one array), or
+ * NULL for no clipping; grad_norm: one device float that receives the norm (needed with partials). */
+int fgs_adamw_step(const fgs_adamw_tensors* tensors, const fgs_adamw_hyper* hypers, int n_hypers, int dtype, int state_bits,
+                   const double* partials, int n_partials, double max_norm, float* grad_norm, void* stream);
+/* partial sums of the squared elements of `count` tensors (types may differ), in a fixed order; *n_partials receives
+ * their number, at most the capacity that fgs_grad_squares_capacity returns for the same count */
+int fgs_grad_squares_capacity(int64_t count, int* out);
+int fgs_grad_squares(const void* const* grads, const int64_t* n_elements, const uint8_t* dtypes, int64_t count, double* partials, int capacity,
+                     int* n_partials, void* stream);
+/* values of 8-bit moments (exact in bf16 and in fp32): for each of `count` arrays the codes, the exponent bytes, whether
+ * they are signed (exp_avg: 1, exp_avg_sq: 0), and the output of type dtype (FGS_DTYPE_F32 or FGS_DTYPE_BF16) */
+int fgs_adamw_read_moments(const uint8_t* const* codes, const uint8_t* const* exponents, const uint8_t* is_signed, const int64_t* n_elements,
+                           int64_t count, void* const* out, int dtype, void* stream);
+
 /* 3DGS-MCMC relocation (densification/include/kernels_mcmc.cuh:10-54): for each of n primitives duplicated into
  * n_samples[i] copies (clamped to 1..50), the new opacity keeps the composite opacity and the scales are rescaled.
  * old_opacities [n] activated, old_scales [n,3] activated; outputs new_opacities [n], new_scales [n,3]. */

@@ -1,0 +1,208 @@
+"""FusedAdamW without a GPU: what it refuses, its state handling, and the 8-bit format of its moments."""
+import copy
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import adamw as O
+
+
+def _param(n=5, dtype=torch.float32, grad=True):
+    p = torch.nn.Parameter(torch.ones(n, dtype=dtype))
+    if grad:
+        p.grad = torch.ones(n, dtype=dtype)
+    return p
+
+
+@pytest.mark.parametrize('options,match', [
+    ({'lr': -1.0}, 'learning rates'), ({'lr': [1e-3] * 8}, 'learning rates'), ({'lr': []}, 'learning rates'), ({'betas': (0.9, 1.0)}, 'betas'),
+    ({'betas': (0.9,)}, 'betas'), ({'eps': -1e-8}, 'eps'), ({'weight_decay': -0.1}, 'weight_decay'), ({'state_bits': 16}, 'state_bits'),
+    ({'max_grad_norm': 0.0}, 'max_grad_norm'), ({'max_grad_norm': float('nan')}, 'max_grad_norm'), ({'lr': float('nan')}, 'learning rates')])
+def test_options_refused(options, match):
+    import FasterGSVDACudaBackend as F
+    with pytest.raises(ValueError, match=match):
+        F.FusedAdamW([_param()], **options)
+
+
+def test_group_options_refused():
+    import FasterGSVDACudaBackend as F
+    with pytest.raises(ValueError, match='state_bits'):
+        F.FusedAdamW([{'params': [_param()], 'state_bits': 4}])
+
+
+def test_cpu_tensors_refused_and_left_alone():
+    import FasterGSVDACudaBackend as F
+    p = _param()
+    opt = F.FusedAdamW([p])
+    with pytest.raises(RuntimeError, match='CUDA'):
+        opt.step()
+    assert not opt.state and torch.equal(p.detach(), torch.ones(5))
+
+
+def test_types_refused():
+    import FasterGSVDACudaBackend as F
+    with pytest.raises(RuntimeError, match='float32, bfloat16 or float16'):
+        F.FusedAdamW([_param(dtype=torch.float64)]).step()
+
+
+def test_step_without_gradients_does_nothing():
+    import FasterGSVDACudaBackend as F
+    p = _param(grad=False)
+    opt = F.FusedAdamW([p])
+    assert opt.step() is None and not opt.state and opt.grad_norm is None
+    assert opt.step(lambda: 3.0) == 3.0
+
+
+def _pack(tensors, code=0, per=0, counts=None, device=-1):
+    from FasterGSVDACudaBackend import adamw as A
+    counts = counts if counts is not None else (ctypes.c_int64 * max(len(tensors), 1))()
+    out = (ctypes.c_uint64 * max(len(tensors), 1))()
+    return A._host.pack(tensors, 'thing', code, device, ctypes.addressof(counts), per, ctypes.addressof(out))
+
+
+def test_host_checks():
+    x = torch.zeros(4, 6)
+    with pytest.raises(RuntimeError, match='contiguous float32'):
+        _pack([x.t()])
+    with pytest.raises(RuntimeError, match='contiguous float32'):
+        _pack([x.expand(3, 4, 6)])
+    with pytest.raises(RuntimeError, match='contiguous bfloat16'):
+        _pack([x], code=1)
+    with pytest.raises(RuntimeError, match='contiguous float32'):
+        _pack([x.to_sparse()])
+    with pytest.raises(RuntimeError, match='CUDA'):
+        _pack([x])
+    with pytest.raises(TypeError):
+        _pack([3])
+    with pytest.raises(ValueError):
+        _pack([x], code=9)
+    assert _pack([]) == -1
+
+
+def test_live_sorts_by_type():
+    from FasterGSVDACudaBackend import adamw as A
+    ps = [_param(3), _param(4, torch.bfloat16), _param(5, grad=False), _param(6, torch.float16), _param(7)]
+    got = A._host.live(ps)
+    assert [(c, [p.numel() for p in a], [g.numel() for g in b]) for c, a, b in got] == [(0, [3, 7], [3, 7]), (1, [4], [4]), (2, [6], [6])]
+    assert got[0][1][1] is ps[4] and got[0][2][1].data_ptr() == ps[4].grad.data_ptr()
+    with pytest.raises(TypeError):
+        A._host.live(ps + [None])
+    with pytest.raises(TypeError):
+        A._host.live(tuple(ps))
+
+
+def _abi_call(**change):
+    from FasterGSVDACudaBackend import _lib
+    one = lambda v: (ctypes.c_uint64 * 1)(v)  # noqa: E731
+    keep = {'param': one(64), 'grad': one(64), 'exp_avg': one(64), 'exp_avg_sq': one(64), 'n_elements': (ctypes.c_int64 * 1)(4),
+            'hyper': (ctypes.c_int32 * 1)(0)}
+    keep.update(change.get('tensors', {}))
+    t = _lib.AdamwTensors(1, **{k: ctypes.addressof(v) for k, v in keep.items()})
+    h = _lib.AdamwHyper()
+    h.learning_rates[0], h.n_learning_rates, h.beta1, h.beta2, h.eps, h.weight_decay, h.step = 1e-3, 1, 0.9, 0.999, 1e-8, 0.0, 1
+    for k, v in change.get('hyper', {}).items():
+        setattr(h, k, v)
+    return _lib.check(_lib.lib.fgs_adamw_step(ctypes.byref(t), ctypes.byref(h), change.get('n_hypers', 1), change.get('dtype', 0),
+                                              change.get('bits', 32), change.get('partials'), change.get('n_partials', 0), change.get('max_norm', 0.0),
+                                              change.get('norm'), None))
+
+
+@pytest.mark.parametrize('change,match', [
+    ({'dtype': 3}, 'dtype'), ({'bits': 4}, 'state_bits'), ({'bits': 8}, 'exponents'), ({'n_hypers': 0}, 'NULL'),
+    ({'hyper': {'step': 0}}, 'step'), ({'hyper': {'n_learning_rates': 8}}, 'learning rates'), ({'hyper': {'beta1': 1.0}}, 'betas'),
+    ({'hyper': {'beta2': float('nan')}}, 'betas'), ({'hyper': {'eps': -1.0}}, 'eps'), ({'partials': 64, 'max_norm': 1.0}, 'grad_norm'),
+    ({'partials': 64, 'norm': 64}, 'max_norm'), ({'tensors': {'hyper': (ctypes.c_int32 * 1)(1)}}, 'index'),
+    ({'tensors': {'grad': (ctypes.c_uint64 * 1)(0)}}, 'NULL'), ({'tensors': {'master': (ctypes.c_uint64 * 1)(64)}}, 'master')])
+def test_c_entry_refuses(change, match):
+    """Bad arguments come back as an error status with a message, before any launch."""
+    with pytest.raises(RuntimeError, match=match):
+        _abi_call(**change)
+
+
+def test_c_entries_of_the_norm_and_the_moments_refuse():
+    from FasterGSVDACudaBackend import _lib
+    lib, check = _lib.lib, _lib.check
+    room, used = ctypes.c_int(0), ctypes.c_int(0)
+    check(lib.fgs_grad_squares_capacity(1025, ctypes.byref(room)))
+    assert room.value == 2 * 592
+    ptr, n, kind = (ctypes.c_uint64 * 1)(64), (ctypes.c_int64 * 1)(4), (ctypes.c_uint8 * 1)(3)
+    a = ctypes.addressof
+    with pytest.raises(RuntimeError, match='dtype'):
+        check(lib.fgs_grad_squares(a(ptr), a(n), a(kind), 1, 64, 592, ctypes.byref(used), None))
+    kind[0] = 0
+    with pytest.raises(RuntimeError, match='partial sums'):
+        check(lib.fgs_grad_squares(a(ptr), a(n), a(kind), 1, 64, 591, ctypes.byref(used), None))
+    with pytest.raises(RuntimeError, match='bad argument'):
+        check(lib.fgs_grad_squares(a(ptr), a(n), a(kind), -1, 64, 592, ctypes.byref(used), None))
+    with pytest.raises(RuntimeError, match='fp32 or bf16'):
+        check(lib.fgs_adamw_read_moments(a(ptr), a(ptr), a(kind), a(n), 1, a(ptr), 2, None))
+
+
+def test_state_keeps_its_types_over_save_and_load():
+    """torch's own load_state_dict would cast codes and float32 copies to the parameters' type."""
+    import FasterGSVDACudaBackend as F
+    p = _param(300, torch.bfloat16)
+    opt = F.FusedAdamW([p], state_bits=8, master_weights=True, max_grad_norm=1.0)
+    state = opt._new_state(p, 8, True)
+    state['exp_avg'].random_(0, 256)
+    opt.state[p] = {**state, 'step': 7}
+    other = F.FusedAdamW([_param(300, torch.bfloat16)], state_bits=8, master_weights=True)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    got = next(iter(other.state.values()))
+    assert got['step'] == 7 and got['exp_avg'].dtype == torch.uint8 and got['exp_avg_exponent'].numel() == 2
+    assert got['master'].dtype == torch.float32 and torch.equal(got['exp_avg'], state['exp_avg'])
+    again = copy.deepcopy(opt)
+    assert again.max_grad_norm == 1.0 and next(iter(again.state.values()))['exp_avg'].dtype == torch.uint8
+
+
+def test_code_values():
+    """Every code's value survives coding in a block of its own exponent, whatever the threshold: it needs no rounding."""
+    for signed in (True, False):
+        top = O.top_of(signed)
+        for e in (0, 1, 14, 15, 16, 31, 32, 127, 200, 253):
+            codes = np.zeros(256, np.uint8)
+            q = np.arange(1, top - 7)  # codes whose exponent is at most e
+            codes[:q.size] = q
+            if signed:
+                codes[q.size:2 * q.size] = q | 128
+            x = O.decode(codes, np.array([e], np.uint8), signed)
+            for step in (1, 2, 1000):
+                got, exp = O.encode(x, step, signed)
+                if not (x != 0).any():
+                    continue
+                if exp[0] == e:
+                    np.testing.assert_array_equal(O.decode(got, exp, signed), x)
+
+
+def test_thresholds_spread_evenly():
+    """Over 4096 steps the average of an element's coded value is the value: the counts of the two neighbouring codes
+    follow the value's place between them within half a percent of a code step (an independent threshold per step would
+    be off by 0.8 % rms)."""
+    rng = np.random.default_rng(0)
+    for signed in (True, False):
+        x = np.exp2(rng.uniform(-6, 0, 256)).astype(np.float32)
+        x[0] = 1.0
+        total = np.zeros(256)
+        for t in range(1, 4097):
+            q, e = O.encode(x, t, signed)
+            total += O.decode(q, e, signed)
+        unit = np.exp2(np.floor(np.log2(x)) - 3)
+        assert np.abs(total / 4096 - x).max() <= (0.005 * unit).max() and (np.abs(total / 4096 - x) <= 0.005 * unit).all()
+
+
+def test_small_values_are_kept():
+    """Below the smallest code the first moment is kept on average, and a nonzero second moment never becomes zero."""
+    x = np.full(256, 1e-6, np.float32)
+    x[0] = 1.0
+    total = np.zeros(256)
+    for t in range(1, 4097):
+        q, e = O.encode(x, t, True)
+        total += O.decode(q, e, True)
+    least = 1.25 * 2.0 ** -15
+    assert np.abs(total[1:] / 4096 - 1e-6).max() <= 0.005 * least
+    x = np.full(256, 1e-30, np.float32)
+    x[0], x[1] = 1.0, 0.0
+    v = O.decode(*O.encode(x, 5, False), False)
+    assert v[1] == 0.0 and (v[2:] == np.float32(1.25 * 2.0 ** -31)).all()

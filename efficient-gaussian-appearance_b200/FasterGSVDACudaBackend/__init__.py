@@ -5,12 +5,14 @@ initialize_residual_mlp, FusedAdam, update_3d_filter, relocation_adjustment and 
 from .rasterization import diff_rasterize, rasterize, update_pruning_scores, RasterizerSettings, initialize_appearance, initialize_residual_mlp
 from .adam import FusedAdam
 from .adamw import FusedAdamW
+from .embedding import embedding_lookup
 from .filter3d import update_3d_filter
 from .densification import relocation_adjustment, add_noise
 
 __all__ = [
     'diff_rasterize', 'rasterize', 'update_pruning_scores', 'RasterizerSettings', 'initialize_appearance', 'initialize_residual_mlp',
     'FusedAdam', 'FusedAdamW',
+    'embedding_lookup',
     'update_3d_filter',
     'relocation_adjustment', 'add_noise',
 ]

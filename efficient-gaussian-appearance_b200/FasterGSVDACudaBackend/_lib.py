@@ -108,6 +108,10 @@ PROTOTYPES = {
     'fgs_grad_squares_capacity': (c_int, [c_int64, _P(c_int)]),
     'fgs_grad_squares': (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, _P(c_int), c_void_p]),
     'fgs_adamw_read_moments': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p]),
+    'fgs_embedding_lookup': (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int, c_double, c_int64, c_void_p, c_void_p]),
+    'fgs_embedding_workspace_bytes': (c_int, [c_int64, c_int64, c_int64, _P(c_size_t)]),
+    'fgs_embedding_grad': (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_double, c_int64, c_void_p, c_void_p, c_size_t,
+                                   c_void_p]),
     'fgs_profile_enable': (c_int, [c_int]),
     'fgs_inference_noalloc': (c_int, [c_void_p, _P(Primitives), _P(Settings), c_void_p, c_int, c_int, c_void_p, _P(c_int64), _P(c_int64)]),
     'fgs_profile_collect': (c_int, [ctypes.c_char_p, c_size_t, _P(c_double), c_int, _P(c_int)]),

@@ -735,8 +735,8 @@ int fgs_adam_step(const fgs_adam_segment* segs, int n, void* stream) {
 
 int fgs_adamw_step(const fgs_adamw_tensors* t, const fgs_adamw_hyper* hypers, int n_hypers, int dtype, int state_bits, const double* partials,
                    int n_partials, double max_norm, float* grad_norm, void* stream) {
-    static_assert(FGS_ADAMW_BLOCK == fgs::kAdamwBlock && FGS_DTYPE_F32 == fgs::kDtypeF32 && FGS_DTYPE_BF16 == fgs::kDtypeBf16 &&
-                      FGS_DTYPE_F16 == fgs::kDtypeF16,
+    static_assert(FGS_ADAMW_BLOCK == fgs::kAdamwBlock && FGS_DTYPE_F32 == int(fgs::kDtypeF32) && FGS_DTYPE_BF16 == int(fgs::kDtypeBf16) &&
+                      FGS_DTYPE_F16 == int(fgs::kDtypeF16),
                   "C ABI constants");
     if (!t || t->count < 0 || t->count > 0x7FFFFFFF) return fail(FGS_ERR_INVALID_ARGUMENT, "bad tensor list");
     if (dtype < FGS_DTYPE_F32 || dtype > FGS_DTYPE_F16) return fail(FGS_ERR_INVALID_ARGUMENT, "unknown dtype");
@@ -822,6 +822,56 @@ int fgs_adamw_read_moments(const uint8_t* const* codes, const uint8_t* const* ex
         if (n_elements[i] > 0 && (!codes[i] || !exponents[i] || !out[i])) return fail(FGS_ERR_INVALID_ARGUMENT, "tensor pointer is NULL");
     FGS_CUDA(fgs::launch_read_moments(codes, exponents, is_signed, n_elements, static_cast<int>(count), out, dtype, static_cast<cudaStream_t>(stream)),
              "read moments");
+    return FGS_OK;
+}
+
+// checks the shape of an embedding table and its indices
+static int embedding_args(int64_t rows, int64_t width, int64_t tokens, int dtype, int index_bytes, double scale, int64_t padding, fgs::EmbeddingArgs* a) {
+    if (rows < 0 || rows > 0x7FFFFFFF || width < 0 || width > 0x7FFFFFFF) return fail(FGS_ERR_INVALID_ARGUMENT, "table dimensions out of range");
+    if (tokens < 0 || tokens > 0x7FFFFFFF) return fail(FGS_ERR_INVALID_ARGUMENT, "number of indices out of range");
+    if (dtype < FGS_DTYPE_F32 || dtype > FGS_DTYPE_F16) return fail(FGS_ERR_INVALID_ARGUMENT, "unknown dtype");
+    if (index_bytes != 4 && index_bytes != 8) return fail(FGS_ERR_INVALID_ARGUMENT, "indices have 4 or 8 bytes");
+    a->rows = rows;
+    a->width = width;
+    a->tokens = tokens;
+    a->dtype = dtype;
+    a->wide_index = index_bytes == 8;
+    a->scale = static_cast<float>(scale);
+    a->padding = padding;
+    return FGS_OK;
+}
+
+int fgs_embedding_lookup(const void* table, int64_t rows, int64_t width, int dtype, const void* indices, int64_t n_indices, int index_bytes,
+                         double scale, int64_t padding_index, void* out, void* stream) {
+    fgs::EmbeddingArgs a;
+    const int rc = embedding_args(rows, width, n_indices, dtype, index_bytes, scale, padding_index, &a);
+    if (rc != FGS_OK) return rc;
+    if (n_indices > 0 && width > 0 && (!indices || !out || (rows > 0 && !table))) return fail(FGS_ERR_INVALID_ARGUMENT, "NULL argument");
+    ProfScope p_("embedding", static_cast<cudaStream_t>(stream));
+    FGS_CUDA(fgs::launch_embedding_lookup(a, table, indices, out, static_cast<cudaStream_t>(stream)), "embedding lookup");
+    return FGS_OK;
+}
+
+int fgs_embedding_workspace_bytes(int64_t n_indices, int64_t rows, int64_t width, size_t* out) {
+    fgs::EmbeddingArgs a;
+    const int rc = embedding_args(rows, width, n_indices, FGS_DTYPE_F32, 8, 1.0, -1, &a);
+    if (rc != FGS_OK) return rc;
+    if (!out) return fail(FGS_ERR_INVALID_ARGUMENT, "NULL argument");
+    *out = fgs::embedding_workspace_bytes(n_indices, rows, width);
+    return FGS_OK;
+}
+
+int fgs_embedding_grad(const void* indices, int64_t n_indices, int index_bytes, const void* grad_out, int dtype, int64_t rows, int64_t width,
+                       double scale, int64_t padding_index, void* grad_table, void* workspace, size_t workspace_bytes, void* stream) {
+    fgs::EmbeddingArgs a;
+    const int rc = embedding_args(rows, width, n_indices, dtype, index_bytes, scale, padding_index, &a);
+    if (rc != FGS_OK) return rc;
+    if (rows > 0 && width > 0 && (!grad_table || (n_indices > 0 && (!indices || !grad_out || !workspace))))
+        return fail(FGS_ERR_INVALID_ARGUMENT, "NULL argument");
+    if (n_indices > 0 && workspace_bytes < fgs::embedding_workspace_bytes(n_indices, rows, width))
+        return fail(FGS_ERR_WORKSPACE, "embedding workspace too small");
+    ProfScope p_("embedding_grad", static_cast<cudaStream_t>(stream));
+    FGS_CUDA(fgs::launch_embedding_grad(a, indices, grad_out, grad_table, workspace, static_cast<cudaStream_t>(stream)), "embedding gradient");
     return FGS_OK;
 }
 

@@ -141,6 +141,18 @@ cudaError_t launch_grad_squares(const void* const* grads, const int64_t* n_eleme
 cudaError_t launch_read_moments(const uint8_t* const* codes, const uint8_t* const* exps, const uint8_t* is_signed, const int64_t* n_elements, int count,
                                 void* const* out, int dtype, cudaStream_t s);
 
+// embedding.cu
+struct EmbeddingArgs {
+    int64_t rows, width, tokens;  // table [rows, width]
+    int dtype;
+    bool wide_index;              // int64 indices (else int32)
+    float scale;
+    int64_t padding;              // index that stands for no row (-1: only negative ones do)
+};
+cudaError_t launch_embedding_lookup(const EmbeddingArgs& a, const void* table, const void* index, void* out, cudaStream_t s);
+size_t embedding_workspace_bytes(int64_t tokens, int64_t rows, int64_t width);
+cudaError_t launch_embedding_grad(const EmbeddingArgs& a, const void* index, const void* g, void* grad, void* ws, cudaStream_t s);
+
 // densification.cu
 cudaError_t launch_relocation(const float* old_opacity, const float* old_scale, const int64_t* n_samples, float* new_opacity, float* new_scale,
                               uint32_t n, cudaStream_t s);

@@ -235,6 +235,18 @@ int fgs_grad_squares(const void* const* grads, const int64_t* n_elements, const 
 int fgs_adamw_read_moments(const uint8_t* const* codes, const uint8_t* const* exponents, const uint8_t* is_signed, const int64_t* n_elements,
                            int64_t count, void* const* out, int dtype, void* stream);
 
+/* Embedding lookup with scaling (no reference counterpart): out[t] = scale * table[indices[t]] for a table [rows, width]
+ * and n_indices indices of 4 or 8 bytes (signed), rows contiguous, out [n_indices, width]. A negative index, or
+ * padding_index, stands for no row and gives zeros (pass -1 for no padding index); an index past the table gives NaN. */
+int fgs_embedding_lookup(const void* table, int64_t rows, int64_t width, int dtype, const void* indices, int64_t n_indices, int index_bytes,
+                         double scale, int64_t padding_index, void* out, void* stream);
+/* Its gradient: grad_table[v] = scale * sum of grad_out[t] over the t with indices[t] = v, in fp32, rounded once; rows
+ * without an index get zeros (grad_table is written whole). The indices are sorted, so the order of the sums, and with
+ * it every bit of the result, depends only on the inputs. */
+int fgs_embedding_workspace_bytes(int64_t n_indices, int64_t rows, int64_t width, size_t* out);
+int fgs_embedding_grad(const void* indices, int64_t n_indices, int index_bytes, const void* grad_out, int dtype, int64_t rows, int64_t width,
+                       double scale, int64_t padding_index, void* grad_table, void* workspace, size_t workspace_bytes, void* stream);
+
 /* 3DGS-MCMC relocation (densification/include/kernels_mcmc.cuh:10-54): for each of n primitives duplicated into
  * n_samples[i] copies (clamped to 1..50), the new opacity keeps the composite opacity and the scales are rescaled.
  * old_opacities [n] activated, old_scales [n,3] activated; outputs new_opacities [n], new_scales [n,3]. */

@@ -1,0 +1,244 @@
+"""embedding_lookup and its gradient on the GPU against the formula in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E32 = 2.0 ** -24  # half a float32 step, relative
+HALF_STEP = {torch.float32: E32, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+SMALLEST = {torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _check_rows(out, table, idx, scale, padding=None):
+    """The scale's conversion and the product: two float32 roundings, then the type's own."""
+    t, i, o = _np(table).reshape(table.shape[0], -1), idx.cpu().numpy().reshape(-1), _np(out)
+    o = o.reshape(i.size, t.shape[1])
+    none = (i < 0) | (i == (padding if padding is not None else -1))
+    bad = i >= t.shape[0]
+    assert (o[none] == 0).all() and np.isnan(o[bad & ~none]).all()
+    live = ~none & ~bad
+    want = scale * t[i[live]]
+    err = np.abs(o[live] - want)
+    assert (err <= (2.01 * E32 + (0 if out.dtype == torch.float32 else 1.01 * HALF_STEP[out.dtype])) * np.abs(want) + SMALLEST[out.dtype]).all()
+
+
+def _check_grad(grad, g, idx, scale, padding=None):
+    """A row of k tokens: at most k - 1 float32 additions in any order, each off by half a step of a partial sum, which is
+    at most the sum of the magnitudes; then the scale's conversion, the product, and the type's own rounding."""
+    rows = grad.shape[0]
+    i = idx.cpu().numpy().reshape(-1)
+    g = _np(g).reshape(i.size, -1)
+    live = (i >= 0) & (i < rows) & (i != (padding if padding is not None else -1))
+    want, size, count = np.zeros((rows, g.shape[1])), np.zeros((rows, g.shape[1])), np.zeros(rows)
+    np.add.at(want, i[live], g[live])
+    np.add.at(size, i[live], np.abs(g[live]))
+    np.add.at(count, i[live], 1)
+    got = _np(grad).reshape(rows, -1)
+    assert (got[count == 0] == 0).all()
+    err = np.abs(got - scale * want)
+    tol = 1.01 * abs(scale) * E32 * np.maximum(count - 1, 0)[:, None] * size
+    tol = tol + (2.01 * E32 + (0 if grad.dtype == torch.float32 else 1.01 * HALF_STEP[grad.dtype])) * (np.abs(scale * want) + tol) + SMALLEST[grad.dtype]
+    assert (err <= tol).all(), float((err - tol).max())
+
+
+def _inputs(cuda, rows, width, tokens, dtype, kind, index_type, seed=0):
+    r = torch.Generator().manual_seed(seed)
+    table = (torch.randn(rows, *width, generator=r) if isinstance(width, tuple) else torch.randn(rows, width, generator=r)).to(dtype).to(cuda)
+    if kind == 'even':
+        idx = torch.randint(0, rows, (tokens,), generator=r)
+    elif kind == 'one':
+        idx = torch.full((tokens,), rows - 1)
+    elif kind == 'skewed':
+        idx = (torch.rand(tokens, generator=r) ** 4 * rows).long().clamp(max=rows - 1)
+    else:  # sorted runs, with gaps
+        idx = torch.arange(tokens) * rows // max(tokens, 1) // 3 * 3
+        idx = idx.clamp(max=rows - 1)
+    absent = torch.rand(tokens, generator=r)
+    if kind != 'one':
+        idx = torch.where(absent < 0.1, -1, idx)
+        idx = torch.where(absent > 0.97, rows + (absent * 100).long(), idx)
+    g = torch.randn(tokens, *(width if isinstance(width, tuple) else (width,)), generator=r).to(dtype).to(cuda)
+    return table, idx.to(index_type).to(cuda), g
+
+
+# rows, width, tokens: one of each; odd and even widths around the access and lane counts; rows that cross chunks;
+# more chunks than one joining CTA looks at; a row longer than one CTA's part
+SIZES = [(1, 1, 1), (5, 1, 7), (3, 2, 100), (1000, 3, 1), (17, 4, 33), (9, 5, 2000), (300, 32, 5000), (4096, 45, 3000), (40, 64, 4097), (2, 127, 640),
+         (700, 128, 257), (3, 129, 1000), (60, 1000, 300), (11, 4099, 50), (70_000, 8, 9000), (4, (15, 3), 777), (6, 8200, 9)]
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('kind', ['even', 'one', 'skewed', 'runs'])
+@pytest.mark.parametrize('size', SIZES, ids=[str(s) for s in SIZES])
+def test_lookup_and_gradient(cuda, size, kind, dtype):
+    import FasterGSVDACudaBackend as F
+    rows, width, tokens = size
+    index_type = torch.int64 if tokens % 2 else torch.int32
+    table, idx, g = _inputs(cuda, rows, width, tokens, dtype, kind, index_type)
+    scale = 1.0 if kind == 'one' else 5.7
+    table.requires_grad_(True)
+    out = F.embedding_lookup(table, idx, scale=scale)
+    assert out.shape == idx.shape + table.shape[1:] and out.dtype == dtype
+    _check_rows(out, table, idx, scale)
+    out.backward(g)
+    assert table.grad.shape == table.shape and table.grad.dtype == dtype
+    _check_grad(table.grad, g, idx, scale)
+    with torch.no_grad():
+        assert torch.equal(F.embedding_lookup(table, idx, scale=scale).nan_to_num(9.0), out.nan_to_num(9.0))
+
+
+def test_many_tokens_of_few_rows(cuda):
+    """Rows over hundreds of chunks, summed by the joining kernel."""
+    import FasterGSVDACudaBackend as F
+    for rows, width in ((1, 8), (3, 33), (37, 16)):
+        table, idx, g = _inputs(cuda, rows, width, 300_001, torch.float32, 'even', torch.int32)
+        table.requires_grad_(True)
+        F.embedding_lookup(table, idx).backward(g)
+        _check_grad(table.grad, g, idx, 1.0)
+
+
+def test_index_shapes_padding_and_strides(cuda):
+    import FasterGSVDACudaBackend as F
+    table, idx, g = _inputs(cuda, 50, 24, 210, torch.bfloat16, 'even', torch.int64)
+    idx = idx.clamp(max=49).view(6, 35)
+    table.requires_grad_(True)
+    out = F.embedding_lookup(table, idx.t(), scale=-0.5, padding_index=7)
+    assert out.shape == (35, 6, 24)
+    _check_rows(out, table, idx.t().contiguous(), -0.5, padding=7)
+    # a gradient in another order, and one that is broadcast
+    go = g.view(6, 35, 24).transpose(0, 1)
+    out.backward(go, retain_graph=True)
+    _check_grad(table.grad, go.contiguous(), idx.t().contiguous(), -0.5, padding=7)
+    table.grad = None
+    out.sum().backward()
+    _check_grad(table.grad, torch.ones(35, 6, 24, dtype=torch.bfloat16), idx.t().contiguous(), -0.5, padding=7)
+    single = F.embedding_lookup(table.detach(), torch.tensor(3, device=cuda))
+    assert single.shape == (24,) and torch.equal(single, table.detach()[3])
+
+
+def test_odd_addresses(cuda):
+    """A table and gradients that start one element past an aligned address take the narrow accesses."""
+    import FasterGSVDACudaBackend as F
+    for dtype in DTYPES:
+        base = torch.randn(1 + 30 * 16, device=cuda).to(dtype)
+        table = base[1:].view(30, 16).requires_grad_(True)
+        idx = torch.randint(0, 30, (99,), device=cuda)
+        out = F.embedding_lookup(table, idx, scale=2.0)
+        _check_rows(out, table, idx, 2.0)
+        g = torch.randn(1 + 99 * 16, device=cuda).to(dtype)[1:].view(99, 16)
+        grad, = torch.autograd.grad(out, table, g)
+        _check_grad(grad, g, idx, 2.0)
+
+
+def test_empty(cuda):
+    import FasterGSVDACudaBackend as F
+    table = torch.randn(4, 3, device=cuda, requires_grad=True)
+    none = torch.empty(0, dtype=torch.int64, device=cuda)
+    out = F.embedding_lookup(table, none)
+    assert out.shape == (0, 3)
+    out.sum().backward()
+    assert not table.grad.any()
+    table.grad = None
+    F.embedding_lookup(table, torch.full((5,), -1, device=cuda)).sum().backward()
+    assert not table.grad.any()
+    empty = torch.empty(0, 3, device=cuda, requires_grad=True)
+    out = F.embedding_lookup(empty, torch.tensor([-1, 0], device=cuda))
+    assert (out[0] == 0).all() and out[1].isnan().all()
+    out.sum().backward()
+    assert empty.grad.shape == (0, 3)
+    assert F.embedding_lookup(torch.empty(4, 0, device=cuda), torch.tensor([1], device=cuda)).shape == (1, 0)
+    wide = torch.empty(4, 0, device=cuda, requires_grad=True)
+    F.embedding_lookup(wide, torch.tensor([1], device=cuda)).sum().backward()
+
+
+def test_gradient_against_differences(cuda):
+    import FasterGSVDACudaBackend as F
+    r = torch.Generator().manual_seed(3)
+    table = torch.randn(6, 5, generator=r).to(cuda).requires_grad_(True)
+    idx = torch.tensor([0, 3, 3, -1, 5, 3, 0], device=cuda)
+    w = torch.randn(7, 5, generator=r).to(cuda)
+    loss = lambda t: (F.embedding_lookup(t, idx, scale=1.5).double().square() * w.double()).sum()  # noqa: E731
+    loss(table).backward()
+    step = 2.0 ** -6  # the loss is quadratic: central differences are exact up to the rounding of the rows
+    for i in range(6):
+        for j in range(5):
+            d = torch.zeros_like(table)
+            d[i, j] = step
+            with torch.no_grad():
+                got = float(loss(table + d) - loss(table - d)) / (2 * step)
+            # each of the 4 values squared per entry: rows off by 3 roundings of at most 8, over 2 * step
+            assert abs(got - float(table.grad[i, j])) <= 4 * 2 * 3 * E32 * 64 * float(w.abs().max()) / step
+
+
+def test_same_bits_on_any_stream(cuda):
+    import FasterGSVDACudaBackend as F
+    table, idx, g = _inputs(cuda, 90, 40, 20_000, torch.float32, 'skewed', torch.int64)
+    table.requires_grad_(True)
+    first, = torch.autograd.grad(F.embedding_lookup(table, idx), table, g)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    grads = []
+    for s in streams:  # several calls at once, each with its own workspace
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            grads.append(torch.autograd.grad(F.embedding_lookup(table, idx), table, g)[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, x) for x in grads)
+
+
+def test_captured_and_replayed(cuda):
+    """Both directions in one graph, replayed on other indices and gradients; a second graph lives beside it."""
+    import FasterGSVDACudaBackend as F
+    table, idx, g = _inputs(cuda, 200, 48, 5000, torch.bfloat16, 'even', torch.int64)
+    table.requires_grad_(True)
+
+    def both():
+        out = F.embedding_lookup(table, idx, scale=3.0)
+        return out.detach(), torch.autograd.grad(out, table, g)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = both()
+        graphs.append((graph, outs))
+    for seed, kind in ((1, 'one'), (2, 'skewed')):
+        t2, i2, g2 = _inputs(cuda, 200, 48, 5000, torch.bfloat16, kind, torch.int64, seed)
+        idx.copy_(i2)
+        g.copy_(g2)
+        with torch.no_grad():
+            table.copy_(t2)
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, (out, grad) in graphs:
+            _check_rows(out, table, idx, 3.0)
+            _check_grad(grad, g, idx, 3.0)
+
+
+def test_refusals(cuda):
+    import FasterGSVDACudaBackend as F
+    table, idx = torch.randn(8, 4, device=cuda), torch.zeros(3, dtype=torch.int64, device=cuda)
+    for bad in (table.t(), table.double(), table.cpu(), torch.tensor(1.0, device=cuda), table.int()):
+        with pytest.raises(RuntimeError, match='table'):
+            F.embedding_lookup(bad, idx)
+    for bad in (idx.cpu(), idx.float(), idx.short(), idx.bool()):
+        with pytest.raises(RuntimeError, match='indices'):
+            F.embedding_lookup(table, bad)
+    for bad in (8, -1):
+        with pytest.raises(ValueError, match='padding_index'):
+            F.embedding_lookup(table, idx, padding_index=bad)
+    table.requires_grad_(True)
+    grad, = torch.autograd.grad(F.embedding_lookup(table, idx).sum(), table, create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()

@@ -4,6 +4,7 @@ The library is the only compute path: if it is missing, importing this module ra
 no CPU fallback.
 """
 import ctypes
+import importlib.util
 import os
 from pathlib import Path
 
@@ -126,6 +127,26 @@ for _name, (_res, _args) in PROTOTYPES.items():
     _fn = getattr(lib, _name)
     _fn.restype = _res
     _fn.argtypes = _args
+
+
+_HOST_PATH = _LIB_PATH.with_name('_fgs_host.so')
+
+
+def _load_host():
+    """The module of csrc/host.cpp (the host side of the many-tensor operators), bound to this library's entry points."""
+    if not _HOST_PATH.exists():
+        raise ImportError(f'{_HOST_PATH} not found; build it with `python efficient-gaussian-appearance_b200/build.py` (or __graft_entry__.build())')
+    import torch  # noqa: F401  (its libraries have to be loaded first)
+    spec = importlib.util.spec_from_file_location('_fgs_host', _HOST_PATH)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    module.bind(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
+        'fgs_last_error', 'fgs_adamw_step', 'fgs_grad_squares_capacity', 'fgs_grad_squares', 'fgs_adamw_read_moments', 'fgs_embedding_lookup',
+        'fgs_embedding_workspace_bytes', 'fgs_embedding_grad')))
+    return module
+
+
+host = _load_host()
 
 
 def check(rc: int) -> None:

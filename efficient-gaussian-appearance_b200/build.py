@@ -70,13 +70,14 @@ def _compile_host() -> Path:
     from torch.utils import cpp_extension
     src = CSRC / 'host.cpp'
     stamp = BUILD / 'host.stamp'
-    key = torch.__version__ + sys.version + hashlib.sha256(src.read_bytes()).hexdigest()
+    header = HERE.parent / 'include' / 'fgs_b200.h'
+    key = torch.__version__ + sys.version + hashlib.sha256(src.read_bytes() + header.read_bytes()).hexdigest()
     if HOST_LIB.exists() and stamp.exists() and stamp.read_text() == key:
         return HOST_LIB
     libs = [p for p in cpp_extension.library_paths() if Path(p).exists()]
     cmd = [CXX, '-O2', '-std=c++17', '-fPIC', '-shared', f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}',
-           *[f'-I{p}' for p in cpp_extension.include_paths()], f"-I{sysconfig.get_paths()['include']}", str(src), '-o', str(HOST_LIB),
-           *[f'-L{p}' for p in libs], '-lc10', '-ltorch_cpu', '-ltorch_python']
+           *[f'-I{p}' for p in (*cpp_extension.include_paths(), Path(NVCC).parent.parent / 'include')], f"-I{sysconfig.get_paths()['include']}", str(src), '-o', str(HOST_LIB),
+           *[f'-L{p}' for p in libs], '-lc10', '-lc10_cuda', '-ltorch_cpu', '-ltorch_python']
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f'{CXX} failed for {src.name}:\n{res.stdout}\n{res.stderr}')

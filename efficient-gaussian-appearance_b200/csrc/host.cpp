@@ -1,114 +1,452 @@
-// Host side of the many-tensor operators (Python module _fgs_host): reads gradients, addresses and sizes of tensor
-// lists and checks them, at about 15 ns per tensor where the same through Python attributes takes about 75 ns for each
-// of the five things that are checked. No compute and no CUDA calls; the lists are read anew at every call.
+// Host side of the many-tensor operators and of the embedding lookup (Python module _fgs_host): reads tensors, checks
+// them and calls the C entry points of libfgs_b200.so, whose addresses `bind` receives. A step over 300 tensors reads
+// and checks some 2000 tensor properties, at about 75 ns each through Python attributes; the lookup's backward runs on
+// autograd's thread without the interpreter. Everything is read anew at every call.
 #include <Python.h>
 #include <exception>
+#include <stdexcept>
+#include <string>
+#include <vector>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include "../../include/fgs_b200.h"
 
 namespace {
 
+constexpr int64_t kBlock = FGS_ADAMW_BLOCK;
+
+struct Entries {
+    decltype(&fgs_last_error) last_error;
+    decltype(&fgs_adamw_step) adamw_step;
+    decltype(&fgs_grad_squares_capacity) grad_squares_capacity;
+    decltype(&fgs_grad_squares) grad_squares;
+    decltype(&fgs_adamw_read_moments) read_moments;
+    decltype(&fgs_embedding_lookup) lookup;
+    decltype(&fgs_embedding_workspace_bytes) workspace_bytes;
+    decltype(&fgs_embedding_grad) lookup_grad;
+} lib;
+
+[[noreturn]] void refuse(const std::string& why) { throw std::runtime_error(why); }
+
+void check(int rc) {
+    if (rc != FGS_OK) refuse(lib.last_error());
+}
+
+// Python objects that belong to this scope
+struct Ref {
+    PyObject* p;
+    explicit Ref(PyObject* o = nullptr) : p(o) {}
+    Ref(const Ref&) = delete;
+    ~Ref() { Py_XDECREF(p); }
+};
+
+struct PythonError {};  // the interpreter's error is set
+
+PyObject* must(PyObject* o) {
+    if (!o) throw PythonError();
+    return o;
+}
+
+// Runs f() for Python: C++ exceptions become Python ones.
+template <typename F>
+PyObject* guarded(F&& f) {
+    try {
+        return f();
+    } catch (const PythonError&) {
+        return nullptr;
+    } catch (const c10::Error& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
+    } catch (const std::length_error& e) {
+        PyErr_SetString(PyExc_ValueError, e.what());
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    }
+    return nullptr;
+}
+
+enum { kU8 = 3 };
 const char* kTypeNames[] = {"float32", "bfloat16", "float16", "uint8"};
 
 int type_code(const at::Tensor& t) {
     switch (t.scalar_type()) {
-        case at::kFloat: return 0;
-        case at::kBFloat16: return 1;
-        case at::kHalf: return 2;
-        case at::kByte: return 3;
+        case at::kFloat: return FGS_DTYPE_F32;
+        case at::kBFloat16: return FGS_DTYPE_BF16;
+        case at::kHalf: return FGS_DTYPE_F16;
+        case at::kByte: return kU8;
         default: return -1;
     }
 }
 
-// live(params) -> [(type code, parameters, gradients), ...]: the parameters that have a gradient, by type
-PyObject* live(PyObject*, PyObject* arg) {
-    if (!PyList_Check(arg)) return PyErr_Format(PyExc_TypeError, "a list of parameters is needed");
-    PyObject* lists[3][2] = {};
-    PyObject* out = nullptr;
-    try {
-        const Py_ssize_t n = PyList_GET_SIZE(arg);
-        for (Py_ssize_t i = 0; i < n; i++) {
-            PyObject* o = PyList_GET_ITEM(arg, i);
-            if (!THPVariable_Check(o)) {
-                PyErr_SetString(PyExc_TypeError, "parameters must be tensors");
-                goto done;
-            }
-            const at::Tensor& p = THPVariable_Unpack(o);
-            const at::Tensor& g = p.grad();
-            if (!g.defined()) continue;
-            const int c = type_code(p);
-            if (c < 0 || c > 2) {
-                PyErr_SetString(PyExc_RuntimeError, "parameters must be float32, bfloat16 or float16 tensors");
-                goto done;
-            }
-            for (int k = 0; k < 2; k++)
-                if (!lists[c][k] && !(lists[c][k] = PyList_New(0))) goto done;
-            PyObject* go = THPVariable_Wrap(g);
-            if (!go) goto done;
-            const bool bad = PyList_Append(lists[c][0], o) != 0 || PyList_Append(lists[c][1], go) != 0;
-            Py_DECREF(go);
-            if (bad) goto done;
-        }
-        out = PyList_New(0);
-        for (int c = 0; out && c < 3; c++) {
-            if (!lists[c][0]) continue;
-            PyObject* t = Py_BuildValue("(iOO)", c, lists[c][0], lists[c][1]);
-            if (!t || PyList_Append(out, t) != 0) Py_CLEAR(out);
-            Py_XDECREF(t);
-        }
-    } catch (const std::exception& e) {
-        Py_CLEAR(out);
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+// data address of a contiguous CUDA tensor of the given type and element count on `device` (-1: any, and sets it)
+void* address(const at::Tensor& t, const char* name, int code, int64_t count, int& device) {
+    if (t.layout() != at::kStrided || type_code(t) != code || !t.is_contiguous())
+        refuse(std::string(name) + " must be a contiguous " + kTypeNames[code] + " tensor");
+    if (!t.is_cuda()) refuse(std::string(name) + " must be a CUDA tensor");
+    if (device < 0) device = t.get_device();
+    if (t.get_device() != device) refuse(std::string(name) + " must be on device cuda:" + std::to_string(device) + " like the others");
+    if (t.numel() != count)
+        refuse(std::string(name) + " has " + std::to_string(t.numel()) + " elements, expected " + std::to_string(count));
+    return t.data_ptr();
+}
+
+const at::Tensor& tensor_of(PyObject* o, const char* name) {
+    if (!o || !THPVariable_Check(o)) refuse(std::string(name) + " must be a tensor");
+    return THPVariable_Unpack(o);
+}
+
+// names of the state and of the group options, made once
+struct Names {
+    PyObject *params, *lr, *betas, *eps, *weight_decay, *state_bits, *master_weights, *step, *exp_avg, *exp_avg_sq, *exp_avg_exponent,
+        *exp_avg_sq_exponent, *master;
+} names;
+
+const at::Tensor& state_tensor(PyObject* state, PyObject* key) {
+    PyObject* o = PyDict_GetItemWithError(state, key);
+    const char* name = PyUnicode_AsUTF8(key);
+    if (!o) refuse(std::string("the optimizer state has no ") + name + ": it was made with other state_bits or master_weights");
+    return tensor_of(o, name);
+}
+
+double number(PyObject* o) {
+    const double x = PyFloat_AsDouble(must(o));
+    if (x == -1.0 && PyErr_Occurred()) throw PythonError();
+    return x;
+}
+
+PyObject* option(PyObject* group, PyObject* key) {
+    PyObject* o = PyDict_GetItemWithError(group, key);
+    if (!o) refuse(std::string("a parameter group has no ") + PyUnicode_AsUTF8(key));
+    return o;
+}
+
+fgs_adamw_hyper hyper_of(PyObject* group, int64_t step) {
+    fgs_adamw_hyper h{};
+    PyObject* lr = option(group, names.lr);
+    if (PyList_Check(lr) || PyTuple_Check(lr)) {
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(lr);
+        if (n < 1 || n > 7) refuse("between 1 and 7 learning rates are supported");
+        for (Py_ssize_t i = 0; i < n; i++) h.learning_rates[i] = number(PySequence_Fast_GET_ITEM(lr, i));
+        h.n_learning_rates = static_cast<int32_t>(n);
+    } else {
+        h.learning_rates[0] = number(lr);
+        h.n_learning_rates = 1;
     }
-done:
-    for (auto& pair : lists)
-        for (PyObject* l : pair) Py_XDECREF(l);
+    Ref b1(must(PySequence_GetItem(option(group, names.betas), 0))), b2(must(PySequence_GetItem(option(group, names.betas), 1)));
+    h.beta1 = number(b1.p);
+    h.beta2 = number(b2.p);
+    h.eps = number(option(group, names.eps));
+    h.weight_decay = number(option(group, names.weight_decay));
+    h.step = step;
+    return h;
+}
+
+// tensors of one call of the kernel: one type, one kind of state
+struct Job {
+    std::vector<void*> param, exp_avg, exp_avg_sq;
+    std::vector<const void*> grad;
+    std::vector<uint8_t*> exp_avg_exponent, exp_avg_sq_exponent;
+    std::vector<float*> master;
+    std::vector<int64_t> count;
+    std::vector<int32_t> hyper;
+};
+
+// adamw_step(state dict, parameter groups, new_state(parameter, bits, master), max_grad_norm or None) -> the norm or None
+PyObject* adamw_step(PyObject*, PyObject* args) {
+    PyObject *all_state, *groups, *new_state, *limit;
+    if (!PyArg_ParseTuple(args, "O!O!OO", &PyDict_Type, &all_state, &PyList_Type, &groups, &new_state, &limit)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const double max_norm = limit == Py_None ? 0.0 : number(limit);
+        if (limit != Py_None && !(max_norm > 0.0)) refuse("max_grad_norm must be positive (or None for no clipping)");
+        Job jobs[3][2][2];
+        std::vector<fgs_adamw_hyper> hypers;
+        std::vector<Py_ssize_t> hyper_group;
+        std::vector<std::pair<PyObject*, int64_t>> counted;  // states and their new step counts (borrowed)
+        Ref fresh(must(PyList_New(0)));                      // parameter, state, parameter, state ...
+        int device = -1;
+        bool any = false;
+        for (Py_ssize_t gi = 0; gi < PyList_GET_SIZE(groups); gi++) {
+            PyObject* group = PyList_GET_ITEM(groups, gi);
+            if (!PyDict_Check(group)) refuse("parameter groups must be dicts");
+            PyObject* params = option(group, names.params);
+            if (!PyList_Check(params)) refuse("a group's parameters must be a list");
+            const long bits = PyLong_AsLong(option(group, names.state_bits));
+            if (bits != 8 && bits != 32) {
+                PyErr_Clear();
+                refuse("state_bits must be 8 or 32");
+            }
+            const int wants_master = PyObject_IsTrue(option(group, names.master_weights));
+            for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); i++) {
+                PyObject* o = PyList_GET_ITEM(params, i);
+                const at::Tensor& p = tensor_of(o, "a parameter");
+                const at::Tensor& g = p.grad();
+                if (!g.defined()) continue;
+                any = true;
+                const int code = type_code(p);
+                if (code < 0 || code > FGS_DTYPE_F16) refuse("parameters must be float32, bfloat16 or float16 tensors");
+                const bool eight = bits == 8, master = wants_master && code != FGS_DTYPE_F32;
+                Job& job = jobs[code][eight][master];
+                const int64_t n = p.numel();
+                job.param.push_back(address(p, "a parameter", code, n, device));
+                job.grad.push_back(address(g, "a gradient", code, n, device));
+                PyObject* state = PyDict_GetItemWithError(all_state, o);
+                if (!state && PyErr_Occurred()) throw PythonError();
+                if (!state || (PyDict_Check(state) && PyDict_GET_SIZE(state) == 0)) {
+                    Ref made(must(PyObject_CallFunction(new_state, "Oii", o, static_cast<int>(bits), static_cast<int>(master))));
+                    if (PyList_Append(fresh.p, o) || PyList_Append(fresh.p, made.p)) throw PythonError();
+                    state = made.p;  // the list keeps it
+                }
+                if (!PyDict_Check(state)) refuse("the optimizer state of a parameter must be a dict");
+                PyObject* was = PyDict_GetItemWithError(state, names.step);
+                if (!was) refuse("the optimizer state has no step");
+                Ref whole(must(PyNumber_Long(was)));
+                const int64_t t = PyLong_AsLongLong(whole.p) + 1;
+                if (t < 1) {
+                    PyErr_Clear();
+                    refuse("step must not be negative");
+                }
+                const int kind = eight ? kU8 : FGS_DTYPE_F32;
+                job.exp_avg.push_back(address(state_tensor(state, names.exp_avg), "exp_avg", kind, n, device));
+                job.exp_avg_sq.push_back(address(state_tensor(state, names.exp_avg_sq), "exp_avg_sq", kind, n, device));
+                if (eight) {
+                    const int64_t blocks = (n + kBlock - 1) / kBlock;
+                    job.exp_avg_exponent.push_back(
+                        static_cast<uint8_t*>(address(state_tensor(state, names.exp_avg_exponent), "exp_avg_exponent", kU8, blocks, device)));
+                    job.exp_avg_sq_exponent.push_back(
+                        static_cast<uint8_t*>(address(state_tensor(state, names.exp_avg_sq_exponent), "exp_avg_sq_exponent", kU8, blocks, device)));
+                }
+                if (master) job.master.push_back(static_cast<float*>(address(state_tensor(state, names.master), "master", FGS_DTYPE_F32, n, device)));
+                job.count.push_back(n);
+                size_t h = hypers.size();
+                while (h > 0 && hyper_group[h - 1] == gi && hypers[h - 1].step != t) h--;
+                if (h == 0 || hyper_group[h - 1] != gi) {
+                    hypers.push_back(hyper_of(group, t));
+                    hyper_group.push_back(gi);
+                    h = hypers.size();
+                }
+                job.hyper.push_back(static_cast<int32_t>(h - 1));
+                counted.emplace_back(state, t);
+            }
+        }
+        if (!any) Py_RETURN_NONE;
+        const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+        if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+            refuse("FusedAdamW.step cannot be captured into a CUDA graph: its step count is a host value");
+        const cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
+        at::Tensor norm, partials;
+        int n_partials = 0;
+        if (max_norm > 0.0) {
+            const auto on = at::TensorOptions().device(at::kCUDA, static_cast<c10::DeviceIndex>(device));
+            int room = 0;
+            for (auto& by_type : jobs)
+                for (auto& by_bits : by_type)
+                    for (Job& j : by_bits) {
+                        int need = 0;
+                        check(lib.grad_squares_capacity(static_cast<int64_t>(j.count.size()), &need));
+                        room += need;
+                    }
+            partials = at::empty({room}, on.dtype(at::kDouble));
+            norm = at::empty({}, on.dtype(at::kFloat));
+            double* to = partials.data_ptr<double>();
+            for (int code = 0; code < 3; code++)
+                for (auto& by_bits : jobs[code])
+                    for (Job& j : by_bits) {
+                        if (j.count.empty()) continue;
+                        int used = 0;
+                        const std::vector<uint8_t> types(j.count.size(), static_cast<uint8_t>(code));
+                        check(lib.grad_squares(j.grad.data(), j.count.data(), types.data(), static_cast<int64_t>(j.count.size()), to + n_partials,
+                                               room - n_partials, &used, stream));
+                        n_partials += used;
+                    }
+            if (n_partials == 0) norm.zero_();  // empty gradients only: no kernel writes the norm
+        }
+        for (int code = 0; code < 3; code++)
+            for (int eight = 0; eight < 2; eight++)
+                for (int master = 0; master < 2; master++) {
+                    Job& j = jobs[code][eight][master];
+                    if (j.count.empty()) continue;
+                    const fgs_adamw_tensors t{static_cast<int64_t>(j.count.size()), j.param.data(), j.grad.data(), j.exp_avg.data(), j.exp_avg_sq.data(),
+                                              eight ? j.exp_avg_exponent.data() : nullptr, eight ? j.exp_avg_sq_exponent.data() : nullptr,
+                                              master ? j.master.data() : nullptr, j.count.data(), j.hyper.data()};
+                    check(lib.adamw_step(&t, hypers.data(), static_cast<int>(hypers.size()), code, eight ? 8 : 32,
+                                         n_partials ? partials.data_ptr<double>() : nullptr, n_partials, max_norm,
+                                         n_partials ? norm.data_ptr<float>() : nullptr, stream));
+                }
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(fresh.p); i += 2)
+            if (PyDict_SetItem(all_state, PyList_GET_ITEM(fresh.p, i), PyList_GET_ITEM(fresh.p, i + 1))) throw PythonError();
+        for (const auto& c : counted) {
+            Ref t(must(PyLong_FromLongLong(c.second)));
+            if (PyDict_SetItem(c.first, names.step, t.p)) throw PythonError();
+        }
+        if (!norm.defined()) Py_RETURN_NONE;
+        return THPVariable_Wrap(norm);
+    });
+}
+
+// read_moments(state dict, parameters, outputs of exp_avg, outputs of exp_avg_sq)
+PyObject* read_moments(PyObject*, PyObject* args) {
+    PyObject *all_state, *params, *outs[2];
+    if (!PyArg_ParseTuple(args, "O!O!O!O!", &PyDict_Type, &all_state, &PyList_Type, &params, &PyList_Type, &outs[0], &PyList_Type, &outs[1]))
+        return nullptr;
+    return guarded([&]() -> PyObject* {
+        const Py_ssize_t n = PyList_GET_SIZE(params);
+        if (PyList_GET_SIZE(outs[0]) != n || PyList_GET_SIZE(outs[1]) != n) refuse("one tensor per parameter is needed");
+        std::vector<const uint8_t*> codes, exponents;
+        std::vector<void*> to;
+        std::vector<uint8_t> is_signed;
+        std::vector<int64_t> counts;
+        int device = -1, out_code = -1;
+        std::vector<std::pair<at::Tensor, at::Tensor>> copies;  // moments in 32 bits; an undefined source: zeros
+        for (Py_ssize_t i = 0; i < n; i++) {
+            PyObject* o = PyList_GET_ITEM(params, i);
+            const int64_t count = tensor_of(o, "a parameter").numel();
+            PyObject* state = PyDict_GetItemWithError(all_state, o);
+            if (!state && PyErr_Occurred()) throw PythonError();
+            const bool none = !state || !PyDict_Check(state) || PyDict_GET_SIZE(state) == 0;
+            for (int k = 0; k < 2; k++) {
+                const at::Tensor& out = tensor_of(PyList_GET_ITEM(outs[k], i), "an output");
+                if (out_code < 0) out_code = type_code(out);
+                if (out_code != FGS_DTYPE_F32 && out_code != FGS_DTYPE_BF16) refuse("moments are read as float32 or bfloat16");
+                if (out.numel() != count) throw std::length_error("moments must be read into tensors of the size of their parameter");
+                void* at_out = address(out, "an output", out_code, count, device);
+                if (none) {
+                    copies.emplace_back(out, at::Tensor());
+                    continue;
+                }
+                const at::Tensor& m = state_tensor(state, k ? names.exp_avg_sq : names.exp_avg);
+                if (m.scalar_type() != at::kByte) {
+                    address(m, "a moment", FGS_DTYPE_F32, count, device);
+                    copies.emplace_back(out, m);
+                    continue;
+                }
+                codes.push_back(static_cast<const uint8_t*>(address(m, "a moment", kU8, count, device)));
+                exponents.push_back(static_cast<const uint8_t*>(address(state_tensor(state, k ? names.exp_avg_sq_exponent : names.exp_avg_exponent),
+                                                                        "an exponent", kU8, (count + kBlock - 1) / kBlock, device)));
+                to.push_back(at_out);
+                is_signed.push_back(k == 0);
+                counts.push_back(count);
+            }
+        }
+        if (device < 0) Py_RETURN_NONE;
+        const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+        for (auto& c : copies) {
+            if (c.second.defined()) c.first.copy_(c.second.view(c.first.sizes()));
+            else c.first.zero_();
+        }
+        check(lib.read_moments(codes.data(), exponents.data(), is_signed.data(), counts.data(), static_cast<int64_t>(codes.size()), to.data(), out_code,
+                               c10::cuda::getCurrentCUDAStream().stream()));
+        Py_RETURN_NONE;
+    });
+}
+
+// ---------------------------------------------------------------------------------------------------
+// embedding lookup
+
+at::Tensor lookup(const at::Tensor& table, const at::Tensor& indices, double scale, int64_t padding) {
+    const c10::cuda::CUDAGuard guard(table.device());
+    std::vector<int64_t> shape = indices.sizes().vec();
+    int64_t width = 1;
+    for (int64_t d = 1; d < table.dim(); d++) {
+        shape.push_back(table.size(d));
+        width *= table.size(d);
+    }
+    at::Tensor out = at::empty(shape, table.options().requires_grad(false));
+    check(lib.lookup(table.data_ptr(), table.size(0), width, type_code(table), indices.data_ptr(), indices.numel(),
+                     static_cast<int>(indices.element_size()), scale, padding, out.data_ptr(), c10::cuda::getCurrentCUDAStream().stream()));
     return out;
 }
 
-// pack(tensors, name, type code, device index, counts address, per, addresses address): writes every tensor's data
-// address; counts: int64 per tensor, written with its element count (per = 0), or checked: count elements (per = 1) or
-// one per `per` of them. Returns the device index. Raises RuntimeError for a tensor of another type, device (device
-// index -1: the first tensor's, which must be a CUDA one), size or layout.
-PyObject* pack(PyObject*, PyObject* args) {
-    PyObject* list;
-    const char* name;
-    int code, device;
-    long long per;
-    unsigned long long counts_at, addresses_at;
-    if (!PyArg_ParseTuple(args, "O!siiKLK", &PyList_Type, &list, &name, &code, &device, &counts_at, &per, &addresses_at)) return nullptr;
-    if (code < 0 || code > 3) return PyErr_Format(PyExc_ValueError, "unknown type code");
-    auto* counts = reinterpret_cast<int64_t*>(counts_at);
-    auto* addresses = reinterpret_cast<uint64_t*>(addresses_at);
-    try {
-        const Py_ssize_t n = PyList_GET_SIZE(list);
-        for (Py_ssize_t i = 0; i < n; i++) {
-            PyObject* o = PyList_GET_ITEM(list, i);
-            if (!THPVariable_Check(o)) return PyErr_Format(PyExc_TypeError, "%s must be a tensor", name);
-            const at::Tensor& t = THPVariable_Unpack(o);
-            if (t.layout() != at::kStrided || type_code(t) != code || !t.is_contiguous())
-                return PyErr_Format(PyExc_RuntimeError, "%s must be a contiguous %s tensor", name, kTypeNames[code]);
-            if (!t.is_cuda()) return PyErr_Format(PyExc_RuntimeError, "%s must be a CUDA tensor", name);
-            if (device < 0) device = t.get_device();
-            if (t.get_device() != device) return PyErr_Format(PyExc_RuntimeError, "%s must be on device cuda:%d like the others", name, device);
-            const int64_t numel = t.numel();
-            if (per == 0) counts[i] = numel;
-            else if (numel != (counts[i] + per - 1) / per)
-                return PyErr_Format(PyExc_RuntimeError, "%s has %lld elements, expected %lld", name, static_cast<long long>(numel),
-                                    static_cast<long long>((counts[i] + per - 1) / per));
-            addresses[i] = reinterpret_cast<uint64_t>(t.data_ptr());
-        }
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-        return nullptr;
+struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& table, const at::Tensor& indices, double scale, int64_t padding) {
+        ctx->save_for_backward({indices});
+        ctx->saved_data["shape"] = table.sizes().vec();
+        ctx->saved_data["type"] = static_cast<int64_t>(table.scalar_type());
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["padding"] = padding;
+        return lookup(table, indices, scale, padding);
     }
-    return PyLong_FromLong(device);
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        const at::Tensor indices = ctx->get_saved_variables()[0];
+        const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+        const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+        const at::Tensor g = grads[0].detach().to(type).contiguous();
+        const c10::cuda::CUDAGuard guard(g.device());
+        at::Tensor grad = at::empty(shape, g.options());
+        int64_t width = 1;
+        for (size_t d = 1; d < shape.size(); d++) width *= shape[d];
+        size_t bytes = 0;
+        check(lib.workspace_bytes(indices.numel(), shape[0], width, &bytes));
+        const at::Tensor space = at::empty({static_cast<int64_t>(bytes)}, g.options().dtype(at::kByte));
+        check(lib.lookup_grad(indices.data_ptr(), indices.numel(), static_cast<int>(indices.element_size()), g.data_ptr(), type_code(g), shape[0], width,
+                              ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), grad.data_ptr(), space.data_ptr(), bytes,
+                              c10::cuda::getCurrentCUDAStream().stream()));
+        if (at::GradMode::is_enabled() && grads[0].requires_grad()) {  // asked for a graph of the gradient: an error if it is used
+            grad.set_requires_grad(true);
+            auto error = std::make_shared<torch::autograd::DelayedError>("embedding_lookup is differentiable once", 1);
+            grad = (*error)({grad})[0];
+        }
+        return {grad, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+// embedding_lookup(table, indices, scale, padding index or None)
+PyObject* embedding_lookup(PyObject*, PyObject* args) {
+    PyObject *table_o, *indices_o, *padding_o;
+    double scale;
+    if (!PyArg_ParseTuple(args, "OOdO", &table_o, &indices_o, &scale, &padding_o)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor& table = tensor_of(table_o, "table");
+        const int code = type_code(table);
+        if (table.layout() != at::kStrided || !table.is_cuda() || code < 0 || code > FGS_DTYPE_F16 || table.dim() < 1 || !table.is_contiguous())
+            refuse("table must be a contiguous CUDA float32, bfloat16 or float16 tensor [rows, ...]");
+        const at::Tensor& given = tensor_of(indices_o, "indices");
+        if (given.layout() != at::kStrided || (given.scalar_type() != at::kLong && given.scalar_type() != at::kInt) || given.device() != table.device())
+            refuse("indices must be an int64 or int32 tensor on the device of the table");
+        int64_t padding = -1;
+        if (padding_o != Py_None) {
+            padding = PyLong_AsLongLong(padding_o);
+            if (padding == -1 && PyErr_Occurred()) throw PythonError();
+            if (padding < 0 || padding >= table.size(0)) {
+                PyErr_SetString(PyExc_ValueError, "padding_index must be a row of the table (negative indices are padding anyway)");
+                throw PythonError();
+            }
+        }
+        const at::Tensor indices = given.contiguous();
+        return THPVariable_Wrap(table.requires_grad() && at::GradMode::is_enabled() ? EmbeddingLookup::apply(table, indices, scale, padding)
+                                                                                   : lookup(table, indices, scale, padding));
+    });
 }
 
-PyMethodDef kMethods[] = {{"live", live, METH_O, "parameters with a gradient, by type"},
-                          {"pack", pack, METH_VARARGS, "checked addresses of a list of tensors"},
+// bind(addresses of the C entry points, in the order of Entries)
+PyObject* bind(PyObject*, PyObject* args) {
+    unsigned long long a[8];
+    if (!PyArg_ParseTuple(args, "KKKKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6, a + 7)) return nullptr;
+    lib = {reinterpret_cast<decltype(lib.last_error)>(a[0]),   reinterpret_cast<decltype(lib.adamw_step)>(a[1]),
+           reinterpret_cast<decltype(lib.grad_squares_capacity)>(a[2]), reinterpret_cast<decltype(lib.grad_squares)>(a[3]),
+           reinterpret_cast<decltype(lib.read_moments)>(a[4]), reinterpret_cast<decltype(lib.lookup)>(a[5]),
+           reinterpret_cast<decltype(lib.workspace_bytes)>(a[6]), reinterpret_cast<decltype(lib.lookup_grad)>(a[7])};
+    Py_RETURN_NONE;
+}
+
+PyMethodDef kMethods[] = {{"bind", bind, METH_VARARGS, "addresses of the C entry points"},
+                          {"adamw_step", adamw_step, METH_VARARGS, "one AdamW step over parameter groups"},
+                          {"read_moments", read_moments, METH_VARARGS, "values of the moments"},
+                          {"embedding_lookup", embedding_lookup, METH_VARARGS, "scaled rows of a table"},
                           {nullptr, nullptr, 0, nullptr}};
-PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fgs_host", "checked addresses of tensor lists", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fgs_host", "host side of the many-tensor operators", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fgs_host() { return PyModule_Create(&kModule); }
+PyMODINIT_FUNC PyInit__fgs_host() {
+    const auto name = [](const char* s) { return PyUnicode_InternFromString(s); };
+    names = {name("params"),  name("lr"),         name("betas"),            name("eps"),                 name("weight_decay"), name("state_bits"), name("master_weights"),
+             name("step"),    name("exp_avg"),    name("exp_avg_sq"),       name("exp_avg_exponent"),    name("exp_avg_sq_exponent"), name("master")};
+    return PyModule_Create(&kModule);
+}

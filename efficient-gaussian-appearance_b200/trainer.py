@@ -43,6 +43,7 @@ import torch.nn.functional as tf
 
 from FasterGSVDACudaBackend import rasterization as R, _lib
 from FasterGSVDACudaBackend.adam import _segment, adam_step_segments
+from FasterGSVDACudaBackend.embedding import embedding_lookup
 
 # ranks from which the 'auto' exchange reads and writes through NVSwitch multicast: the peer exchange moves
 # 2 (N - 1) / N of the vector per link direction at about 0.67 TB/s (measured at 2 and 8 GPUs), the multicast one
@@ -123,6 +124,11 @@ def morton_order(means: torch.Tensor) -> torch.Tensor:
     _lib.check(_lib.lib.fgs_morton_codes(m.data_ptr(), n, (ctypes.c_float * 3)(*lo), (ctypes.c_float * 3)(*hi), codes.data_ptr(),
                                          torch.cuda.current_stream(m.device).cuda_stream))
     return torch.argsort(codes, stable=True)  # codes < 2^63: the signed order is the code order
+
+
+def _rows(table: torch.Tensor, order: torch.Tensor) -> torch.Tensor:
+    """The rows of a contiguous [N, cols] table in the given order (a copy); CPU ranks index it with torch."""
+    return embedding_lookup(table, order) if table.is_cuda else table[order]
 
 
 class FusedLoss:
@@ -338,16 +344,16 @@ class Trainer:
             if g.name == 'mlp_weights':
                 continue
             p_rows = self.params[g.offset:g.offset + g.numel].view(n, g.cols)
-            p_rows.copy_(p_rows[order])
+            p_rows.copy_(_rows(p_rows, order))
             for local, full in ((self.exp_avg, full_m if world > 1 else None), (self.exp_avg_sq, full_v if world > 1 else None)):
                 if full is None:
                     rows_m = local[g.shard_offset:g.shard_offset + rows * g.cols].view(rows, g.cols)[:n]
-                    rows_m.copy_(rows_m[order])
+                    rows_m.copy_(_rows(rows_m, order))
                     continue
                 # the group's moments of all ranks in row order: rank r's part sits at r * shard + shard_offset
                 parts = full.view(world, self.shard)[:, g.shard_offset:g.shard_offset + rows * g.cols]
                 allrows = parts.reshape(world * rows, g.cols)
-                allrows[:n] = allrows[:n][order]
+                allrows[:n] = _rows(allrows[:n], order)
                 local[g.shard_offset:g.shard_offset + rows * g.cols].copy_(allrows[self.rank * rows:(self.rank + 1) * rows].reshape(-1))
 
     def adam_segments(self, grads: torch.Tensor | None = None, with_mlp: bool = True) -> list:

@@ -55,42 +55,38 @@ def test_step_without_gradients_does_nothing():
     assert opt.step(lambda: 3.0) == 3.0
 
 
-def _pack(tensors, code=0, per=0, counts=None, device=-1):
-    from FasterGSVDACudaBackend import adamw as A
-    counts = counts if counts is not None else (ctypes.c_int64 * max(len(tensors), 1))()
-    out = (ctypes.c_uint64 * max(len(tensors), 1))()
-    return A._host.pack(tensors, 'thing', code, device, ctypes.addressof(counts), per, ctypes.addressof(out))
-
-
-def test_host_checks():
-    x = torch.zeros(4, 6)
-    with pytest.raises(RuntimeError, match='contiguous float32'):
-        _pack([x.t()])
-    with pytest.raises(RuntimeError, match='contiguous float32'):
-        _pack([x.expand(3, 4, 6)])
+def test_layouts_refused():
+    """Strides, sparse gradients and gradients of another type are refused before anything is looked at on a device."""
+    import FasterGSVDACudaBackend as F
+    p = torch.nn.Parameter(torch.zeros(4, 6).t())
+    p.grad = torch.zeros(6, 4)
+    with pytest.raises(RuntimeError, match='parameter must be a contiguous float32'):
+        F.FusedAdamW([p]).step()
+    q = torch.nn.Parameter(torch.ones(4, 4, dtype=torch.bfloat16).expand(2, 4, 4))
+    q.grad = torch.ones(2, 4, 4, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match='contiguous bfloat16'):
-        _pack([x], code=1)
-    with pytest.raises(RuntimeError, match='contiguous float32'):
-        _pack([x.to_sparse()])
+        F.FusedAdamW([q]).step()
+
+
+def test_entries_of_the_host_module_refuse():
+    import FasterGSVDACudaBackend as F
+    host = F._lib.host
+    with pytest.raises(TypeError):
+        host.adamw_step([], [], None, None)
+    for groups, match in (([3], 'dicts'), ([{}], 'params'), ([{'params': ()}], 'list'), ([{'params': [3], 'state_bits': 8, 'master_weights': 0}], 'tensor'),
+                          ([{'params': [], 'state_bits': 5, 'master_weights': 0}], 'state_bits')):
+        with pytest.raises(RuntimeError, match=match):
+            host.adamw_step({}, groups, None, None)
+    with pytest.raises(RuntimeError, match='max_grad_norm'):
+        host.adamw_step({}, [], None, -1.0)
+    with pytest.raises(TypeError):
+        host.adamw_step({}, [], None, 'x')
+    with pytest.raises(RuntimeError, match='one tensor'):
+        host.read_moments({}, [_param()], [], [])
     with pytest.raises(RuntimeError, match='CUDA'):
-        _pack([x])
-    with pytest.raises(TypeError):
-        _pack([3])
-    with pytest.raises(ValueError):
-        _pack([x], code=9)
-    assert _pack([]) == -1
-
-
-def test_live_sorts_by_type():
-    from FasterGSVDACudaBackend import adamw as A
-    ps = [_param(3), _param(4, torch.bfloat16), _param(5, grad=False), _param(6, torch.float16), _param(7)]
-    got = A._host.live(ps)
-    assert [(c, [p.numel() for p in a], [g.numel() for g in b]) for c, a, b in got] == [(0, [3, 7], [3, 7]), (1, [4], [4]), (2, [6], [6])]
-    assert got[0][1][1] is ps[4] and got[0][2][1].data_ptr() == ps[4].grad.data_ptr()
-    with pytest.raises(TypeError):
-        A._host.live(ps + [None])
-    with pytest.raises(TypeError):
-        A._host.live(tuple(ps))
+        host.read_moments({}, [_param()], [torch.zeros(5)], [torch.zeros(5)])
+    with pytest.raises(RuntimeError, match='float32 or bfloat16'):
+        host.read_moments({}, [_param()], [torch.zeros(5).half()], [torch.zeros(5).half()])
 
 
 def _abi_call(**change):

@@ -31,6 +31,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBlock = kAdamwBlock;  // elements per warp and round; also the elements that share an exponent
 static_assert(kBlock == 32 * 8, "eight elements per lane");
 constexpr int kCtasPerSm = 4;
+constexpr uint32_t kTurn = 0x9e3779b9u;  // 2^32 / golden ratio: the thresholds' step from element to element
 
 struct Hyper {
     float lr[7], decay[7];  // lr / (1 - b1^t), 1 - lr wd
@@ -54,7 +55,7 @@ struct Table {
     uint8_t hyper[CAP];  // index into h; bit 7: every array is aligned for whole-lane accesses
     Hyper h[kMaxAdamwHypers];
     int n_tensors;
-    uint32_t chunks, rounds;  // chunk: `rounds` times kWarps blocks
+    uint32_t chunks;  // of kWarps blocks
     const double* partials;   // sums of squared gradients (nullptr: no clipping)
     int n_partials;
     double max_norm;
@@ -146,10 +147,30 @@ __device__ inline void store_codes(uint8_t* a, int lane, uint32_t left, const ui
     }
 }
 
+// Square root within 2^-23 of the value, division within 2^-22: together 6 roundings of half a step on an update that
+// is itself a small part of the parameter; the exact ones took half of the 8-bit step's instructions.
+__device__ inline float root(float x) {
+    float y;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ inline float quotient(float x, float y) { return __fdividef(x, y); }
+
 template <bool SIGNED>
 __device__ inline void decode(const uint32_t (&q)[8], int exponent, float (&x)[8]) {
     constexpr int top = SIGNED ? 127 : 255;
     const int base = 8 * (exponent + 1) - top;
+    if (base >= 0 && exponent != 255) {  // the usual case: every nonzero code is a normal float
+        const uint32_t up = static_cast<uint32_t>(base) << 20;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t c = (q[j] & top) << 20;
+            uint32_t bits = c ? c + up : 0u;
+            if (SIGNED) bits |= (q[j] << 24) & 0x80000000u;
+            x[j] = __uint_as_float(bits);
+        }
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const int c = static_cast<int>(q[j] & top);
@@ -161,30 +182,43 @@ __device__ inline void decode(const uint32_t (&q)[8], int exponent, float (&x)[8
     }
 }
 
-// codes of a block (all 32 lanes; elements that do not exist are zero); returns the exponent byte
+// codes of a block (all 32 lanes; elements that do not exist are zero); returns the exponent byte. `u0`: the threshold
+// of element 0 of the block.
 template <bool SIGNED, bool VEC>
-__device__ inline uint32_t encode(const float (&x)[8], uint32_t element, uint32_t dither, int lane, uint32_t (&q)[8]) {
+__device__ inline uint32_t encode(const float (&x)[8], uint32_t u0, int lane, uint32_t (&q)[8]) {
     constexpr int top = SIGNED ? 127 : 255;
-    uint32_t high = 0;
+    uint32_t high = 0, small = 0xffffffffu;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const uint32_t b = __float_as_uint(x[j]) & 0x7fffffffu;
         high = b > high ? b : high;
+        small = b < small ? b : small;
     }
     high = __reduce_max_sync(0xffffffffu, high) >> 23;
     const int base = 8 * (static_cast<int>(high) + 1) - top;
     const int floor = base > 0 ? base : 0;
     const uint32_t least = static_cast<uint32_t>(floor + 1) << 20;
-    const int low = floor + 1 - base;                     // the smallest code in use
+    const uint32_t u = u0 + place<VEC>(lane, 0) * kTurn;
+    if (high < 254 && small >= least) {  // the usual case: no element under the smallest code, none near the largest float
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t b = __float_as_uint(x[j]) & 0x7fffffffu;
+            const uint32_t uj = u + (VEC ? j : 32 * j) * kTurn;
+            q[j] = ((b + (uj >> 12)) >> 20) - static_cast<uint32_t>(base);
+            if (SIGNED) q[j] |= (__float_as_uint(x[j]) >> 24) & 128u;
+        }
+        return high;
+    }
+    const int low = floor + 1 - base;                         // the smallest code in use
     const int cap = top < 0x7f7 - base ? top : 0x7f7 - base;  // no code past the largest finite float
     const float share = __uint_as_float(least) * 5.9604644775390625e-8f;  // least / 2^24
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const uint32_t u = (element + place<VEC>(lane, j)) * 0x9e3779b9u + dither;
+        const uint32_t uj = u + (VEC ? j : 32 * j) * kTurn;
         const uint32_t b = __float_as_uint(x[j]) & 0x7fffffffu;
-        int c = static_cast<int>((b + (u >> 12)) >> 20) - base;
+        int c = static_cast<int>((b + (uj >> 12)) >> 20) - base;
         if (b < least) {
-            const bool keep = SIGNED ? __uint_as_float(b) > static_cast<float>(u >> 8) * share : b > 0;
+            const bool keep = SIGNED ? __uint_as_float(b) > static_cast<float>(uj >> 8) * share : b > 0;
             c = keep ? low : 0;
         }
         c = c < cap ? c : cap;
@@ -214,15 +248,24 @@ __device__ inline void update_block(const Table<CAP>& T, int t, const Hyper& H, 
     }
     if (MASTER) load_block<VEC>(T.master[t] + start, lane, left, p);
     else load_block<VEC>(param, lane, left, p);
-    const bool one_lr = H.n_lr == 1;
-    uint32_t column = one_lr ? 0u : static_cast<uint32_t>(start % static_cast<uint32_t>(H.n_lr));
+    // the moments decide the codes, so their products and sums are rounded one by one; the update is not coded
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const float gc = clip * g[j];
         m[j] = H.beta1 * m[j] + H.rest1 * gc;
         v[j] = H.beta2 * v[j] + H.rest2 * gc * gc;
-        const uint32_t c = one_lr ? 0u : (column + place<VEC>(lane, j)) % static_cast<uint32_t>(H.n_lr);
-        p[j] = p[j] * H.decay[c] - H.lr[c] * (m[j] / (sqrtf(v[j]) * H.root_rcp + H.eps));
+    }
+    if (H.n_lr == 1) {
+        const float lr = H.lr[0], decay = H.decay[0];
+#pragma unroll
+        for (int j = 0; j < 8; j++) p[j] = fmaf(-lr, quotient(m[j], fmaf(root(v[j]), H.root_rcp, H.eps)), p[j] * decay);
+    } else {
+        const uint32_t n_lr = static_cast<uint32_t>(H.n_lr), column = static_cast<uint32_t>(start % n_lr);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t c = (column + place<VEC>(lane, j)) % n_lr;
+            p[j] = fmaf(-H.lr[c], quotient(m[j], fmaf(root(v[j]), H.root_rcp, H.eps)), p[j] * H.decay[c]);
+        }
     }
     if (MASTER) store_block<VEC>(T.master[t] + start, lane, left, p);
     store_block<VEC>(param, lane, left, p);
@@ -233,10 +276,10 @@ __device__ inline void update_block(const Table<CAP>& T, int t, const Hyper& H, 
                 if (place<VEC>(lane, j) >= left) m[j] = v[j] = 0.0f;
         }
         uint32_t q[8];
-        const uint32_t element = static_cast<uint32_t>(start);
-        const uint32_t em = encode<true, VEC>(m, element, H.dither_m, lane, q);
+        const uint32_t u = static_cast<uint32_t>(start) * kTurn;
+        const uint32_t em = encode<true, VEC>(m, u + H.dither_m, lane, q);
         store_codes<VEC>(static_cast<uint8_t*>(T.m[t]) + start, lane, left, q);
-        const uint32_t ev = encode<false, VEC>(v, element, H.dither_v, lane, q);
+        const uint32_t ev = encode<false, VEC>(v, u + H.dither_v, lane, q);
         store_codes<VEC>(static_cast<uint8_t*>(T.v[t]) + start, lane, left, q);
         if (lane == 0) {
             T.m_exp[t][block] = static_cast<uint8_t>(em);
@@ -258,6 +301,11 @@ __device__ inline int owner(const TAB& T, uint32_t chunk) {
         else hi = mid;
     }
     return lo;
+}
+
+// first chunk of CTA `cta` when `chunks` are dealt out in runs as equal as they go
+__device__ inline uint32_t share_of(uint32_t chunks, uint32_t cta, uint32_t ctas) {
+    return static_cast<uint32_t>(static_cast<uint64_t>(chunks) * cta / ctas);
 }
 
 // sum of one double per thread over the CTA, the same in every thread and every run
@@ -285,20 +333,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __gri
         clip = c < 1.0 ? static_cast<float>(c) : norm == norm ? 1.0f : __int_as_float(0x7fc00000);
         if (blockIdx.x == 0 && threadIdx.x == 0) *T.norm_out = static_cast<float>(norm);
     }
-    for (uint32_t i = blockIdx.x; i < T.chunks; i += gridDim.x) {
-        // with clipping the norm has just read the gradients front to back: start at the end, which is still in L2
-        const uint32_t chunk = T.partials ? T.chunks - 1 - i : i;
-        const int t = owner(T, chunk);
+    const uint32_t first = share_of(T.chunks, blockIdx.x, gridDim.x), end = share_of(T.chunks, blockIdx.x + 1, gridDim.x);
+    if (first == end) return;
+    // with clipping the norm has just walked the same shares front to back: their ends are still in L2
+    const bool back = T.partials != nullptr;
+    int t = owner(T, back ? end - 1 : first);
+    for (uint32_t i = first; i < end; i++) {
+        const uint32_t chunk = back ? first + end - 1 - i : i;
+        while (chunk >= T.first[t + 1]) t++;
+        while (chunk < T.first[t]) t--;
         const uint64_t n = T.n[t];
         const Hyper& H = T.h[T.hyper[t] & 127];
-        const bool vec = T.hyper[t] & 128;
-        const uint64_t first = static_cast<uint64_t>(chunk - T.first[t]) * T.rounds;
-        for (uint32_t r = 0; r < T.rounds; r++) {
-            const uint64_t start = ((first + r) * kWarps + warp) * kBlock;
-            if (start >= n) break;
-            if (vec && n - start >= kBlock) update_block<P, EIGHT, MASTER, true>(T, t, H, start, kBlock, clip, lane);
-            else update_block<P, EIGHT, MASTER, false>(T, t, H, start, n - start < kBlock ? static_cast<uint32_t>(n - start) : kBlock, clip, lane);
-        }
+        const uint64_t start = (static_cast<uint64_t>(chunk - T.first[t]) * kWarps + warp) * kBlock;
+        if (start >= n) continue;
+        if ((T.hyper[t] & 128) && n - start >= kBlock) update_block<P, EIGHT, MASTER, true>(T, t, H, start, kBlock, clip, lane);
+        else update_block<P, EIGHT, MASTER, false>(T, t, H, start, n - start < kBlock ? static_cast<uint32_t>(n - start) : kBlock, clip, lane);
     }
 }
 
@@ -327,7 +376,6 @@ cudaError_t launch_all(const AdamwTensors& A, const AdamwHyper* hypers, int dtyp
         Table<CAP> T;
         int k = 0, n_hyper = 0;
         int hyper_of[kMaxAdamwHypers];
-        uint64_t blocks = 0;
         for (; i < A.count && k < CAP; i++) {
             if (A.n_elements[i] <= 0) continue;
             int h = 0;
@@ -359,17 +407,14 @@ cudaError_t launch_all(const AdamwTensors& A, const AdamwHyper* hypers, int dtyp
             const bool vec = aligned(A.param[i], wide) && aligned(A.grad[i], wide) && aligned(A.m[i], moments) && aligned(A.v[i], moments) &&
                              (!master || aligned(A.master[i], 32));
             T.hyper[k] = static_cast<uint8_t>(h | (vec ? 128 : 0));
-            blocks += (T.n[k] + kBlock - 1) / kBlock;
             k++;
         }
         if (k == 0) return cudaSuccess;
         T.n_tensors = k;
-        // chunks of four rounds spare the search for a chunk's tensor; few blocks are spread over as many CTAs as there are
-        T.rounds = blocks >= static_cast<uint64_t>(sms) * kCtasPerSm * kWarps * 4 ? 4 : 1;
         uint64_t chunks = 0;
         for (int j = 0; j < k; j++) {
             T.first[j] = static_cast<uint32_t>(chunks);
-            const uint64_t per = static_cast<uint64_t>(kBlock) * kWarps * T.rounds;
+            const uint64_t per = static_cast<uint64_t>(kBlock) * kWarps;
             chunks += (T.n[j] + per - 1) / per;
             if (chunks > 0xFFFFFFFFull - 65536) return cudaErrorInvalidValue;
         }
@@ -428,11 +473,13 @@ __device__ inline float chunk_squares(const P* g, uint64_t left, bool vec) {
     return s;
 }
 
-__global__ void __launch_bounds__(kThreads) grad_squares_kernel(const __grid_constant__ NormTable T) {
+__global__ void __launch_bounds__(kThreads, kNormPartials / 148) grad_squares_kernel(const __grid_constant__ NormTable T) {
     __shared__ double scratch[kWarps];
     double total = 0.0;
-    for (uint32_t chunk = blockIdx.x; chunk < T.chunks; chunk += gridDim.x) {
-        const int t = owner(T, chunk);
+    const uint32_t first = share_of(T.chunks, blockIdx.x, gridDim.x), end = share_of(T.chunks, blockIdx.x + 1, gridDim.x);
+    int t = owner(T, first);
+    for (uint32_t chunk = first; chunk < end; chunk++) {
+        while (chunk >= T.first[t + 1]) t++;
         const uint64_t start = static_cast<uint64_t>(chunk - T.first[t]) * kNormChunk;
         const uint64_t left = T.n[t] - start;
         const bool vec = T.kind[t] & 128;
@@ -463,27 +510,57 @@ struct ReadTable {
 };
 static_assert(sizeof(ReadTable) <= 32764, "kernel parameter limit");
 
-template <typename O, bool SIGNED, bool VEC>
-__device__ inline void read_block(const ReadTable& T, int t, uint64_t start, uint32_t left, int lane) {
-    uint32_t q[8];
-    float x[8];
-    load_codes<VEC>(T.codes[t] + start, lane, left, q);
-    decode<SIGNED>(q, T.exps[t][start / kBlock], x);
-    store_block<VEC>(static_cast<O*>(T.out[t]) + start, lane, left, x);
+constexpr uint32_t kReadBlocks = 4;  // blocks of a warp's run
+
+template <typename O, bool SIGNED>
+__device__ inline void read_blocks(const uint8_t* codes, const uint8_t* exps, O* out, uint64_t start, uint64_t left, bool vec, int lane) {
+    if (vec && left >= kReadBlocks * kBlock) {  // 16 codes per lane and access, both accesses in flight
+        uint4 r[2];
+        uint32_t e[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            r[h] = *reinterpret_cast<const uint4*>(codes + start + h * 2 * kBlock + lane * 16);
+            e[h] = exps[start / kBlock + 2 * h + (lane >> 4)];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const uint32_t lo = k ? r[h].z : r[h].x, hi = k ? r[h].w : r[h].y;
+                uint32_t q[8];
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) q[j] = ((j < 4 ? lo : hi) >> (8 * (j & 3))) & 255u;
+                decode<SIGNED>(q, static_cast<int>(e[h]), x);
+                store8(out + start + h * 2 * kBlock + lane * 16 + 8 * k, x);
+            }
+        }
+        return;
+    }
+    for (uint32_t b = 0; b < kReadBlocks && b * kBlock < left; b++) {
+        const uint32_t have = left - b * kBlock < kBlock ? static_cast<uint32_t>(left - b * kBlock) : kBlock;
+        uint32_t q[8];
+        float x[8];
+        load_codes<false>(codes + start + b * kBlock, lane, have, q);
+        decode<SIGNED>(q, exps[start / kBlock + b], x);
+        store_block<false>(out + start + b * kBlock, lane, have, x);
+    }
 }
 
 template <typename O>
 __global__ void __launch_bounds__(kThreads) read_moments_kernel(const __grid_constant__ ReadTable T) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (uint32_t chunk = blockIdx.x; chunk < T.chunks; chunk += gridDim.x) {
-        const int t = owner(T, chunk);
+    const uint32_t first = share_of(T.chunks, blockIdx.x, gridDim.x), end = share_of(T.chunks, blockIdx.x + 1, gridDim.x);
+    int t = owner(T, first);
+    for (uint32_t chunk = first; chunk < end; chunk++) {
+        while (chunk >= T.first[t + 1]) t++;
         const uint64_t n = T.n[t];
-        const uint64_t start = (static_cast<uint64_t>(chunk - T.first[t]) * kWarps + warp) * kBlock;
+        const uint64_t start = (static_cast<uint64_t>(chunk - T.first[t]) * kWarps + warp) * (kReadBlocks * kBlock);
         if (start >= n) continue;
-        const uint32_t left = n - start < kBlock ? static_cast<uint32_t>(n - start) : kBlock;
-        const bool vec = (T.kind[t] & 128) && left == kBlock;
-        if (T.kind[t] & 1) vec ? read_block<O, true, true>(T, t, start, left, lane) : read_block<O, true, false>(T, t, start, left, lane);
-        else vec ? read_block<O, false, true>(T, t, start, left, lane) : read_block<O, false, false>(T, t, start, left, lane);
+        O* out = static_cast<O*>(T.out[t]);
+        const bool vec = T.kind[t] & 128;
+        if (T.kind[t] & 1) read_blocks<O, true>(T.codes[t], T.exps[t], out, start, n - start, vec, lane);
+        else read_blocks<O, false>(T.codes[t], T.exps[t], out, start, n - start, vec, lane);
     }
 }
 
@@ -541,9 +618,9 @@ cudaError_t launch_read_moments(const uint8_t* const* codes, const uint8_t* cons
             T.exps[k] = exps[i];
             T.out[k] = out[i];
             T.n[k] = static_cast<uint64_t>(n_elements[i]);
-            T.kind[k] = static_cast<uint8_t>((is_signed[i] ? 1 : 0) | (aligned(codes[i], 8) && aligned(out[i], dtype == kDtypeF32 ? 32 : 16) ? 128 : 0));
+            T.kind[k] = static_cast<uint8_t>((is_signed[i] ? 1 : 0) | (aligned(codes[i], 16) && aligned(out[i], dtype == kDtypeF32 ? 32 : 16) ? 128 : 0));
             T.first[k] = static_cast<uint32_t>(chunks);
-            chunks += (T.n[k] + kBlock * kWarps - 1) / (kBlock * kWarps);
+            chunks += (T.n[k] + kReadBlocks * kBlock * kWarps - 1) / (kReadBlocks * kBlock * kWarps);
             if (chunks > 0xFFFFFFFFull - 65536) return cudaErrorInvalidValue;
             k++;
         }

@@ -87,8 +87,9 @@ def bounds(p, m, v, g, t: int, lr, betas, eps: float, weight_decay: float, clipp
     the norm's and the factor's own conversion and the product: 20 e on g.
     m: each product has a rounded factor and its own rounding, and g's error; the sum's one: (3 + 20) e (|b1 m| + |(1 - b1) g|).
     v: factor, two products, sum, and twice g's error: (4 + 40) e v (all terms are positive).
-    update u = lr' m / (sqrt(v) r + eps): v's half, root, r, product, sum, quotient, lr', product: (7 + 22) e |u|, and m's
-    error through it. p: factor, product and the final difference: 3 e (|p| + |u|), which covers the difference's result."""
+    update u = lr' (m / (sqrt(v) r + eps)): half of v's (2 + 20), the root within 2^-23 (2), r (1), the fused sum (1), the
+    quotient within 2 ulp (4), lr' (1): (11 + 20) e |u|, and m's error through it. p: factor, product and the final fused
+    difference: 3 e (|p| + |u|), which covers the difference's result."""
     e = 2.0 ** -24
     cg = 20 if clipped else 0
     lrs = np.asarray(lr if isinstance(lr, (list, tuple)) else [lr], np.float64)
@@ -99,6 +100,6 @@ def bounds(p, m, v, g, t: int, lr, betas, eps: float, weight_decay: float, clipp
     dv = (4 + 2 * cg) * e * new_v
     slope = lr / (1 - betas[0] ** t) / (np.sqrt(new_v / (1 - betas[1] ** t)) + eps)
     u = np.abs(slope * new_m)
-    dp = slope * dm + (9 + cg) * e * u + 3 * e * (np.abs(p) + u)
+    dp = slope * dm + (11 + cg) * e * u + 3 * e * (np.abs(p) + u)
     tiny = 2.0 ** -148  # results among the subnormals: two roundings of half their spacing
     return 1.01 * dp + tiny, 1.01 * dm + tiny, 1.01 * dv + tiny

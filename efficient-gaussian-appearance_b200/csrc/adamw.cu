@@ -30,7 +30,12 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBlock = kAdamwBlock;  // elements per warp and round; also the elements that share an exponent
 static_assert(kBlock == 32 * 8, "eight elements per lane");
-constexpr int kCtasPerSm = 4;
+// resident CTAs per SM that the registers are bounded for: with 8-bit moments 3 (80 registers; 4 spill 100 bytes and take
+// 143 instead of 129 us for 40M bf16 elements)
+template <typename P, bool EIGHT, bool MASTER>
+constexpr int ctas_per_sm() {
+    return EIGHT ? 3 : 4;
+}
 constexpr uint32_t kTurn = 0x9e3779b9u;  // 2^32 / golden ratio: the thresholds' step from element to element
 
 struct Hyper {
@@ -55,12 +60,18 @@ struct Table {
     uint8_t hyper[CAP];  // index into h; bit 7: every array is aligned for whole-lane accesses
     Hyper h[kMaxAdamwHypers];
     int n_tensors;
-    uint32_t chunks;  // of kWarps blocks
+    uint32_t chunks;  // 32-bit moments: of kWarps blocks, one CTA's at a time; 8-bit moments: of `blocks` blocks, one warp's
+    uint32_t blocks;
     const double* partials;   // sums of squared gradients (nullptr: no clipping)
+    const float* factor;      // the clip factor, where it has been made from them (else nullptr)
     int n_partials;
     double max_norm;
     float* norm_out;
 };
+constexpr uint32_t kMaxRun = 8;  // blocks of a warp's run (at most 32: one lane each)
+
+// whether the hardware hands out the CTAs as SMs become free (else: one resident grid, equal shares)
+inline bool long_step(uint32_t chunks, uint32_t blocks, int sms) { return static_cast<uint64_t>(chunks) * blocks > static_cast<uint64_t>(sms) * 4 * kWarps * 8; }
 constexpr int kFewTensors = 24, kManyTensors = 384;
 static_assert(sizeof(Table<kManyTensors>) <= 32764, "kernel parameter limit");
 
@@ -70,6 +81,13 @@ __device__ inline float to_float(__half x) { return __half2float(x); }
 __device__ inline void from_float(float x, float& y) { y = x; }
 __device__ inline void from_float(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
 __device__ inline void from_float(float x, __half& y) { y = __float2half_rn(x); }
+
+template <typename H>
+__device__ inline void unpack8(const uint4& r, float (&x)[8]) {
+    const H* h = reinterpret_cast<const H*>(&r);
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = to_float(h[j]);
+}
 
 // eight consecutive elements of a lane: 32-byte accesses for fp32, 16 for the halves, 8 for codes
 __device__ inline void load8(const float* a, float (&x)[8]) {
@@ -84,10 +102,7 @@ __device__ inline void store8(float* a, const float (&x)[8]) {
 }
 template <typename H>
 __device__ inline void load8(const H* a, float (&x)[8]) {
-    const uint4 r = *reinterpret_cast<const uint4*>(a);
-    const H* h = reinterpret_cast<const H*>(&r);
-#pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = to_float(h[j]);
+    unpack8<H>(*reinterpret_cast<const uint4*>(a), x);
 }
 template <typename H>
 __device__ inline void store8(H* a, const float (&x)[8]) {
@@ -122,24 +137,22 @@ __device__ inline void store_block(P* a, int lane, uint32_t left, const float (&
             if (place<VEC>(lane, j) < left) from_float(x[j], a[place<VEC>(lane, j)]);
     }
 }
+// code bytes of a lane's eight elements: two packed words (VEC) or one per register
 template <bool VEC>
-__device__ inline void load_codes(const uint8_t* a, int lane, uint32_t left, uint32_t (&q)[8]) {
+__device__ inline void load_codes(const uint8_t* a, int lane, uint32_t left, uint32_t* q) {
     if (VEC) {
         const uint2 r = *reinterpret_cast<const uint2*>(a + lane * 8);
-#pragma unroll
-        for (int j = 0; j < 8; j++) q[j] = ((j < 4 ? r.x : r.y) >> (8 * (j & 3))) & 255u;
+        q[0] = r.x;
+        q[1] = r.y;
     } else {
 #pragma unroll
         for (int j = 0; j < 8; j++) q[j] = place<VEC>(lane, j) < left ? a[place<VEC>(lane, j)] : 0u;
     }
 }
 template <bool VEC>
-__device__ inline void store_codes(uint8_t* a, int lane, uint32_t left, const uint32_t (&q)[8]) {
+__device__ inline void store_codes(uint8_t* a, int lane, uint32_t left, const uint32_t* q) {
     if (VEC) {
-        uint2 r;
-        r.x = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
-        r.y = q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24;
-        *reinterpret_cast<uint2*>(a + lane * 8) = r;
+        *reinterpret_cast<uint2*>(a + lane * 8) = make_uint2(q[0], q[1]);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; j++)
@@ -156,138 +169,178 @@ __device__ inline float root(float x) {
 }
 __device__ inline float quotient(float x, float y) { return __fdividef(x, y); }
 
-template <bool SIGNED>
-__device__ inline void decode(const uint32_t (&q)[8], int exponent, float (&x)[8]) {
+// values of one code each; the codes come as bytes of packed words (four each) or one per register (q[j] < 256)
+template <bool SIGNED, bool PACKED>
+__device__ inline void decode(const uint32_t* q, int exponent, float (&x)[8]) {
     constexpr int top = SIGNED ? 127 : 255;
     const int base = 8 * (exponent + 1) - top;
     if (base >= 0 && exponent != 255) {  // the usual case: every nonzero code is a normal float
         const uint32_t up = static_cast<uint32_t>(base) << 20;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const uint32_t c = (q[j] & top) << 20;
-            uint32_t bits = c ? c + up : 0u;
-            if (SIGNED) bits |= (q[j] << 24) & 0x80000000u;
+            const uint32_t high = PACKED ? __byte_perm(q[j / 4], 0, (j & 3) << 12 | 0x444) : q[j] << 24;  // the code in bits 24..31
+            uint32_t bits = (high >> 4) & (static_cast<uint32_t>(top) << 20);
+            if (bits != 0) bits += up;
+            if (SIGNED) bits |= high & 0x80000000u;
             x[j] = __uint_as_float(bits);
         }
         return;
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const int c = static_cast<int>(q[j] & top);
+        const uint32_t code = PACKED ? (q[j / 4] >> (8 * (j & 3))) & 255u : q[j];
+        const int c = static_cast<int>(code & top);
         const int k = c + base;
         uint32_t bits = c > 0 && k > 0 ? static_cast<uint32_t>(k) << 20 : 0u;
         if (exponent == 255) bits = 0x7fc00000u;
-        if (SIGNED) bits |= (q[j] & 128u) << 24;
+        if (SIGNED) bits |= (code & 128u) << 24;
         x[j] = __uint_as_float(bits);
     }
 }
 
-// codes of a block (all 32 lanes; elements that do not exist are zero); returns the exponent byte. `u0`: the threshold
-// of element 0 of the block.
+// codes of a block (all 32 lanes; elements that do not exist are zero), packed (VEC) or one per register; returns the
+// exponent byte. `u0`: the threshold of element 0 of the block.
 template <bool SIGNED, bool VEC>
-__device__ inline uint32_t encode(const float (&x)[8], uint32_t u0, int lane, uint32_t (&q)[8]) {
+__device__ inline uint32_t encode(const float (&x)[8], uint32_t u0, int lane, uint32_t* q) {
     constexpr int top = SIGNED ? 127 : 255;
-    uint32_t high = 0, small = 0xffffffffu;
+    uint32_t b[8];  // bits of the magnitudes (the second moment has no sign; that of a NaN is cut off below)
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const uint32_t b = __float_as_uint(x[j]) & 0x7fffffffu;
-        high = b > high ? b : high;
-        small = b < small ? b : small;
+    for (int j = 0; j < 8; j++) b[j] = SIGNED ? __float_as_uint(x[j]) & 0x7fffffffu : __float_as_uint(x[j]);
+    uint32_t high = b[0] > b[1] ? b[0] : b[1], small = b[0] < b[1] ? b[0] : b[1];
+#pragma unroll
+    for (int j = 2; j < 8; j += 2) {
+        high = __vimax3_u32(high, b[j], b[j + 1]);
+        small = __vimin3_u32(small, b[j], b[j + 1]);
     }
-    high = __reduce_max_sync(0xffffffffu, high) >> 23;
+    high = (__reduce_max_sync(0xffffffffu, high) >> 23) & 255u;
     const int base = 8 * (static_cast<int>(high) + 1) - top;
     const int floor = base > 0 ? base : 0;
     const uint32_t least = static_cast<uint32_t>(floor + 1) << 20;
     const uint32_t u = u0 + place<VEC>(lane, 0) * kTurn;
-    if (high < 254 && small >= least) {  // the usual case: no element under the smallest code, none near the largest float
+    if (VEC && high < 254 && small >= least) {  // the usual case: nothing under the smallest code or near the largest float
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t b = __float_as_uint(x[j]) & 0x7fffffffu;
-            const uint32_t uj = u + (VEC ? j : 32 * j) * kTurn;
-            q[j] = ((b + (uj >> 12)) >> 20) - static_cast<uint32_t>(base);
-            if (SIGNED) q[j] |= (__float_as_uint(x[j]) >> 24) & 128u;
+        for (int w = 0; w < 2; w++) {
+            uint32_t word = static_cast<uint32_t>(-base) * 0x01010101u;  // every k - base fits its byte: their sum has no carries
+#pragma unroll
+            for (int j = 0; j < 4; j++) word += ((b[4 * w + j] + ((u + (4 * w + j) * kTurn) >> 12)) >> 20) << (8 * j);
+            if (SIGNED) {
+                const uint32_t lo = __byte_perm(__float_as_uint(x[4 * w]), __float_as_uint(x[4 * w + 1]), 0x0073);
+                const uint32_t hi = __byte_perm(__float_as_uint(x[4 * w + 2]), __float_as_uint(x[4 * w + 3]), 0x0073);
+                word |= __byte_perm(lo, hi, 0x5410) & 0x80808080u;
+            }
+            q[w] = word;
         }
         return high;
     }
     const int low = floor + 1 - base;                         // the smallest code in use
     const int cap = top < 0x7f7 - base ? top : 0x7f7 - base;  // no code past the largest finite float
     const float share = __uint_as_float(least) * 5.9604644775390625e-8f;  // least / 2^24
+    if (VEC) q[0] = q[1] = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const uint32_t uj = u + (VEC ? j : 32 * j) * kTurn;
-        const uint32_t b = __float_as_uint(x[j]) & 0x7fffffffu;
-        int c = static_cast<int>((b + (uj >> 12)) >> 20) - base;
-        if (b < least) {
-            const bool keep = SIGNED ? __uint_as_float(b) > static_cast<float>(uj >> 8) * share : b > 0;
+        const uint32_t bj = b[j] & 0x7fffffffu;
+        int c = static_cast<int>((bj + (uj >> 12)) >> 20) - base;
+        if (bj < least) {
+            const bool keep = SIGNED ? __uint_as_float(bj) > static_cast<float>(uj >> 8) * share : bj > 0;
             c = keep ? low : 0;
         }
         c = c < cap ? c : cap;
-        q[j] = static_cast<uint32_t>(c) & 255u;
-        if (SIGNED) q[j] = (q[j] & 127u) | (x[j] < 0.0f ? 128u : 0u);
+        uint32_t code = static_cast<uint32_t>(c) & 255u;
+        if (SIGNED) code = (code & 127u) | (x[j] < 0.0f ? 128u : 0u);
+        if (VEC) q[j / 4] |= code << (8 * (j & 3));
+        else q[j] = code;
     }
     return high;
 }
 
-template <typename P, bool EIGHT, bool MASTER, bool VEC, int CAP>
-__device__ inline void update_block(const Table<CAP>& T, int t, const Hyper& H, uint64_t start, uint32_t left, float clip, int lane) {
-    P* param = static_cast<P*>(T.param[t]) + start;
-    const P* grad = static_cast<const P*>(T.grad[t]) + start;
+// the addresses of a chunk's first elements
+template <typename P>
+struct Chunk {
+    P* param;
+    const P* grad;
+    void* m;
+    void* v;
+    float* master;
+};
+
+// What a lane reads of one block. Halves read as a whole stay packed until they are used: converting them waits for the load.
+template <typename P, bool EIGHT, bool MASTER>
+struct Loaded {
     float p[8], g[8], m[8], v[8];
-    const uint64_t block = start / kBlock;
-    load_block<VEC>(grad, lane, left, g);
+    uint4 packed_p, packed_g;
+    uint32_t qm[8], qv[8];
+};
+
+template <typename P, bool EIGHT, bool MASTER, bool VEC>
+__device__ inline void load_all(const Chunk<P>& C, uint32_t at, uint32_t left, int lane, Loaded<P, EIGHT, MASTER>& L) {
+    constexpr bool packed = VEC && sizeof(P) == 2;
+    if (packed) L.packed_g = *reinterpret_cast<const uint4*>(C.grad + at + lane * 8);
+    else load_block<VEC>(C.grad + at, lane, left, L.g);
+    if (MASTER) load_block<VEC>(C.master + at, lane, left, L.p);
+    else if (packed) L.packed_p = *reinterpret_cast<const uint4*>(C.param + at + lane * 8);
+    else load_block<VEC>(C.param + at, lane, left, L.p);
     if (EIGHT) {
-        uint32_t qm[8], qv[8];
-        load_codes<VEC>(static_cast<const uint8_t*>(T.m[t]) + start, lane, left, qm);
-        load_codes<VEC>(static_cast<const uint8_t*>(T.v[t]) + start, lane, left, qv);
-        const int em = T.m_exp[t][block], ev = T.v_exp[t][block];
-        decode<true>(qm, em, m);
-        decode<false>(qv, ev, v);
+        load_codes<VEC>(static_cast<const uint8_t*>(C.m) + at, lane, left, L.qm);
+        load_codes<VEC>(static_cast<const uint8_t*>(C.v) + at, lane, left, L.qv);
     } else {
-        load_block<VEC>(static_cast<const float*>(T.m[t]) + start, lane, left, m);
-        load_block<VEC>(static_cast<const float*>(T.v[t]) + start, lane, left, v);
+        load_block<VEC>(static_cast<const float*>(C.m) + at, lane, left, L.m);
+        load_block<VEC>(static_cast<const float*>(C.v) + at, lane, left, L.v);
     }
-    if (MASTER) load_block<VEC>(T.master[t] + start, lane, left, p);
-    else load_block<VEC>(param, lane, left, p);
+}
+
+// The update of a lane's eight elements: p, m, v in L become the new ones. `start`: the block's first element within the tensor.
+template <typename P, bool EIGHT, bool MASTER, bool VEC>
+__device__ inline void update(const Hyper& H, uint64_t start, float clip, int lane, Loaded<P, EIGHT, MASTER>& L, uint32_t em, uint32_t ev) {
+    if constexpr (VEC && sizeof(P) == 2) {
+        unpack8<P>(L.packed_g, L.g);
+        if (!MASTER) unpack8<P>(L.packed_p, L.p);
+    }
+    if (EIGHT) {
+        decode<true, VEC>(L.qm, static_cast<int>(em), L.m);
+        decode<false, VEC>(L.qv, static_cast<int>(ev), L.v);
+    }
     // the moments decide the codes, so their products and sums are rounded one by one; the update is not coded
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const float gc = clip * g[j];
-        m[j] = H.beta1 * m[j] + H.rest1 * gc;
-        v[j] = H.beta2 * v[j] + H.rest2 * gc * gc;
+        const float gc = clip * L.g[j];
+        L.m[j] = H.beta1 * L.m[j] + H.rest1 * gc;
+        L.v[j] = H.beta2 * L.v[j] + H.rest2 * gc * gc;
     }
     if (H.n_lr == 1) {
         const float lr = H.lr[0], decay = H.decay[0];
 #pragma unroll
-        for (int j = 0; j < 8; j++) p[j] = fmaf(-lr, quotient(m[j], fmaf(root(v[j]), H.root_rcp, H.eps)), p[j] * decay);
+        for (int j = 0; j < 8; j++) L.p[j] = fmaf(-lr, quotient(L.m[j], fmaf(root(L.v[j]), H.root_rcp, H.eps)), L.p[j] * decay);
     } else {
         const uint32_t n_lr = static_cast<uint32_t>(H.n_lr), column = static_cast<uint32_t>(start % n_lr);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const uint32_t c = (column + place<VEC>(lane, j)) % n_lr;
-            p[j] = fmaf(-H.lr[c], quotient(m[j], fmaf(root(v[j]), H.root_rcp, H.eps)), p[j] * H.decay[c]);
+            L.p[j] = fmaf(-H.lr[c], quotient(L.m[j], fmaf(root(L.v[j]), H.root_rcp, H.eps)), L.p[j] * H.decay[c]);
         }
     }
-    if (MASTER) store_block<VEC>(T.master[t] + start, lane, left, p);
-    store_block<VEC>(param, lane, left, p);
+}
+
+template <typename P, bool EIGHT, bool MASTER, bool VEC>
+__device__ inline void store_all(const Chunk<P>& C, const Hyper& H, uint64_t start, uint32_t at, uint32_t left, int lane, float (&p)[8], float (&m)[8],
+                                 float (&v)[8], uint32_t& em, uint32_t& ev) {
+    if (MASTER) store_block<VEC>(C.master + at, lane, left, p);
+    store_block<VEC>(C.param + at, lane, left, p);
     if (EIGHT) {
         if (!VEC) {  // places past the end take no part in the block's exponent (nor in anything else)
 #pragma unroll
             for (int j = 0; j < 8; j++)
                 if (place<VEC>(lane, j) >= left) m[j] = v[j] = 0.0f;
         }
-        uint32_t q[8];
+        uint32_t q[VEC ? 2 : 8];
         const uint32_t u = static_cast<uint32_t>(start) * kTurn;
-        const uint32_t em = encode<true, VEC>(m, u + H.dither_m, lane, q);
-        store_codes<VEC>(static_cast<uint8_t*>(T.m[t]) + start, lane, left, q);
-        const uint32_t ev = encode<false, VEC>(v, u + H.dither_v, lane, q);
-        store_codes<VEC>(static_cast<uint8_t*>(T.v[t]) + start, lane, left, q);
-        if (lane == 0) {
-            T.m_exp[t][block] = static_cast<uint8_t>(em);
-            T.v_exp[t][block] = static_cast<uint8_t>(ev);
-        }
+        em = encode<true, VEC>(m, u + H.dither_m, lane, q);
+        store_codes<VEC>(static_cast<uint8_t*>(C.m) + at, lane, left, q);
+        ev = encode<false, VEC>(v, u + H.dither_v, lane, q);
+        store_codes<VEC>(static_cast<uint8_t*>(C.v) + at, lane, left, q);
     } else {
-        store_block<VEC>(static_cast<float*>(T.m[t]) + start, lane, left, m);
-        store_block<VEC>(static_cast<float*>(T.v[t]) + start, lane, left, v);
+        store_block<VEC>(static_cast<float*>(C.m) + at, lane, left, m);
+        store_block<VEC>(static_cast<float*>(C.v) + at, lane, left, v);
     }
 }
 
@@ -320,41 +373,131 @@ __device__ inline double block_sum(double x, double* scratch) {
     return s;
 }
 
+template <typename P, bool EIGHT, bool MASTER, typename TAB>
+__device__ inline Chunk<P> chunk_at(const TAB& T, int t, uint64_t start) {
+    return Chunk<P>{static_cast<P*>(T.param[t]) + start, static_cast<const P*>(T.grad[t]) + start, static_cast<char*>(T.m[t]) + start * (EIGHT ? 1 : 4),
+                    static_cast<char*>(T.v[t]) + start * (EIGHT ? 1 : 4), MASTER ? T.master[t] + start : nullptr};
+}
+
+// A warp's run of blocks with 8-bit moments: lane b keeps the exponents of block b, read and written with one access per
+// run. (One byte load and store per block, from different warps, made every read of a sector wait for the partial writes
+// to it: 59M elements took 385 us, against 185 us without them.)
+template <typename P, bool MASTER, int CAP>
+__device__ inline void update_run(const Table<CAP>& T, uint32_t run, float clip, int lane) {
+    const int t = owner(T, run);
+    const Hyper& H = T.h[T.hyper[t] & 127];
+    const uint64_t start = static_cast<uint64_t>(run - T.first[t]) * (T.blocks * kBlock);
+    const uint64_t left = T.n[t] - start;
+    const uint32_t have = left < T.blocks * kBlock ? static_cast<uint32_t>(left) : T.blocks * kBlock;  // elements
+    const uint32_t blocks = (have + kBlock - 1) / kBlock;
+    const Chunk<P> C = chunk_at<P, true, MASTER>(T, t, start);
+    uint8_t* m_exp = T.m_exp[t] + start / kBlock;
+    uint8_t* v_exp = T.v_exp[t] + start / kBlock;
+    uint32_t em = 0, ev = 0;
+    if (lane < blocks) {
+        em = m_exp[lane];
+        ev = v_exp[lane];
+    }
+    const bool vec = T.hyper[t] & 128;
+    for (uint32_t b = 0; b < blocks; b++) {
+        const uint32_t at = b * kBlock;
+        uint32_t em_b = __shfl_sync(0xffffffffu, em, b), ev_b = __shfl_sync(0xffffffffu, ev, b);
+        Loaded<P, true, MASTER> L;
+        if (vec && have - at >= kBlock) {
+            load_all<P, true, MASTER, true>(C, at, kBlock, lane, L);
+            update<P, true, MASTER, true>(H, start + at, clip, lane, L, em_b, ev_b);
+            store_all<P, true, MASTER, true>(C, H, start + at, at, kBlock, lane, L.p, L.m, L.v, em_b, ev_b);
+        } else {
+            const uint32_t n = have - at < kBlock ? have - at : kBlock;
+            load_all<P, true, MASTER, false>(C, at, n, lane, L);
+            update<P, true, MASTER, false>(H, start + at, clip, lane, L, em_b, ev_b);
+            store_all<P, true, MASTER, false>(C, H, start + at, at, n, lane, L.p, L.m, L.v, em_b, ev_b);
+        }
+        if (lane == b) {
+            em = em_b;
+            ev = ev_b;
+        }
+    }
+    if (lane < blocks) {
+        m_exp[lane] = static_cast<uint8_t>(em);
+        v_exp[lane] = static_cast<uint8_t>(ev);
+    }
+}
+
+__device__ inline float clip_factor(double norm, double max_norm) {
+    const double c = max_norm / (norm + 1e-6);
+    return c < 1.0 ? static_cast<float>(c) : norm == norm ? 1.0f : __int_as_float(0x7fc00000);
+}
+
+// the norm and the clip factor from the partial sums, for steps of so many CTAs that not each should add them up
+__global__ void __launch_bounds__(kThreads) clip_kernel(const double* __restrict__ partials, int n_partials, double max_norm, float* __restrict__ factor,
+                                                        float* __restrict__ norm_out) {
+    __shared__ double scratch[kWarps];
+    double x = 0.0;
+    for (int i = threadIdx.x; i < n_partials; i += kThreads) x += partials[i];
+    const double norm = sqrt(block_sum(x, scratch));
+    if (threadIdx.x == 0) {
+        *factor = clip_factor(norm, max_norm);
+        *norm_out = static_cast<float>(norm);
+    }
+}
+
 template <typename P, bool EIGHT, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __grid_constant__ Table<CAP> T) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<P, EIGHT, MASTER>()) adamw_kernel(const __grid_constant__ Table<CAP> T) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float clip = 1.0f;
-    if (T.partials) {  // every CTA adds the partial sums in the same order: no further launch, no atomics
+    if (T.factor) {
+        clip = *T.factor;
+    } else if (T.partials) {  // every CTA adds the partial sums in the same order: no further launch, no atomics
         __shared__ double scratch[kWarps];
         double x = 0.0;
         for (int i = threadIdx.x; i < T.n_partials; i += kThreads) x += T.partials[i];
         const double norm = sqrt(block_sum(x, scratch));
-        const double c = T.max_norm / (norm + 1e-6);
-        clip = c < 1.0 ? static_cast<float>(c) : norm == norm ? 1.0f : __int_as_float(0x7fc00000);
+        clip = clip_factor(norm, T.max_norm);
         if (blockIdx.x == 0 && threadIdx.x == 0) *T.norm_out = static_cast<float>(norm);
     }
     const uint32_t first = share_of(T.chunks, blockIdx.x, gridDim.x), end = share_of(T.chunks, blockIdx.x + 1, gridDim.x);
     if (first == end) return;
     // with clipping the norm has just walked the same shares front to back: their ends are still in L2
     const bool back = T.partials != nullptr;
-    int t = owner(T, back ? end - 1 : first);
-    for (uint32_t i = first; i < end; i++) {
-        const uint32_t chunk = back ? first + end - 1 - i : i;
-        while (chunk >= T.first[t + 1]) t++;
-        while (chunk < T.first[t]) t--;
-        const uint64_t n = T.n[t];
-        const Hyper& H = T.h[T.hyper[t] & 127];
-        const uint64_t start = (static_cast<uint64_t>(chunk - T.first[t]) * kWarps + warp) * kBlock;
-        if (start >= n) continue;
-        if ((T.hyper[t] & 128) && n - start >= kBlock) update_block<P, EIGHT, MASTER, true>(T, t, H, start, kBlock, clip, lane);
-        else update_block<P, EIGHT, MASTER, false>(T, t, H, start, n - start < kBlock ? static_cast<uint32_t>(n - start) : kBlock, clip, lane);
+    if constexpr (EIGHT) {
+        for (uint32_t i = first + warp; i < end; i += kWarps) update_run<P, MASTER>(T, back ? first + end - 1 - i : i, clip, lane);
+    } else {
+        const uint32_t at = static_cast<uint32_t>(warp) * kBlock;
+        int t = owner(T, back ? end - 1 : first);
+        for (uint32_t i = first; i < end; i++) {
+            const uint32_t chunk = back ? first + end - 1 - i : i;
+            while (chunk >= T.first[t + 1]) t++;
+            while (chunk < T.first[t]) t--;
+            const Hyper& H = T.h[T.hyper[t] & 127];
+            const uint64_t start = static_cast<uint64_t>(chunk - T.first[t]) * (kWarps * kBlock);
+            const uint64_t left = T.n[t] - start;
+            const Chunk<P> C = chunk_at<P, EIGHT, MASTER>(T, t, start);
+            Loaded<P, EIGHT, MASTER> L;
+            uint32_t none = 0;
+            if ((T.hyper[t] & 128) && left >= kWarps * kBlock) {
+                load_all<P, EIGHT, MASTER, true>(C, at, kBlock, lane, L);
+                update<P, EIGHT, MASTER, true>(H, start + at, clip, lane, L, 0, 0);
+                store_all<P, EIGHT, MASTER, true>(C, H, start + at, at, kBlock, lane, L.p, L.m, L.v, none, none);
+            } else if (at < left) {
+                const uint32_t have = left - at < kBlock ? static_cast<uint32_t>(left - at) : kBlock;
+                load_all<P, EIGHT, MASTER, false>(C, at, have, lane, L);
+                update<P, EIGHT, MASTER, false>(H, start + at, clip, lane, L, 0, 0);
+                store_all<P, EIGHT, MASTER, false>(C, H, start + at, at, have, lane, L.p, L.m, L.v, none, none);
+            }
+        }
     }
 }
 
 template <typename P, bool EIGHT, bool MASTER, int CAP>
 cudaError_t launch_table(const Table<CAP>& T, int sms, cudaStream_t s) {
-    const uint32_t cap = static_cast<uint32_t>(sms) * kCtasPerSm;
-    adamw_kernel<P, EIGHT, MASTER, CAP><<<T.chunks < cap ? T.chunks : cap, kThreads, 0, s>>>(T);
+    const uint32_t resident = static_cast<uint32_t>(sms) * ctas_per_sm<P, EIGHT, MASTER>();
+    const uint32_t units = EIGHT ? (T.chunks + kWarps - 1) / kWarps : T.chunks;
+    uint32_t grid = units < resident ? units : resident;
+    // Long steps: CTAs of four chunks each, which the hardware hands out as SMs become free. Equal shares of one resident
+    // grid ended at 123k to 172k cycles on different SMs (20M elements, 8-bit moments).
+    if (long_step(T.chunks, T.blocks, sms)) grid = EIGHT ? units : (units + 3) / 4;
+    adamw_kernel<P, EIGHT, MASTER, CAP><<<grid, kThreads, 0, s>>>(T);
     return cudaGetLastError();
 }
 
@@ -370,6 +513,7 @@ bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(
 template <int CAP>
 cudaError_t launch_all(const AdamwTensors& A, const AdamwHyper* hypers, int dtype, bool eight, bool master, const AdamwClip& clip, cudaStream_t s) {
     const int sms = sm_count();
+    bool factor_made = false;
     const uintptr_t wide = dtype == kDtypeF32 ? 32 : 16;
     int i = 0;
     while (i < A.count) {
@@ -411,10 +555,17 @@ cudaError_t launch_all(const AdamwTensors& A, const AdamwHyper* hypers, int dtyp
         }
         if (k == 0) return cudaSuccess;
         T.n_tensors = k;
+        uint64_t blocks = 0;
+        for (int j = 0; j < k; j++) blocks += (T.n[j] + kBlock - 1) / kBlock;
+        T.blocks = kWarps;
+        if (eight) {  // short steps are spread over as many warps as there are blocks
+            T.blocks = 1;
+            while (T.blocks < kMaxRun && blocks / T.blocks > static_cast<uint64_t>(sms) * 4 * kWarps * 4) T.blocks *= 2;
+        }
         uint64_t chunks = 0;
         for (int j = 0; j < k; j++) {
             T.first[j] = static_cast<uint32_t>(chunks);
-            const uint64_t per = static_cast<uint64_t>(kBlock) * kWarps;
+            const uint64_t per = static_cast<uint64_t>(kBlock) * T.blocks;
             chunks += (T.n[j] + per - 1) / per;
             if (chunks > 0xFFFFFFFFull - 65536) return cudaErrorInvalidValue;
         }
@@ -423,6 +574,12 @@ cudaError_t launch_all(const AdamwTensors& A, const AdamwHyper* hypers, int dtyp
         T.n_partials = clip.n_partials;
         T.max_norm = clip.max_norm;
         T.norm_out = clip.norm_out;
+        T.factor = nullptr;
+        if (clip.partials && long_step(T.chunks, T.blocks, sms)) {
+            if (!factor_made) clip_kernel<<<1, kThreads, 0, s>>>(clip.partials, clip.n_partials, clip.max_norm, clip.factor, clip.norm_out);
+            factor_made = true;
+            T.factor = clip.factor;
+        }
         cudaError_t e;
 #define FGS_ADAMW(P, M) (eight ? launch_table<P, true, M, CAP>(T, sms, s) : launch_table<P, false, M, CAP>(T, sms, s))
         if (dtype == kDtypeF32) e = FGS_ADAMW(float, false);
@@ -526,12 +683,9 @@ __device__ inline void read_blocks(const uint8_t* codes, const uint8_t* exps, O*
         for (int h = 0; h < 2; h++) {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                const uint32_t lo = k ? r[h].z : r[h].x, hi = k ? r[h].w : r[h].y;
-                uint32_t q[8];
+                const uint32_t q[2] = {k ? r[h].z : r[h].x, k ? r[h].w : r[h].y};
                 float x[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) q[j] = ((j < 4 ? lo : hi) >> (8 * (j & 3))) & 255u;
-                decode<SIGNED>(q, static_cast<int>(e[h]), x);
+                decode<SIGNED, true>(q, static_cast<int>(e[h]), x);
                 store8(out + start + h * 2 * kBlock + lane * 16 + 8 * k, x);
             }
         }
@@ -542,7 +696,7 @@ __device__ inline void read_blocks(const uint8_t* codes, const uint8_t* exps, O*
         uint32_t q[8];
         float x[8];
         load_codes<false>(codes + start + b * kBlock, lane, have, q);
-        decode<SIGNED>(q, exps[start / kBlock + b], x);
+        decode<SIGNED, false>(q, exps[start / kBlock + b], x);
         store_block<false>(out + start + b * kBlock, lane, have, x);
     }
 }

@@ -781,7 +781,7 @@ int fgs_adamw_step(const fgs_adamw_tensors* t, const fgs_adamw_hyper* hypers, in
         }
         const fgs::AdamwTensors A{static_cast<int>(t->count), t->param, t->grad, t->exp_avg, t->exp_avg_sq, t->exp_avg_exponent,
                                   t->exp_avg_sq_exponent, t->master, t->n_elements, t->hyper};
-        const fgs::AdamwClip clip{partials, n_partials, max_norm, grad_norm};
+        const fgs::AdamwClip clip{partials, n_partials, max_norm, grad_norm ? grad_norm + 1 : nullptr, grad_norm};
         ProfScope p_("adamw", static_cast<cudaStream_t>(stream));
         FGS_CUDA(fgs::launch_adamw(A, H.data(), dtype, eight, master, clip, static_cast<cudaStream_t>(stream)), "adamw");
     } catch (const std::exception& e) {

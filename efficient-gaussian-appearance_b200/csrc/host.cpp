@@ -252,7 +252,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                         room += need;
                     }
             partials = at::empty({room}, on.dtype(at::kDouble));
-            norm = at::empty({}, on.dtype(at::kFloat));
+            norm = at::empty({2}, on.dtype(at::kFloat));  // the norm, and room for the clip factor
             double* to = partials.data_ptr<double>();
             for (int code = 0; code < 3; code++)
                 for (auto& by_bits : jobs[code])
@@ -285,7 +285,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
             if (PyDict_SetItem(c.first, names.step, t.p)) throw PythonError();
         }
         if (!norm.defined()) Py_RETURN_NONE;
-        return THPVariable_Wrap(norm);
+        return THPVariable_Wrap(norm.select(0, 0));
     });
 }
 

@@ -132,6 +132,7 @@ struct AdamwTensors {
 struct AdamwClip {
     const double* partials; int n_partials;  // partials == nullptr: no clipping
     double max_norm;
+    float* factor;    // room for one float
     float* norm_out;
 };
 cudaError_t launch_adamw(const AdamwTensors& A, const AdamwHyper* hypers, int dtype, bool eight, bool master, const AdamwClip& clip, cudaStream_t s);

@@ -222,7 +222,7 @@ typedef struct {
     const int32_t* hyper;           /* index into the hyperparameter sets */
 } fgs_adamw_tensors;
 /* `partials`: the n_partials values of fgs_grad_squares (any number of its calls, one after another in one array), or
- * NULL for no clipping; grad_norm: one device float that receives the norm (needed with partials). */
+ * NULL for no clipping; grad_norm (needed with partials): two device floats, which receive the norm and the clip factor. */
 int fgs_adamw_step(const fgs_adamw_tensors* tensors, const fgs_adamw_hyper* hypers, int n_hypers, int dtype, int state_bits,
                    const double* partials, int n_partials, double max_norm, float* grad_norm, void* stream);
 /* partial sums of the squared elements of `count` tensors (types may differ), in a fixed order; *n_partials receives

@@ -7,12 +7,13 @@
 // Forward: one pass, bound by HBM (rows in, rows out). A CTA takes tiles of whole rows (or a part of a long one) in the
 // widest accesses that the row length and the addresses allow.
 //
-// Backward: no atomics, the same sums at every run. The tokens are sorted by index (stable radix sort, sort.cu: tokens
-// of one row keep their order), the sorted list is cut into chunks of C tokens, and a group of lanes walks each chunk
-// with a row's columns in registers: tokens of the same row follow each other, so their sum stays in fp32 registers. A row whose tokens
-// all lie in one chunk is written there. A row that crosses chunk borders leaves a partial sum per chunk (fp32), which
-// a second kernel adds up in the chunks' order. Rows without a token are set to zero by further CTAs of the first
-// kernel, which read one flag byte per row. Bound by HBM: g is read once, the gradient written once.
+// Backward: no atomics, the same sums at every run. The tokens are sorted by index (stably: tokens of one row keep their
+// order; one cluster up to 65536 tokens, sort.cu beyond), and the sorted list is cut into spans, one CTA each, and those
+// into chunks, one group of lanes each, which walks its chunk with a part of the columns in registers: tokens of one row
+// follow each other, so a row's sum stays in fp32 registers. Rows that cross chunks are put together in shared memory,
+// rows that cross spans leave one fp32 sum per span, which a second kernel adds up. Rows without a token are found by
+// binary search in the sorted list and cleared by further CTAs. Bound by HBM: g is read once, the gradient written once.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "launch.h"
@@ -116,29 +117,203 @@ int access_elements(const EmbeddingArgs& a, int size, const void* p, const void*
 // ---------------------------------------------------------------------------------------------------
 // gradient
 
-// sort keys (the row; `rows` for tokens that add to none), token numbers, and the flags of the rows that have a token
+// The indices as sort keys: the row, or `rows` for tokens that add to none.
+template <typename I>
+__device__ inline uint32_t key_of(I index, int64_t rows, int64_t padding) {
+    const uint32_t r = row_of(index, rows, padding);
+    return r < kBadRow ? r : static_cast<uint32_t>(rows);
+}
+
 template <typename I>
 __global__ void __launch_bounds__(kThreads) keys_kernel(const I* __restrict__ index, uint32_t tokens, int64_t rows, int64_t padding,
-                                                        uint32_t* __restrict__ keys, uint32_t* __restrict__ vals, uint8_t* __restrict__ used) {
+                                                        uint32_t* __restrict__ keys, uint32_t* __restrict__ vals) {
     const uint32_t t = blockIdx.x * kThreads + threadIdx.x;
     if (t >= tokens) return;
-    const uint32_t r = row_of(index[t], rows, padding);
-    keys[t] = r < kBadRow ? r : static_cast<uint32_t>(rows);
+    keys[t] = key_of(index[t], rows, padding);
     vals[t] = t;
-    if (r < kBadRow) used[r] = 1;
+}
+
+// Stable radix sort of up to 65536 indices in one launch: a cluster of up to 8 CTAs holds all (key, token) pairs in its
+// shared memory, each CTA a run of 1024 x ITEMS positions. Per pass of at most 8 bits: every warp ranks its keys by
+// ballots (a warp owns consecutive positions, so the order of equal digits is kept), the CTAs tell one another their
+// digit counts, and every pair is stored straight into its place in the shared memory of the CTA that owns the place.
+// Bound by latency (two cluster barriers per pass); as several launches over global memory the same sort of 32768
+// indices by 16 bits took 28 us.
+constexpr int kSortThreads = 1024, kSortWarps = 32, kDigits = 256, kMaxCluster = 8, kMaxItems = 8;
+constexpr int kRunStride = kDigits + 1;  // spreads the warps' counts of one digit over the banks
+constexpr uint32_t kClusterSortMax = kSortThreads * kMaxItems * kMaxCluster;
+
+size_t cluster_sort_smem(int items) {
+    return 2 * sizeof(uint64_t) * kSortThreads * static_cast<size_t>(items) + sizeof(uint32_t) * (kSortWarps * kRunStride + kMaxCluster * kDigits + 2 * kDigits);
+}
+
+template <typename I, int ITEMS>
+__global__ void __launch_bounds__(kSortThreads, 1) cluster_sort_kernel(const I* __restrict__ index, uint32_t tokens, int64_t rows, int64_t padding,
+                                                                       int end_bit, uint32_t* __restrict__ keys, uint32_t* __restrict__ vals) {
+    namespace cg = cooperative_groups;
+    extern __shared__ uint64_t pairs[];  // two buffers of kSortThreads * ITEMS pairs: key in the high word
+    constexpr uint32_t kRun = kSortThreads * ITEMS;
+    uint32_t* run = reinterpret_cast<uint32_t*>(pairs + 2 * kRun);  // [warp][digit]
+    uint32_t* counts = run + kSortWarps * kRunStride;               // [CTA][digit]
+    uint32_t* base = counts + kMaxCluster * kDigits;                // first place of this CTA's keys of each digit
+    uint32_t* totals = base + kDigits;
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t rank = cluster.block_rank(), ctas = cluster.num_blocks();
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const uint32_t first = rank * kRun + static_cast<uint32_t>(warp) * (32 * ITEMS) + lane;  // this thread's places: first + 32 j
+    uint32_t key[ITEMS], val[ITEMS];
+#pragma unroll
+    for (int j = 0; j < ITEMS; j++) {
+        const uint32_t p = first + 32 * j;
+        val[j] = p;
+        key[j] = p < tokens ? key_of(index[p], rows, padding) : 0xFFFFFFFFu;  // sorts behind all others, which came before it
+    }
+    const int passes = (end_bit + 7) / 8, bits = (end_bit + passes - 1) / passes;
+    const uint32_t mask = (1u << bits) - 1u;
+    cluster.sync();  // every CTA runs before its shared memory is written to
+    for (int pass = 0; pass < passes; pass++) {
+        const int shift = pass * bits;
+        uint64_t* to = pairs + (pass & 1) * kRun;
+        for (int i = t; i < kSortWarps * kRunStride; i += kSortThreads) run[i] = 0;
+        __syncthreads();
+        uint32_t place[ITEMS];
+        uint32_t* mine = run + warp * kRunStride;
+#pragma unroll
+        for (int j = 0; j < ITEMS; j++) {
+            const uint32_t d = (key[j] >> shift) & mask;
+            uint32_t same = 0xFFFFFFFFu;
+#pragma unroll
+            for (int b = 0; b < 8; b++) {
+                if (b >= bits) break;
+                const bool set = (d >> b) & 1u;
+                const uint32_t with = __ballot_sync(0xFFFFFFFFu, set);
+                same &= set ? with : ~with;
+            }
+            const uint32_t before = __popc(same & ((1u << lane) - 1u));
+            const uint32_t prior = mine[d];
+            place[j] = prior + before;
+            __syncwarp();
+            if (before == 0) mine[d] = prior + __popc(same);
+            __syncwarp();
+        }
+        __syncthreads();
+        // four threads per digit: exclusive sums of its counts over the warps, and the CTA's count, told to every CTA
+        {
+            const int d = t >> 2, q = t & 3;
+            uint32_t c[8], sum = 0;
+#pragma unroll
+            for (int w = 0; w < 8; w++) {
+                c[w] = run[(8 * q + w) * kRunStride + d];
+                sum += c[w];
+            }
+            uint32_t incl = sum;
+            for (int o = 1; o < 4; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, incl, o, 4);
+                if (q >= o) incl += y;
+            }
+            uint32_t at = incl - sum;
+#pragma unroll
+            for (int w = 0; w < 8; w++) {
+                run[(8 * q + w) * kRunStride + d] = at;
+                at += c[w];
+            }
+            const uint32_t total = __shfl_sync(0xFFFFFFFFu, incl, 3, 4);
+            for (uint32_t r = q; r < ctas; r += 4) cluster.map_shared_rank(counts, r)[rank * kDigits + d] = total;
+        }
+        cluster.sync();
+        if (t < kDigits) {
+            uint32_t before = 0, all = 0;
+            for (uint32_t r = 0; r < ctas; r++) {
+                const uint32_t c = counts[r * kDigits + t];
+                before += r < rank ? c : 0u;
+                all += c;
+            }
+            base[t] = before;
+            uint32_t incl = all;  // inclusive sum over the warp's digits
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            if (lane == 31) totals[warp] = incl;
+            base[t] += incl - all;
+        }
+        __syncthreads();
+        if (t < kDigits) {
+            uint32_t before = 0;
+            for (int w = 0; w < warp; w++) before += totals[w];
+            base[t] += before;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < ITEMS; j++) {
+            const uint32_t d = (key[j] >> shift) & mask;
+            const uint32_t p = base[d] + mine[d] + place[j];
+            cluster.map_shared_rank(to, p / kRun)[p % kRun] = static_cast<uint64_t>(key[j]) << 32 | val[j];
+        }
+        cluster.sync();
+#pragma unroll
+        for (int j = 0; j < ITEMS; j++) {
+            const uint64_t x = to[warp * (32 * ITEMS) + 32 * j + lane];
+            key[j] = static_cast<uint32_t>(x >> 32);
+            val[j] = static_cast<uint32_t>(x);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < ITEMS; j++) {
+        const uint32_t p = first + 32 * j;
+        if (p < tokens) {
+            keys[p] = key[j];
+            vals[p] = val[j];
+        }
+    }
+}
+
+template <typename I, int ITEMS>
+cudaError_t launch_cluster_sort(const EmbeddingArgs& a, const void* index, int end_bit, uint32_t* keys, uint32_t* vals, cudaStream_t s) {
+    const uint32_t per = kSortThreads * ITEMS;
+    uint32_t ctas = 1;
+    while (ctas * per < static_cast<uint32_t>(a.tokens)) ctas *= 2;
+    const size_t smem = cluster_sort_smem(ITEMS);
+    cudaError_t e = cudaFuncSetAttribute(cluster_sort_kernel<I, ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(ctas);
+    config.blockDim = dim3(kSortThreads);
+    config.dynamicSmemBytes = smem;
+    config.stream = s;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = ctas;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, cluster_sort_kernel<I, ITEMS>, static_cast<const I*>(index), static_cast<uint32_t>(a.tokens), a.rows, a.padding,
+                              end_bit, keys, vals);
+}
+
+// as many CTAs as a cluster has before each takes more than 1024 indices
+template <typename I>
+cudaError_t cluster_sort(const EmbeddingArgs& a, const void* index, int end_bit, uint32_t* keys, uint32_t* vals, cudaStream_t s) {
+    const uint32_t most = kSortThreads * kMaxCluster;
+    if (a.tokens <= most) return launch_cluster_sort<I, 1>(a, index, end_bit, keys, vals, s);
+    if (a.tokens <= 2 * most) return launch_cluster_sort<I, 2>(a, index, end_bit, keys, vals, s);
+    if (a.tokens <= 4 * most) return launch_cluster_sort<I, 4>(a, index, end_bit, keys, vals, s);
+    return launch_cluster_sort<I, 8>(a, index, end_bit, keys, vals, s);
 }
 
 struct SumArgs {
     const uint32_t* keys;    // sorted rows
     const uint32_t* tokens;  // their tokens
-    const uint8_t* used;
-    float* head;             // [chunks][width] partial sum of the row that began in an earlier chunk
-    float* tail;             // [chunks][width] partial sum of the row that goes on in the next chunk
-    uint32_t n, rows, units, chunk, chunks;
-    uint32_t lanes, groups;  // lanes of a group (a power of two, at most 32), column parts of a row
-    uint32_t sum_ctas;
+    float* head;             // [spans][width] sum within a CTA's span of the row that began before it
+    float* tail;             // [spans][width] sum within the span of the row that goes on behind it
+    uint32_t n, rows, units;
+    uint32_t lanes, parts;   // lanes of a group (a power of two, at most 32), column parts of a row
+    uint32_t chunk, span, spans;  // sorted positions of a group and of a CTA; CTAs per column part
+    uint32_t zero_rows;      // rows that a clearing CTA looks at
     float scale;
 };
+
+constexpr uint32_t kNone = 0xFFFFFFFFu;  // no key
 
 template <typename P, int N>
 __device__ inline void write_row(P* grad, uint64_t row, uint32_t units, uint32_t col, const float (&acc)[N], float scale) {
@@ -148,154 +323,224 @@ __device__ inline void write_row(P* grad, uint64_t row, uint32_t units, uint32_t
     reinterpret_cast<typename Pack<P, N>::A*>(grad)[row * units + col] = x.raw;
 }
 
-// One group of `lanes` lanes per (chunk, part of the columns).
+// clears the rows without a token among `zero_rows` rows
 template <typename P, int N>
-__global__ void __launch_bounds__(kThreads) sum_kernel(const P* __restrict__ g, P* __restrict__ grad, const SumArgs a) {
+__device__ inline void clear_rows(P* grad, const SumArgs& a, uint32_t cta, uint8_t* used) {
     using A = typename Pack<P, N>::A;
-    if (blockIdx.x >= a.sum_ctas) {  // rows without a token
-        const uint64_t total = static_cast<uint64_t>(a.rows) * a.units;
-        const uint64_t stride = static_cast<uint64_t>(gridDim.x - a.sum_ctas) * kThreads;
-        Pack<P, N> zero;
-#pragma unroll
-        for (int j = 0; j < N; j++) zero.x[j] = from_float<P>(0.0f);
-        for (uint64_t u = static_cast<uint64_t>(blockIdx.x - a.sum_ctas) * kThreads + threadIdx.x; u < total; u += stride)
-            if (!a.used[u / a.units]) reinterpret_cast<A*>(grad)[u] = zero.raw;
-        return;
-    }
-    const uint64_t worker = (static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x) / a.lanes;
-    const uint32_t chunk = static_cast<uint32_t>(worker / a.groups);
-    const uint32_t col = static_cast<uint32_t>(worker % a.groups) * a.lanes + threadIdx.x % a.lanes;
-    if (chunk >= a.chunks || col >= a.units) return;
-    const uint32_t p0 = chunk * a.chunk;
-    const uint32_t p1 = a.n - p0 < a.chunk ? a.n : p0 + a.chunk;
-    const A* src = reinterpret_cast<const A*>(g);
-    const uint32_t width = a.units * N;
-    bool first = p0 > 0 && a.keys[p0 - 1] == a.keys[p0];  // the running row began in an earlier chunk
-    uint32_t row = a.keys[p0];
-    float acc[N];
-#pragma unroll
-    for (int j = 0; j < N; j++) acc[j] = 0.0f;
-    constexpr int kAhead = 8;
-    for (uint32_t p = p0; p < p1 && row < a.rows; p += kAhead) {
-        Pack<P, N> x[kAhead];
-        uint32_t key[kAhead];
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            key[k] = a.rows;
-            if (p + k >= p1) continue;
-            key[k] = a.keys[p + k];
-            if (key[k] < a.rows) x[k].raw = src[static_cast<uint64_t>(a.tokens[p + k]) * a.units + col];
+    const uint32_t first = cta * a.zero_rows, count = a.rows - first < a.zero_rows ? a.rows - first : a.zero_rows;
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+        const uint32_t row = first + i;
+        uint32_t lo = 0, hi = a.n;  // the first position whose key is not below the row
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (a.keys[mid] < row) lo = mid + 1;
+            else hi = mid;
         }
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            if (p + k >= p1) break;
-            if (key[k] != row) {  // the row ends here
-                if (first) {
-#pragma unroll
-                    for (int j = 0; j < N; j++) a.head[static_cast<uint64_t>(chunk) * width + col * N + j] = acc[j];
-                } else {
-                    write_row<P, N>(grad, row, a.units, col, acc, a.scale);
-                }
-                first = false;
-                row = key[k];
-#pragma unroll
-                for (int j = 0; j < N; j++) acc[j] = 0.0f;
-                if (row >= a.rows) break;
-            }
-#pragma unroll
-            for (int j = 0; j < N; j++) acc[j] += to_float(x[k].x[j]);
-        }
+        used[i] = lo < a.n && a.keys[lo] == row;
     }
-    if (row >= a.rows) return;
-    const bool on = p1 < a.n && a.keys[p1] == row;
-    if (first || on) {
-        float* to = first ? a.head : a.tail;
+    __syncthreads();
+    Pack<P, N> zero;
 #pragma unroll
-        for (int j = 0; j < N; j++) to[static_cast<uint64_t>(chunk) * width + col * N + j] = acc[j];
+    for (int j = 0; j < N; j++) zero.x[j] = from_float<P>(0.0f);
+    A* to = reinterpret_cast<A*>(grad) + static_cast<uint64_t>(first) * a.units;
+    if (a.units >= kThreads) {
+        for (uint32_t i = 0; i < count; i++) {
+            if (used[i]) continue;
+            for (uint32_t u = threadIdx.x; u < a.units; u += kThreads) to[static_cast<uint64_t>(i) * a.units + u] = zero.raw;
+        }
     } else {
-        write_row<P, N>(grad, row, a.units, col, acc, a.scale);
+        for (uint32_t u = threadIdx.x; u < count * a.units; u += kThreads)
+            if (!used[u / a.units]) to[u] = zero.raw;
     }
 }
 
-// Adds the partial sums of each row that crosses a chunk border: the CTA's warps look at 256 chunks for rows that begin
-// in them and go on, and then sum each of those with all threads: slots of `lanes` lanes take the row's chunks in turn,
-// and the slots' sums are added in order.
+// A CTA takes a span of sorted positions and a part of the columns; its groups of lanes take a chunk of the span each.
+// Within a group a row's sum stays in registers; rows that cross chunk borders are put together in shared memory, by
+// doubling along the groups that lie whole within the row.
 template <typename P, int N>
-__global__ void __launch_bounds__(kThreads) join_kernel(P* __restrict__ grad, const SumArgs a) {
-    __shared__ uint32_t found[32];
-    __shared__ uint32_t last[32];
-    __shared__ int n_found;
+__global__ void __launch_bounds__(kThreads) sum_kernel(const P* __restrict__ g, P* __restrict__ grad, const SumArgs a) {
+    using A = typename Pack<P, N>::A;
+    extern __shared__ uint32_t staged[];  // the span's keys with one more on either side, and its tokens
     __shared__ float part[kThreads * N];
-    const uint32_t width = a.units * N;
-    if (threadIdx.x == 0) n_found = 0;
-    if (threadIdx.x < 32) {
-        const uint32_t chunk = blockIdx.x * 32 + threadIdx.x;
-        bool starts = false;
-        uint32_t end = 0;
-        if (chunk < a.chunks) {
-            const uint64_t p0 = static_cast<uint64_t>(chunk) * a.chunk, p1 = p0 + a.chunk;
-            if (p1 < a.n) {
-                const uint32_t row = a.keys[p1 - 1];
-                starts = row < a.rows && a.keys[p1] == row && !(p0 > 0 && a.keys[p0] == row && a.keys[p0 - 1] == row);
-                if (starts) {  // the first position past p1 with another row
-                    uint32_t lo = static_cast<uint32_t>(p1), hi = a.n;
-                    while (hi - lo > 1) {
-                        const uint32_t mid = lo + (hi - lo) / 2;
-                        if (a.keys[mid] == row) lo = mid;
-                        else hi = mid;
-                    }
-                    end = lo / a.chunk;
-                }
-            }
-        }
-        const uint32_t mask = __ballot_sync(0xffffffffu, starts);
-        if (starts) {
-            const int at = __popc(mask & ((1u << threadIdx.x) - 1u));
-            found[at] = chunk;
-            last[at] = end;
-        }
-        if (threadIdx.x == 0) n_found = __popc(mask);
+    __shared__ uint8_t full[kThreads];    // group: its head row goes on in the next group
+    const uint32_t sum_ctas = a.spans * a.parts;
+    if (blockIdx.x >= sum_ctas) {
+        clear_rows<P, N>(grad, a, blockIdx.x - sum_ctas, reinterpret_cast<uint8_t*>(part));
+        return;
+    }
+    const uint32_t span = blockIdx.x / a.parts, column_part = blockIdx.x % a.parts;
+    const uint32_t p0 = span * a.span, have = a.n - p0 < a.span ? a.n - p0 : a.span;
+    uint32_t* keys = staged + 1;
+    uint32_t* tokens = keys + a.span + 1;
+    for (uint32_t i = threadIdx.x; i < have; i += kThreads) {
+        keys[i] = a.keys[p0 + i];
+        tokens[i] = a.tokens[p0 + i];
+    }
+    if (threadIdx.x == 0) {
+        staged[0] = p0 > 0 ? a.keys[p0 - 1] : kNone;
+        keys[have] = p0 + have < a.n ? a.keys[p0 + have] : kNone;
     }
     __syncthreads();
-    const uint32_t slots = kThreads / a.lanes, slot = threadIdx.x / a.lanes;
-    const uint32_t col = blockIdx.y * a.lanes + threadIdx.x % a.lanes;
-    for (int f = 0; f < n_found; f++) {
-        float acc[N];
+    const uint32_t lane = threadIdx.x % a.lanes, group = threadIdx.x / a.lanes;
+    const uint32_t col = column_part * a.lanes + lane;
+    const uint32_t c0 = group * a.chunk, c1 = c0 + a.chunk < have ? c0 + a.chunk : have;
+    const bool live = c0 < have && col < a.units;
+    const A* src = reinterpret_cast<const A*>(g) + col;
+    float acc[N], head[N];  // the running row; the row that the group began within
 #pragma unroll
-        for (int j = 0; j < N; j++) acc[j] = 0.0f;
-        if (col < a.units) {
-            if (slot == 0) {
+    for (int j = 0; j < N; j++) acc[j] = head[j] = 0.0f;
+    uint32_t row = a.rows;
+    bool first = false, on = false;
+    if (live) {
+        row = keys[c0];
+        first = row < a.rows && keys[static_cast<int>(c0) - 1] == row;
+        bool began = first;  // the running row began before the group
+        constexpr int kAhead = 8;
+        for (uint32_t p = c0; p < c1 && row < a.rows; p += kAhead) {
+            Pack<P, N> x[kAhead];
+            uint32_t key[kAhead];
 #pragma unroll
-                for (int j = 0; j < N; j++) acc[j] = a.tail[static_cast<uint64_t>(found[f]) * width + col * N + j];
+            for (int k = 0; k < kAhead; k++) {
+                key[k] = p + k < c1 ? keys[p + k] : a.rows;
+                if (key[k] < a.rows) x[k].raw = src[static_cast<uint64_t>(tokens[p + k]) * a.units];
             }
-#pragma unroll 4
-            for (uint32_t c = found[f] + 1 + slot; c <= last[f]; c += slots) {
 #pragma unroll
-                for (int j = 0; j < N; j++) acc[j] += a.head[static_cast<uint64_t>(c) * width + col * N + j];
+            for (int k = 0; k < kAhead; k++) {
+                if (p + k >= c1) break;
+                if (key[k] != row) {  // the row ends here
+                    if (began) {
+#pragma unroll
+                        for (int j = 0; j < N; j++) head[j] = acc[j];
+                    } else {
+                        write_row<P, N>(grad, row, a.units, col, acc, a.scale);
+                    }
+                    began = false;
+                    row = key[k];
+#pragma unroll
+                    for (int j = 0; j < N; j++) acc[j] = 0.0f;
+                    if (row >= a.rows) break;
+                }
+#pragma unroll
+                for (int j = 0; j < N; j++) acc[j] += to_float(x[k].x[j]);
             }
         }
+        on = row < a.rows && keys[c1] == row;
+        if (row < a.rows) {
+            if (began) {  // one row only
 #pragma unroll
-        for (int j = 0; j < N; j++) part[threadIdx.x * N + j] = acc[j];
-        __syncthreads();
-        for (uint32_t half = slots / 2; half > 0; half /= 2) {
-            if (slot < half) {
+                for (int j = 0; j < N; j++) head[j] = acc[j];
+            } else if (!on) {
+                write_row<P, N>(grad, row, a.units, col, acc, a.scale);
+            }
+        }
+        // from here on: first: the group has a head; through: it is all one row, which goes on; on && !through: it has a tail
+        on = on && !began;
+        if (lane == 0) full[group] = began && row < a.rows && keys[c1] == row;
+    } else if (lane == 0) {
+        full[group] = 0;
+    }
+    const uint32_t groups = kThreads / a.lanes;
 #pragma unroll
-                for (int j = 0; j < N; j++) part[threadIdx.x * N + j] += part[(threadIdx.x + half * a.lanes) * N + j];
+    for (int j = 0; j < N; j++) part[j * kThreads + threadIdx.x] = head[j];
+    bool through = false;
+    __syncthreads();
+    through = full[group];
+    if (__syncthreads_or(through)) {  // heads behind one another: add them up along the groups
+        for (uint32_t d = 1; d < groups; d *= 2) {
+            float more[N];
+            bool linked = through && group + d < groups;
+            if (linked) {
+#pragma unroll
+                for (int j = 0; j < N; j++) more[j] = part[j * kThreads + threadIdx.x + d * a.lanes];
+            }
+            const bool next = linked && full[group + d];
+            __syncthreads();
+            if (linked) {
+#pragma unroll
+                for (int j = 0; j < N; j++) part[j * kThreads + threadIdx.x] += more[j];
+                through = next;
+                if (lane == 0) full[group] = next;
             }
             __syncthreads();
         }
-        if (slot == 0 && col < a.units) {
-#pragma unroll
-            for (int j = 0; j < N; j++) acc[j] = part[threadIdx.x * N + j];
-            write_row<P, N>(grad, a.keys[static_cast<uint64_t>(found[f] + 1) * a.chunk], a.units, col, acc, a.scale);
-        }
-        __syncthreads();
     }
+    // full[g]: the chain of heads from group g reaches the span's end and goes on behind it
+    if (!live) return;
+    const uint32_t width = a.units * N;
+    if (on) {  // a row that begins in this group: its sum so far, and the heads behind it
+        bool leaves = group + 1 == groups || c1 == have;
+        if (!leaves) {
+#pragma unroll
+            for (int j = 0; j < N; j++) acc[j] += part[j * kThreads + threadIdx.x + a.lanes];
+            leaves = full[group + 1];
+        }
+        if (leaves) {
+#pragma unroll
+            for (int j = 0; j < N; j++) a.tail[static_cast<uint64_t>(span) * width + col * N + j] = acc[j];
+        } else {
+            write_row<P, N>(grad, row, a.units, col, acc, a.scale);
+        }
+    }
+    if (group == 0 && first) {
+#pragma unroll
+        for (int j = 0; j < N; j++) a.head[static_cast<uint64_t>(span) * width + col * N + j] = part[j * kThreads + threadIdx.x];
+    }
+}
+
+// Adds the spans' sums of each row that crosses span borders. A CTA looks at one span for a row that begins in it and
+// goes on; slots of `lanes` lanes take the row's spans in turn, and the slots' sums are added pairwise.
+template <typename P, int N>
+__global__ void __launch_bounds__(kThreads) join_kernel(P* __restrict__ grad, const SumArgs a) {
+    __shared__ float part[kThreads * N];
+    const uint32_t span = blockIdx.x;
+    const uint64_t p0 = static_cast<uint64_t>(span) * a.span, p1 = p0 + a.span;
+    if (p1 >= a.n) return;
+    const uint32_t row = a.keys[p1];
+    if (row >= a.rows || a.keys[p1 - 1] != row || (p0 > 0 && a.keys[p0 - 1] == row)) return;
+    uint32_t lo = static_cast<uint32_t>(p1), hi = a.n;  // the row's last position
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (a.keys[mid] == row) lo = mid;
+        else hi = mid;
+    }
+    const uint32_t last = lo / a.span, width = a.units * N;
+    const uint32_t slots = kThreads / a.lanes, slot = threadIdx.x / a.lanes;
+    const uint32_t col = blockIdx.y * a.lanes + threadIdx.x % a.lanes;
+    float acc[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) acc[j] = 0.0f;
+    if (col < a.units) {
+        if (slot == 0) {
+#pragma unroll
+            for (int j = 0; j < N; j++) acc[j] = a.tail[static_cast<uint64_t>(span) * width + col * N + j];
+        }
+#pragma unroll 4
+        for (uint32_t c = span + 1 + slot; c <= last; c += slots) {
+#pragma unroll
+            for (int j = 0; j < N; j++) acc[j] += a.head[static_cast<uint64_t>(c) * width + col * N + j];
+        }
+    }
+    uint32_t busy = slots;  // slots that may hold a sum
+    while (busy > 1 && busy / 2 >= last - span) busy /= 2;
+    if (busy > 1) {
+#pragma unroll
+        for (int j = 0; j < N; j++) part[j * kThreads + threadIdx.x] = acc[j];
+        __syncthreads();
+        for (uint32_t half = busy / 2; half > 0; half /= 2) {
+            if (slot < half) {
+#pragma unroll
+                for (int j = 0; j < N; j++) part[j * kThreads + threadIdx.x] += part[j * kThreads + threadIdx.x + half * a.lanes];
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++) acc[j] = part[j * kThreads + threadIdx.x];
+    }
+    if (slot == 0 && col < a.units) write_row<P, N>(grad, row, a.units, col, acc, a.scale);
 }
 
 struct GradBuffers {
     uint32_t *keys_a, *keys_b, *vals_a, *vals_b;
-    uint8_t* used;
     void* sort_temp;
     size_t sort_bytes;
     float *head, *tail;
@@ -310,15 +555,28 @@ int bits_of(uint64_t x) {
     return b;
 }
 
-// tokens of a chunk: enough chunks to give each of 148 x 2048 threads a column, between 8 and 256 tokens
-uint32_t chunk_of(uint64_t tokens, uint64_t width) {
-    const uint64_t c = tokens * ((width + 3) / 4) / (148ull * 2048ull);
-    uint32_t p = 8;
-    while (p < c && p < 256) p *= 2;
-    return p;
+// How the sorted tokens are cut: enough groups to give each of 148 x 2048 threads a column, 8 to 64 positions each, and
+// at most 4096 positions (their keys and tokens are staged in shared memory) per CTA.
+void cut(uint64_t tokens, uint64_t units, SumArgs* S) {
+    S->lanes = 1;
+    while (S->lanes < 32 && S->lanes < units) S->lanes *= 2;
+    S->parts = static_cast<uint32_t>((units + S->lanes - 1) / S->lanes);
+    const uint32_t groups = kThreads / S->lanes;
+    const uint64_t want = tokens * units / (148ull * 2048ull);
+    S->chunk = 8;
+    while (S->chunk < want && S->chunk < 64 && S->chunk * 2 * groups <= 4096) S->chunk *= 2;
+    S->span = S->chunk * groups;
+    S->spans = static_cast<uint32_t>((tokens + S->span - 1) / S->span);
 }
 
-size_t carve(void* ws, uint64_t tokens, uint64_t rows, uint64_t width, GradBuffers* B) {
+// access width of the rows in elements: the widest (at most 16 bytes) that divides a row
+int row_elements(uint64_t width, int size) {
+    int n = 16 / size;
+    while (width % static_cast<uint64_t>(n)) n /= 2;
+    return n;
+}
+
+size_t carve(void* ws, uint64_t tokens, uint64_t rows, uint64_t width, int size, GradBuffers* B) {
     char* base = static_cast<char*>(ws);
     size_t off = 0;
     const auto take = [&](size_t bytes) {
@@ -328,16 +586,22 @@ size_t carve(void* ws, uint64_t tokens, uint64_t rows, uint64_t width, GradBuffe
         return p;
     };
     GradBuffers b;
+    const bool small = tokens <= kClusterSortMax;
     b.keys_a = reinterpret_cast<uint32_t*>(take(4 * tokens));
-    b.keys_b = reinterpret_cast<uint32_t*>(take(4 * tokens));
     b.vals_a = reinterpret_cast<uint32_t*>(take(4 * tokens));
-    b.vals_b = reinterpret_cast<uint32_t*>(take(4 * tokens));
-    b.used = reinterpret_cast<uint8_t*>(take(rows));
-    b.sort_bytes = tile_sort_temp_bytes(tokens, 32, true);
+    b.keys_b = reinterpret_cast<uint32_t*>(take(small ? 0 : 4 * tokens));
+    b.vals_b = reinterpret_cast<uint32_t*>(take(small ? 0 : 4 * tokens));
+    b.sort_bytes = small ? 0 : tile_sort_temp_bytes(tokens, 32, true);
     b.sort_temp = take(b.sort_bytes);
-    const uint64_t chunk = chunk_of(tokens, width), chunks = (tokens + chunk - 1) / chunk;
-    b.head = reinterpret_cast<float*>(take(4 * chunks * width));
-    b.tail = reinterpret_cast<float*>(take(4 * chunks * width));
+    // narrower accesses (misaligned addresses) make more units and longer chunks, never more spans
+    uint64_t spans = 1;
+    for (int n = row_elements(width, size); n >= 1; n /= 2) {
+        SumArgs S{};
+        cut(tokens, width / n, &S);
+        spans = S.spans > spans ? S.spans : spans;
+    }
+    b.head = reinterpret_cast<float*>(take(4 * spans * width));
+    b.tail = reinterpret_cast<float*>(take(4 * spans * width));
     if (B) *B = b;
     return off;
 }
@@ -347,20 +611,18 @@ cudaError_t launch_sums(const EmbeddingArgs& a, const void* g, void* grad, SumAr
     const uint64_t units = static_cast<uint64_t>(a.width) / N;
     if (units > 0x7FFFFFFFull) return cudaErrorInvalidValue;
     S.units = static_cast<uint32_t>(units);
-    S.lanes = 1;
-    while (S.lanes < 32 && S.lanes < units) S.lanes *= 2;
-    S.groups = static_cast<uint32_t>((units + S.lanes - 1) / S.lanes);
-    const uint64_t threads = static_cast<uint64_t>(S.chunks) * S.groups * S.lanes;
-    const uint64_t sum_ctas = (threads + kThreads - 1) / kThreads;
-    const uint64_t cells = static_cast<uint64_t>(a.rows) * units;
-    const uint64_t zero_ctas = cells / (kThreads * 8) + 1 < 148 * 8 ? cells / (kThreads * 8) + 1 : 148 * 8;
-    if (sum_ctas + zero_ctas > 0x7FFFFFFFull || S.groups > 65535) return cudaErrorInvalidValue;
-    S.sum_ctas = static_cast<uint32_t>(sum_ctas);
-    sum_kernel<P, N><<<static_cast<unsigned>(sum_ctas + zero_ctas), kThreads, 0, s>>>(static_cast<const P*>(g), static_cast<P*>(grad), S);
+    cut(static_cast<uint64_t>(a.tokens), units, &S);
+    uint64_t zero_rows = 8192 / units;  // about 128 KB of a CTA's rows
+    zero_rows = zero_rows < 1 ? 1 : zero_rows > kThreads ? kThreads : zero_rows;
+    S.zero_rows = static_cast<uint32_t>(zero_rows);
+    const uint64_t ctas = static_cast<uint64_t>(S.spans) * S.parts + (static_cast<uint64_t>(a.rows) + zero_rows - 1) / zero_rows;
+    if (ctas > 0x7FFFFFFFull || S.parts > 65535) return cudaErrorInvalidValue;
+    const size_t smem = sizeof(uint32_t) * (2 * static_cast<size_t>(S.span) + 2);
+    sum_kernel<P, N><<<static_cast<unsigned>(ctas), kThreads, smem, s>>>(static_cast<const P*>(g), static_cast<P*>(grad), S);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    if (S.chunks > 1) {
-        join_kernel<P, N><<<dim3((S.chunks + 31) / 32, S.groups), kThreads, 0, s>>>(static_cast<P*>(grad), S);
+    if (S.spans > 1) {
+        join_kernel<P, N><<<dim3(S.spans, S.parts), kThreads, 0, s>>>(static_cast<P*>(grad), S);
         e = cudaGetLastError();
     }
     return e;
@@ -389,7 +651,12 @@ cudaError_t launch_embedding_lookup(const EmbeddingArgs& a, const void* table, c
 }
 
 size_t embedding_workspace_bytes(int64_t tokens, int64_t rows, int64_t width) {
-    return carve(nullptr, static_cast<uint64_t>(tokens), static_cast<uint64_t>(rows), static_cast<uint64_t>(width), nullptr);
+    size_t most = 0;  // for any type
+    for (int size = 2; size <= 4; size *= 2) {
+        const size_t b = carve(nullptr, static_cast<uint64_t>(tokens), static_cast<uint64_t>(rows), static_cast<uint64_t>(width), size, nullptr);
+        most = b > most ? b : most;
+    }
+    return most;
 }
 
 cudaError_t launch_embedding_grad(const EmbeddingArgs& a, const void* index, const void* g, void* grad, void* ws, cudaStream_t s) {
@@ -397,29 +664,31 @@ cudaError_t launch_embedding_grad(const EmbeddingArgs& a, const void* index, con
     const int size = a.dtype == kDtypeF32 ? 4 : 2;
     if (a.tokens == 0) return cudaMemsetAsync(grad, 0, static_cast<size_t>(a.rows) * static_cast<size_t>(a.width) * static_cast<size_t>(size), s);
     GradBuffers B;
-    carve(ws, static_cast<uint64_t>(a.tokens), static_cast<uint64_t>(a.rows), static_cast<uint64_t>(a.width), &B);
+    carve(ws, static_cast<uint64_t>(a.tokens), static_cast<uint64_t>(a.rows), static_cast<uint64_t>(a.width), size, &B);
     const uint32_t tokens = static_cast<uint32_t>(a.tokens);
-    cudaError_t e = cudaMemsetAsync(B.used, 0, static_cast<size_t>(a.rows), s);
-    if (e != cudaSuccess) return e;
-    const unsigned ctas = (tokens + kThreads - 1) / kThreads;
-    if (a.wide_index) keys_kernel<<<ctas, kThreads, 0, s>>>(static_cast<const int64_t*>(index), tokens, a.rows, a.padding, B.keys_a, B.vals_a, B.used);
-    else keys_kernel<<<ctas, kThreads, 0, s>>>(static_cast<const int32_t*>(index), tokens, a.rows, a.padding, B.keys_a, B.vals_a, B.used);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    const void* keys = nullptr;
-    const uint32_t* vals = nullptr;
-    e = tile_sort(B.keys_a, B.keys_b, B.vals_a, B.vals_b, tokens, bits_of(static_cast<uint64_t>(a.rows)), true, B.sort_temp, B.sort_bytes, &keys, &vals, s);
-    if (e != cudaSuccess) return e;
+    const int end_bit = bits_of(static_cast<uint64_t>(a.rows));
     SumArgs S{};
-    S.keys = static_cast<const uint32_t*>(keys);
-    S.tokens = vals;
-    S.used = B.used;
+    cudaError_t e;
+    if (tokens <= kClusterSortMax) {
+        e = a.wide_index ? cluster_sort<int64_t>(a, index, end_bit, B.keys_a, B.vals_a, s) : cluster_sort<int32_t>(a, index, end_bit, B.keys_a, B.vals_a, s);
+        if (e != cudaSuccess) return e;
+        S.keys = B.keys_a;
+        S.tokens = B.vals_a;
+    } else {
+        const unsigned ctas = (tokens + kThreads - 1) / kThreads;
+        if (a.wide_index) keys_kernel<<<ctas, kThreads, 0, s>>>(static_cast<const int64_t*>(index), tokens, a.rows, a.padding, B.keys_a, B.vals_a);
+        else keys_kernel<<<ctas, kThreads, 0, s>>>(static_cast<const int32_t*>(index), tokens, a.rows, a.padding, B.keys_a, B.vals_a);
+        e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        const void* keys = nullptr;
+        e = tile_sort(B.keys_a, B.keys_b, B.vals_a, B.vals_b, tokens, end_bit, true, B.sort_temp, B.sort_bytes, &keys, &S.tokens, s);
+        if (e != cudaSuccess) return e;
+        S.keys = static_cast<const uint32_t*>(keys);
+    }
     S.head = B.head;
     S.tail = B.tail;
     S.n = tokens;
     S.rows = static_cast<uint32_t>(a.rows);
-    S.chunk = chunk_of(tokens, static_cast<uint64_t>(a.width));
-    S.chunks = (tokens + S.chunk - 1) / S.chunk;
     S.scale = a.scale;
     const int n = access_elements(a, size, g, grad);
 #define FGS_SUMS(P, N) launch_sums<P, N>(a, g, grad, S, s)

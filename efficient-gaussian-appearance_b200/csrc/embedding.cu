@@ -59,52 +59,113 @@ __device__ inline uint32_t row_of(I index, int64_t rows, int64_t padding) {
     return i < rows ? static_cast<uint32_t>(i) : kBadRow;
 }
 
-// a CTA takes `per` tokens (rows of `units` accesses), or with per = 1 the part blockIdx.y of one row
-template <typename P, int N, typename I>
+template <bool STREAM, typename A>
+__device__ inline void store(A* to, A x) {
+    if (STREAM) __stcs(to, x);
+    else *to = x;
+}
+
+template <typename P, int N>
+__device__ inline void scale_pack(Pack<P, N>& x, uint32_t row, float scale) {
+    const float fill = row == kNoRow ? 0.0f : __int_as_float(0x7fc00000);
+#pragma unroll
+    for (int j = 0; j < N; j++) x.x[j] = from_float<P>(row < kBadRow ? scale * to_float(x.x[j]) : fill);
+}
+
+// Short rows: a group of `lanes` lanes takes kUnits rows, whose loads are in flight together, and walks their columns.
+template <typename P, int N, typename I, bool STREAM>
 __global__ void __launch_bounds__(kThreads) lookup_kernel(const P* __restrict__ table, const I* __restrict__ index, P* __restrict__ out, int64_t rows,
-                                                          int64_t tokens, uint32_t units, uint32_t per, float scale, int64_t padding) {
+                                                          int64_t tokens, uint32_t units, uint32_t lanes, float scale, int64_t padding) {
     using A = typename Pack<P, N>::A;
-    const A* src = reinterpret_cast<const A*>(table);
-    A* dst = reinterpret_cast<A*>(out);
-    const uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * per;
-    const uint32_t have = tokens - t0 < per ? static_cast<uint32_t>(tokens - t0) : per;
-    const uint32_t n = have * units;  // at most max(units, kThreads * kUnits)
-    const uint32_t first = blockIdx.y * (kThreads * kUnits) + threadIdx.x;
-    Pack<P, N> x[kUnits];
+    const uint32_t lane = threadIdx.x & (lanes - 1), groups = kThreads / lanes, group = threadIdx.x / lanes;
+    // the CTA's tokens are those of kUnits rounds over its groups, so that it writes one stretch of the output
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (groups * kUnits) + group;
     uint32_t row[kUnits];
 #pragma unroll
     for (int k = 0; k < kUnits; k++) {
+        const int64_t t = t0 + k * groups;
+        row[k] = t < tokens ? row_of(index[t], rows, padding) : kNoRow;
+    }
+    for (uint32_t c = lane; c < units; c += lanes) {
+        Pack<P, N> x[kUnits];
+#pragma unroll
+        for (int k = 0; k < kUnits; k++)
+            if (row[k] < kBadRow) x[k].raw = reinterpret_cast<const A*>(table)[static_cast<uint64_t>(row[k]) * units + c];
+#pragma unroll
+        for (int k = 0; k < kUnits; k++) {
+            const int64_t t = t0 + k * groups;
+            if (t >= tokens) continue;
+            scale_pack(x[k], row[k], scale);
+            store<STREAM>(reinterpret_cast<A*>(out) + t * units + c, x[k].raw);
+        }
+    }
+}
+
+// Long rows: a CTA takes a part (kThreads * kUnits accesses) of one row.
+template <typename P, int N, typename I, bool STREAM>
+__global__ void __launch_bounds__(kThreads) lookup_long_kernel(const P* __restrict__ table, const I* __restrict__ index, P* __restrict__ out, int64_t rows,
+                                                               uint32_t units, float scale, int64_t padding) {
+    using A = typename Pack<P, N>::A;
+    const uint32_t row = row_of(index[blockIdx.x], rows, padding);
+    const uint32_t first = blockIdx.y * (kThreads * kUnits) + threadIdx.x;
+    const A* src = reinterpret_cast<const A*>(table) + static_cast<uint64_t>(row) * units;
+    A* dst = reinterpret_cast<A*>(out) + static_cast<uint64_t>(blockIdx.x) * units;
+    Pack<P, N> x[kUnits];
+#pragma unroll
+    for (int k = 0; k < kUnits; k++) {
         const uint32_t u = first + k * kThreads;
-        row[k] = kNoRow;
-        if (u >= n) continue;
-        const uint32_t t = per == 1 ? 0u : u / units;
-        row[k] = row_of(index[t0 + t], rows, padding);
-        if (row[k] < kBadRow) x[k].raw = src[static_cast<uint64_t>(row[k]) * units + (u - t * units)];
+        if (u < units && row < kBadRow) x[k].raw = src[u];
     }
 #pragma unroll
     for (int k = 0; k < kUnits; k++) {
         const uint32_t u = first + k * kThreads;
-        if (u >= n) continue;
-        const float fill = row[k] == kNoRow ? 0.0f : __int_as_float(0x7fc00000);
-#pragma unroll
-        for (int j = 0; j < N; j++) x[k].x[j] = from_float<P>(row[k] < kBadRow ? scale * to_float(x[k].x[j]) : fill);
-        dst[t0 * units + u] = x[k].raw;
+        if (u >= units) continue;
+        scale_pack(x[k], row, scale);
+        store<STREAM>(dst + u, x[k].raw);
     }
+}
+
+// lanes of a group that walks rows of `units` accesses: the power of two up to 32 that leaves the fewest lanes idle
+uint32_t lanes_for(uint64_t units) {
+    uint32_t best = 1;
+    while (best < 32 && best < units) best *= 2;
+    for (uint32_t l = best / 2; l >= 4; l /= 2) {
+        const uint64_t steps = (units + l - 1) / l * l, least = (units + best - 1) / best * best;
+        if (steps < least) best = l;
+    }
+    return best;
+}
+
+// An output larger than half the L2 is written past it: 2M rows of 32 floats take 51 instead of 68 us, and a short one
+// stays there for its reader.
+constexpr uint64_t kStreamBytes = 64ull << 20;
+
+template <typename P, int N, typename I, bool STREAM>
+cudaError_t launch_lookup_as(const EmbeddingArgs& a, const void* table, const void* index, void* out, cudaStream_t s) {
+    const uint64_t units = static_cast<uint64_t>(a.width) / N;
+    if (units > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+    const P* t = static_cast<const P*>(table);
+    const I* i = static_cast<const I*>(index);
+    P* o = static_cast<P*>(out);
+    // long rows, or rows of more than a warp's accesses that are so few that groups of lanes would leave SMs idle
+    if (units >= kThreads * kUnits || (units > 32 && a.tokens < 148 * 8)) {
+        const uint64_t parts = (units + kThreads * kUnits - 1) / (kThreads * kUnits);
+        if (parts > 65535) return cudaErrorInvalidValue;
+        lookup_long_kernel<P, N, I, STREAM><<<dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>(parts)), kThreads, 0, s>>>(
+            t, i, o, a.rows, static_cast<uint32_t>(units), a.scale, a.padding);
+    } else {
+        const uint32_t lanes = lanes_for(units);
+        const uint64_t per = static_cast<uint64_t>(kThreads / lanes) * kUnits;
+        lookup_kernel<P, N, I, STREAM><<<static_cast<unsigned>((static_cast<uint64_t>(a.tokens) + per - 1) / per), kThreads, 0, s>>>(
+            t, i, o, a.rows, a.tokens, static_cast<uint32_t>(units), lanes, a.scale, a.padding);
+    }
+    return cudaGetLastError();
 }
 
 template <typename P, int N, typename I>
 cudaError_t launch_lookup(const EmbeddingArgs& a, const void* table, const void* index, void* out, cudaStream_t s) {
-    const uint64_t units = static_cast<uint64_t>(a.width) / N;
-    if (units > 0x7FFFFFFFull) return cudaErrorInvalidValue;
-    const uint32_t span = kThreads * kUnits;
-    const uint32_t per = units >= span ? 1u : static_cast<uint32_t>(span / units);
-    const uint64_t ctas = (static_cast<uint64_t>(a.tokens) + per - 1) / per;
-    const uint64_t parts = per == 1 ? (units + span - 1) / span : 1;
-    if (ctas > 0x7FFFFFFFull || parts > 65535) return cudaErrorInvalidValue;
-    lookup_kernel<P, N, I><<<dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(parts)), kThreads, 0, s>>>(
-        static_cast<const P*>(table), static_cast<const I*>(index), static_cast<P*>(out), a.rows, a.tokens, static_cast<uint32_t>(units), per, a.scale,
-        a.padding);
-    return cudaGetLastError();
+    const uint64_t bytes = static_cast<uint64_t>(a.tokens) * static_cast<uint64_t>(a.width) * sizeof(P);
+    return bytes > kStreamBytes ? launch_lookup_as<P, N, I, true>(a, table, index, out, s) : launch_lookup_as<P, N, I, false>(a, table, index, out, s);
 }
 
 // widest access (at most 16 bytes) that divides a row and that all addresses are aligned for, in elements
@@ -149,7 +210,8 @@ size_t cluster_sort_smem(int items) {
 
 template <typename I, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads, 1) cluster_sort_kernel(const I* __restrict__ index, uint32_t tokens, int64_t rows, int64_t padding,
-                                                                       int end_bit, uint32_t* __restrict__ keys, uint32_t* __restrict__ vals) {
+                                                                       int end_bit, uint32_t* __restrict__ keys, uint32_t* __restrict__ vals,
+                                                                       uint4* __restrict__ clear, uint64_t clear_bytes) {
     namespace cg = cooperative_groups;
     extern __shared__ uint64_t pairs[];  // two buffers of kSortThreads * ITEMS pairs: key in the high word
     constexpr uint32_t kRun = kSortThreads * ITEMS;
@@ -159,6 +221,13 @@ __global__ void __launch_bounds__(kSortThreads, 1) cluster_sort_kernel(const I* 
     uint32_t* totals = base + kDigits;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank(), ctas = cluster.num_blocks();
+    if (blockIdx.x >= ctas) {  // the other clusters clear the gradient while the first one sorts
+        const uint64_t n = clear_bytes / 16, stride = static_cast<uint64_t>(gridDim.x - ctas) * kSortThreads;
+        const uint64_t i0 = static_cast<uint64_t>(blockIdx.x - ctas) * kSortThreads + threadIdx.x;
+        for (uint64_t i = i0; i < n; i += stride) clear[i] = make_uint4(0, 0, 0, 0);
+        if (i0 < clear_bytes % 16) reinterpret_cast<uint8_t*>(clear + n)[i0] = 0;
+        return;
+    }
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const uint32_t first = rank * kRun + static_cast<uint32_t>(warp) * (32 * ITEMS) + lane;  // this thread's places: first + 32 j
     uint32_t key[ITEMS], val[ITEMS];
@@ -269,7 +338,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) cluster_sort_kernel(const I* 
 }
 
 template <typename I, int ITEMS>
-cudaError_t launch_cluster_sort(const EmbeddingArgs& a, const void* index, int end_bit, uint32_t* keys, uint32_t* vals, cudaStream_t s) {
+cudaError_t launch_cluster_sort(const EmbeddingArgs& a, const void* index, int end_bit, uint32_t* keys, uint32_t* vals, void* clear, uint64_t clear_bytes,
+                                cudaStream_t s) {
     const uint32_t per = kSortThreads * ITEMS;
     uint32_t ctas = 1;
     while (ctas * per < static_cast<uint32_t>(a.tokens)) ctas *= 2;
@@ -277,7 +347,10 @@ cudaError_t launch_cluster_sort(const EmbeddingArgs& a, const void* index, int e
     cudaError_t e = cudaFuncSetAttribute(cluster_sort_kernel<I, ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(ctas);
+    // 32 KB per clearing CTA, and no more of them than the SMs that the sort leaves
+    const uint64_t want = (clear_bytes + 32767) / 32768, room = 148 - ctas;
+    const uint32_t clearing = static_cast<uint32_t>((want < room ? want : room) / ctas * ctas);
+    config.gridDim = dim3(ctas + (clearing > 0 || clear_bytes == 0 ? clearing : ctas));
     config.blockDim = dim3(kSortThreads);
     config.dynamicSmemBytes = smem;
     config.stream = s;
@@ -288,17 +361,18 @@ cudaError_t launch_cluster_sort(const EmbeddingArgs& a, const void* index, int e
     config.attrs = &attribute;
     config.numAttrs = 1;
     return cudaLaunchKernelEx(&config, cluster_sort_kernel<I, ITEMS>, static_cast<const I*>(index), static_cast<uint32_t>(a.tokens), a.rows, a.padding,
-                              end_bit, keys, vals);
+                              end_bit, keys, vals, static_cast<uint4*>(clear), clear_bytes);
 }
 
 // as many CTAs as a cluster has before each takes more than 1024 indices
 template <typename I>
-cudaError_t cluster_sort(const EmbeddingArgs& a, const void* index, int end_bit, uint32_t* keys, uint32_t* vals, cudaStream_t s) {
+cudaError_t cluster_sort(const EmbeddingArgs& a, const void* index, int end_bit, uint32_t* keys, uint32_t* vals, void* clear, uint64_t clear_bytes,
+                         cudaStream_t s) {
     const uint32_t most = kSortThreads * kMaxCluster;
-    if (a.tokens <= most) return launch_cluster_sort<I, 1>(a, index, end_bit, keys, vals, s);
-    if (a.tokens <= 2 * most) return launch_cluster_sort<I, 2>(a, index, end_bit, keys, vals, s);
-    if (a.tokens <= 4 * most) return launch_cluster_sort<I, 4>(a, index, end_bit, keys, vals, s);
-    return launch_cluster_sort<I, 8>(a, index, end_bit, keys, vals, s);
+    if (a.tokens <= most) return launch_cluster_sort<I, 1>(a, index, end_bit, keys, vals, clear, clear_bytes, s);
+    if (a.tokens <= 2 * most) return launch_cluster_sort<I, 2>(a, index, end_bit, keys, vals, clear, clear_bytes, s);
+    if (a.tokens <= 4 * most) return launch_cluster_sort<I, 4>(a, index, end_bit, keys, vals, clear, clear_bytes, s);
+    return launch_cluster_sort<I, 8>(a, index, end_bit, keys, vals, clear, clear_bytes, s);
 }
 
 struct SumArgs {
@@ -310,6 +384,7 @@ struct SumArgs {
     uint32_t lanes, parts;   // lanes of a group (a power of two, at most 32), column parts of a row
     uint32_t chunk, span, spans;  // sorted positions of a group and of a CTA; CTAs per column part
     uint32_t zero_rows;      // rows that a clearing CTA looks at
+    bool cleared;            // rows without a token are zero already
     float scale;
 };
 
@@ -358,7 +433,7 @@ __device__ inline void clear_rows(P* grad, const SumArgs& a, uint32_t cta, uint8
 // Within a group a row's sum stays in registers; rows that cross chunk borders are put together in shared memory, by
 // doubling along the groups that lie whole within the row.
 template <typename P, int N>
-__global__ void __launch_bounds__(kThreads) sum_kernel(const P* __restrict__ g, P* __restrict__ grad, const SumArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) sum_kernel(const P* __restrict__ g, P* __restrict__ grad, const SumArgs a) {
     using A = typename Pack<P, N>::A;
     extern __shared__ uint32_t staged[];  // the span's keys with one more on either side, and its tokens
     __shared__ float part[kThreads * N];
@@ -386,16 +461,16 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const P* __restrict__ g, 
     const uint32_t c0 = group * a.chunk, c1 = c0 + a.chunk < have ? c0 + a.chunk : have;
     const bool live = c0 < have && col < a.units;
     const A* src = reinterpret_cast<const A*>(g) + col;
-    float acc[N], head[N];  // the running row; the row that the group began within
+    float acc[N];  // the running row
 #pragma unroll
-    for (int j = 0; j < N; j++) acc[j] = head[j] = 0.0f;
+    for (int j = 0; j < N; j++) acc[j] = part[j * kThreads + threadIdx.x] = 0.0f;  // part: the row that the group began within
     uint32_t row = a.rows;
     bool first = false, on = false;
     if (live) {
         row = keys[c0];
         first = row < a.rows && keys[static_cast<int>(c0) - 1] == row;
         bool began = first;  // the running row began before the group
-        constexpr int kAhead = 8;
+        constexpr int kAhead = sizeof(Pack<P, N>) >= 16 ? 4 : 8;  // accesses in flight per lane
         for (uint32_t p = c0; p < c1 && row < a.rows; p += kAhead) {
             Pack<P, N> x[kAhead];
             uint32_t key[kAhead];
@@ -410,7 +485,7 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const P* __restrict__ g, 
                 if (key[k] != row) {  // the row ends here
                     if (began) {
 #pragma unroll
-                        for (int j = 0; j < N; j++) head[j] = acc[j];
+                        for (int j = 0; j < N; j++) part[j * kThreads + threadIdx.x] = acc[j];
                     } else {
                         write_row<P, N>(grad, row, a.units, col, acc, a.scale);
                     }
@@ -428,7 +503,7 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const P* __restrict__ g, 
         if (row < a.rows) {
             if (began) {  // one row only
 #pragma unroll
-                for (int j = 0; j < N; j++) head[j] = acc[j];
+                for (int j = 0; j < N; j++) part[j * kThreads + threadIdx.x] = acc[j];
             } else if (!on) {
                 write_row<P, N>(grad, row, a.units, col, acc, a.scale);
             }
@@ -440,11 +515,8 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const P* __restrict__ g, 
         full[group] = 0;
     }
     const uint32_t groups = kThreads / a.lanes;
-#pragma unroll
-    for (int j = 0; j < N; j++) part[j * kThreads + threadIdx.x] = head[j];
-    bool through = false;
     __syncthreads();
-    through = full[group];
+    bool through = full[group];
     if (__syncthreads_or(through)) {  // heads behind one another: add them up along the groups
         for (uint32_t d = 1; d < groups; d *= 2) {
             float more[N];
@@ -497,13 +569,14 @@ __global__ void __launch_bounds__(kThreads) join_kernel(P* __restrict__ grad, co
     if (p1 >= a.n) return;
     const uint32_t row = a.keys[p1];
     if (row >= a.rows || a.keys[p1 - 1] != row || (p0 > 0 && a.keys[p0 - 1] == row)) return;
-    uint32_t lo = static_cast<uint32_t>(p1), hi = a.n;  // the row's last position
-    while (hi - lo > 1) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (a.keys[mid] == row) lo = mid;
-        else hi = mid;
+    uint32_t last = span;  // the last span with the row: those behind this one that begin with it
+    for (;;) {
+        const uint64_t p = (static_cast<uint64_t>(last) + 1 + threadIdx.x) * a.span;
+        const int more = __syncthreads_count(p < a.n && a.keys[p] == row);
+        last += static_cast<uint32_t>(more);
+        if (more < kThreads) break;
     }
-    const uint32_t last = lo / a.span, width = a.units * N;
+    const uint32_t width = a.units * N;
     const uint32_t slots = kThreads / a.lanes, slot = threadIdx.x / a.lanes;
     const uint32_t col = blockIdx.y * a.lanes + threadIdx.x % a.lanes;
     float acc[N];
@@ -558,8 +631,7 @@ int bits_of(uint64_t x) {
 // How the sorted tokens are cut: enough groups to give each of 148 x 2048 threads a column, 8 to 64 positions each, and
 // at most 4096 positions (their keys and tokens are staged in shared memory) per CTA.
 void cut(uint64_t tokens, uint64_t units, SumArgs* S) {
-    S->lanes = 1;
-    while (S->lanes < 32 && S->lanes < units) S->lanes *= 2;
+    S->lanes = lanes_for(units);
     S->parts = static_cast<uint32_t>((units + S->lanes - 1) / S->lanes);
     const uint32_t groups = kThreads / S->lanes;
     const uint64_t want = tokens * units / (148ull * 2048ull);
@@ -615,7 +687,7 @@ cudaError_t launch_sums(const EmbeddingArgs& a, const void* g, void* grad, SumAr
     uint64_t zero_rows = 8192 / units;  // about 128 KB of a CTA's rows
     zero_rows = zero_rows < 1 ? 1 : zero_rows > kThreads ? kThreads : zero_rows;
     S.zero_rows = static_cast<uint32_t>(zero_rows);
-    const uint64_t ctas = static_cast<uint64_t>(S.spans) * S.parts + (static_cast<uint64_t>(a.rows) + zero_rows - 1) / zero_rows;
+    const uint64_t ctas = static_cast<uint64_t>(S.spans) * S.parts + (S.cleared ? 0 : (static_cast<uint64_t>(a.rows) + zero_rows - 1) / zero_rows);
     if (ctas > 0x7FFFFFFFull || S.parts > 65535) return cudaErrorInvalidValue;
     const size_t smem = sizeof(uint32_t) * (2 * static_cast<size_t>(S.span) + 2);
     sum_kernel<P, N><<<static_cast<unsigned>(ctas), kThreads, smem, s>>>(static_cast<const P*>(g), static_cast<P*>(grad), S);
@@ -670,7 +742,13 @@ cudaError_t launch_embedding_grad(const EmbeddingArgs& a, const void* index, con
     SumArgs S{};
     cudaError_t e;
     if (tokens <= kClusterSortMax) {
-        e = a.wide_index ? cluster_sort<int64_t>(a, index, end_bit, B.keys_a, B.vals_a, s) : cluster_sort<int32_t>(a, index, end_bit, B.keys_a, B.vals_a, s);
+        // The sort keeps at most 8 SMs busy; the others clear the whole gradient meanwhile (rows that have tokens are
+        // written again, which costs less than looking for the others afterwards), unless its address is not aligned.
+        const uint64_t bytes = static_cast<uint64_t>(a.rows) * static_cast<uint64_t>(a.width) * static_cast<uint64_t>(size);
+        S.cleared = reinterpret_cast<uintptr_t>(grad) % 16 == 0;
+        const uint64_t clear = S.cleared ? bytes : 0;
+        e = a.wide_index ? cluster_sort<int64_t>(a, index, end_bit, B.keys_a, B.vals_a, grad, clear, s)
+                         : cluster_sort<int32_t>(a, index, end_bit, B.keys_a, B.vals_a, grad, clear, s);
         if (e != cudaSuccess) return e;
         S.keys = B.keys_a;
         S.tokens = B.vals_a;

@@ -60,6 +60,8 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError('betas must be two numbers in [0, 1)')
         if not float(options['eps']) >= 0.0 or not float(options['weight_decay']) >= 0.0:
             raise ValueError('eps and weight_decay must not be negative')
+        if 0.0 < float(options['eps']) < 1.2e-38:
+            raise ValueError('eps must be zero or a normal float32 (at least 1.2e-38)')
         if options['state_bits'] not in (8, 32):
             raise ValueError('state_bits must be 8 or 32')
         super().add_param_group(param_group)
@@ -76,7 +78,6 @@ class FusedAdamW(torch.optim.Optimizer):
             state['master'] = p.detach().float()
         return state
 
-    @torch.no_grad()
     def step(self, closure=None):
         """One update of every parameter that has a gradient. `closure` (optional) recomputes the loss, which is returned."""
         loss = None

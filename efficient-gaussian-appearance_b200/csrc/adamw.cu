@@ -100,6 +100,11 @@ __device__ inline void store8(float* a, const float (&x)[8]) {
                  "f"(x[5]), "f"(x[6]), "f"(x[7])
                  : "memory");
 }
+__device__ inline void store32(void* a, const uint32_t (&x)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]),
+                 "r"(x[6]), "r"(x[7])
+                 : "memory");
+}
 template <typename H>
 __device__ inline void load8(const H* a, float (&x)[8]) {
     unpack8<H>(*reinterpret_cast<const uint4*>(a), x);
@@ -160,29 +165,45 @@ __device__ inline void store_codes(uint8_t* a, int lane, uint32_t left, const ui
     }
 }
 
-// Square root within 2^-23 of the value, division within 2^-22: together 6 roundings of half a step on an update that
-// is itself a small part of the parameter; the exact ones took half of the 8-bit step's instructions.
+// Square root within 2^-23 of the value, reciprocal too: with the product 5 roundings of half a step on an update that is
+// itself a small part of the parameter; the exact ones took half of the 8-bit step's instructions. The reciprocal takes
+// subnormals for zero: sqrt(v) is never one, and eps is not (checked on the host).
 __device__ inline float root(float x) {
     float y;
     asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ inline float quotient(float x, float y) { return __fdividef(x, y); }
+__device__ inline float quotient(float x, float y) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+    return x * r;
+}
+
+// Values of two codes, as bf16 (which holds them exactly), from the halves of x: (q + base) << 4, zero for q = 0. Two
+// codes per instruction, and products in the place of shifts and selections, which run at half the rate: the 8-bit step
+// is bound by them. For blocks with base >= 0, where every nonzero code is a normal float.
+template <bool SIGNED>
+__device__ inline uint32_t decode2(uint32_t x, uint32_t base) {
+    const uint32_t q = SIGNED ? x & 0x007f007fu : x;
+    // 16 in the halves with q != 0
+    const uint32_t some = SIGNED ? ((q + 0x007f007fu) & 0x00800080u) >> 3 : ((q + 0x00ff00ffu) & 0x01000100u) >> 4;
+    const uint32_t bits = q * 16u + some * base;
+    return SIGNED ? bits + (x & 0x00800080u) * 256u : bits;
+}
+// the halves with the bytes 2 k and 2 k + 1 of a packed word
+__device__ inline uint32_t code_pair(uint32_t word, int k) { return __byte_perm(word, 0, k ? 0x4342 : 0x4140); }
 
 // values of one code each; the codes come as bytes of packed words (four each) or one per register (q[j] < 256)
 template <bool SIGNED, bool PACKED>
 __device__ inline void decode(const uint32_t* q, int exponent, float (&x)[8]) {
     constexpr int top = SIGNED ? 127 : 255;
     const int base = 8 * (exponent + 1) - top;
-    if (base >= 0 && exponent != 255) {  // the usual case: every nonzero code is a normal float
-        const uint32_t up = static_cast<uint32_t>(base) << 20;
+    if (base >= 0 && exponent != 255) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t high = PACKED ? __byte_perm(q[j / 4], 0, (j & 3) << 12 | 0x444) : q[j] << 24;  // the code in bits 24..31
-            uint32_t bits = (high >> 4) & (static_cast<uint32_t>(top) << 20);
-            if (bits != 0) bits += up;
-            if (SIGNED) bits |= high & 0x80000000u;
-            x[j] = __uint_as_float(bits);
+        for (int j = 0; j < 8; j += 2) {
+            const uint32_t two = decode2<SIGNED>(PACKED ? code_pair(q[j / 4], (j / 2) & 1) : q[j] | q[j + 1] << 16, static_cast<uint32_t>(base));
+            x[j] = __uint_as_float(two << 16);
+            x[j + 1] = __uint_as_float(two & 0xffff0000u);
         }
         return;
     }
@@ -220,9 +241,10 @@ __device__ inline uint32_t encode(const float (&x)[8], uint32_t u0, int lane, ui
     if (VEC && high < 254 && small >= least) {  // the usual case: nothing under the smallest code or near the largest float
 #pragma unroll
         for (int w = 0; w < 2; w++) {
-            uint32_t word = static_cast<uint32_t>(-base) * 0x01010101u;  // every k - base fits its byte: their sum has no carries
+            uint32_t k[4];  // the code in bits 24..31
 #pragma unroll
-            for (int j = 0; j < 4; j++) word += ((b[4 * w + j] + ((u + (4 * w + j) * kTurn) >> 12)) >> 20) << (8 * j);
+            for (int j = 0; j < 4; j++) k[j] = (b[4 * w + j] + ((u + (4 * w + j) * kTurn) >> 12)) * 16u - (static_cast<uint32_t>(base) << 24);
+            uint32_t word = __byte_perm(__byte_perm(k[0], k[1], 0x0073), __byte_perm(k[2], k[3], 0x0073), 0x5410);
             if (SIGNED) {
                 const uint32_t lo = __byte_perm(__float_as_uint(x[4 * w]), __float_as_uint(x[4 * w + 1]), 0x0073);
                 const uint32_t hi = __byte_perm(__float_as_uint(x[4 * w + 2]), __float_as_uint(x[4 * w + 3]), 0x0073);
@@ -475,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<P, EIGHT, MASTER>()) ada
             const Chunk<P> C = chunk_at<P, EIGHT, MASTER>(T, t, start);
             Loaded<P, EIGHT, MASTER> L;
             uint32_t none = 0;
-            if ((T.hyper[t] & 128) && left >= kWarps * kBlock) {
+            if ((T.hyper[t] & 128) && left >= at + kBlock) {
                 load_all<P, EIGHT, MASTER, true>(C, at, kBlock, lane, L);
                 update<P, EIGHT, MASTER, true>(H, start + at, clip, lane, L, 0, 0);
                 store_all<P, EIGHT, MASTER, true>(C, H, start + at, at, kBlock, lane, L.p, L.m, L.v, none, none);
@@ -608,29 +630,40 @@ struct NormTable {
 };
 static_assert(sizeof(NormTable) <= 32764, "kernel parameter limit");
 
+// 16 bytes, issued where it stands: the compiler would otherwise wait for each load before it issues the next one
+__device__ inline uint4 load16(const void* a) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(a));
+    return r;
+}
+
 template <typename P>
 __device__ inline float chunk_squares(const P* g, uint64_t left, bool vec) {
+    constexpr int kEach = 16 / sizeof(P), kLoads = kNormChunk / kEach / kThreads;
     float s = 0.0f;
-    if (vec && left >= kNormChunk) {
-        float x[4][8];
+    const uint32_t n = left < kNormChunk ? static_cast<uint32_t>(left) : kNormChunk;
+    const uint32_t units = vec ? n / kEach : 0;  // whole accesses
+    uint4 x[kLoads];
 #pragma unroll
-        for (int r = 0; r < 4; r++) load8(g + (r * kThreads + threadIdx.x) * 8, x[r]);
+    for (int r = 0; r < kLoads; r++) {
+        const uint32_t u = r * kThreads + threadIdx.x;
+        x[r] = make_uint4(0, 0, 0, 0);
+        if (u < units) x[r] = load16(g + u * kEach);
+    }
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+    for (int r = 0; r < kLoads; r++) {
+        const P* y = reinterpret_cast<const P*>(&x[r]);
 #pragma unroll
-            for (int j = 0; j < 8; j++) s = fmaf(x[r][j], x[r][j], s);
-    } else {
-        const uint32_t n = left < kNormChunk ? static_cast<uint32_t>(left) : kNormChunk;
-#pragma unroll 8
-        for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
-            const float x = to_float(g[j]);
-            s = fmaf(x, x, s);
-        }
+        for (int j = 0; j < kEach; j++) s = fmaf(to_float(y[j]), to_float(y[j]), s);
+    }
+    for (uint32_t j = units * kEach + threadIdx.x; j < n; j += kThreads) {
+        const float y = to_float(g[j]);
+        s = fmaf(y, y, s);
     }
     return s;
 }
 
-__global__ void __launch_bounds__(kThreads, kNormPartials / 148) grad_squares_kernel(const __grid_constant__ NormTable T) {
+__global__ void __launch_bounds__(kThreads, 5) grad_squares_kernel(const __grid_constant__ NormTable T) {
     __shared__ double scratch[kWarps];
     double total = 0.0;
     const uint32_t first = share_of(T.chunks, blockIdx.x, gridDim.x), end = share_of(T.chunks, blockIdx.x + 1, gridDim.x);
@@ -676,18 +709,26 @@ __device__ inline void read_blocks(const uint8_t* codes, const uint8_t* exps, O*
         uint32_t e[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            r[h] = *reinterpret_cast<const uint4*>(codes + start + h * 2 * kBlock + lane * 16);
+            r[h] = load16(codes + start + h * 2 * kBlock + lane * 16);
             e[h] = exps[start / kBlock + 2 * h + (lane >> 4)];
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
+            O* to = out + start + h * 2 * kBlock + lane * 16;
+            const uint32_t q[4] = {r[h].x, r[h].y, r[h].z, r[h].w};
+            const int base = 8 * (static_cast<int>(e[h]) + 1) - (SIGNED ? 127 : 255);
+            if (sizeof(O) == 2 && base >= 0 && e[h] != 255) {
+                uint32_t w[8];
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const uint32_t q[2] = {k ? r[h].z : r[h].x, k ? r[h].w : r[h].y};
-                float x[8];
-                decode<SIGNED, true>(q, static_cast<int>(e[h]), x);
-                store8(out + start + h * 2 * kBlock + lane * 16 + 8 * k, x);
+                for (int j = 0; j < 8; j++) w[j] = decode2<SIGNED>(code_pair(q[j / 2], j & 1), static_cast<uint32_t>(base));
+                store32(to, w);
+                continue;
             }
+            float x[2][8];
+            decode<SIGNED, true>(q, static_cast<int>(e[h]), x[0]);
+            decode<SIGNED, true>(q + 2, static_cast<int>(e[h]), x[1]);
+            store8(to, x[0]);
+            store8(to + 8, x[1]);
         }
         return;
     }
@@ -747,7 +788,9 @@ cudaError_t launch_grad_squares(const void* const* grads, const int64_t* n_eleme
         T.first[k] = T.chunks = static_cast<uint32_t>(chunks);
         T.n_tensors = k;
         T.partials = partials + *n_partials;
-        const int grid = chunks < kNormPartials ? static_cast<int>(chunks) : kNormPartials;
+        // one resident grid, or CTAs of two chunks that the hardware hands out as SMs become free
+        const uint64_t resident = 148 * 5;
+        const int grid = static_cast<int>(chunks < resident ? chunks : chunks < 2 * resident ? resident : chunks < 2 * kNormPartials ? chunks / 2 : kNormPartials);
         grad_squares_kernel<<<grid, kThreads, 0, s>>>(T);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return e;
@@ -772,7 +815,7 @@ cudaError_t launch_read_moments(const uint8_t* const* codes, const uint8_t* cons
             T.exps[k] = exps[i];
             T.out[k] = out[i];
             T.n[k] = static_cast<uint64_t>(n_elements[i]);
-            T.kind[k] = static_cast<uint8_t>((is_signed[i] ? 1 : 0) | (aligned(codes[i], 16) && aligned(out[i], dtype == kDtypeF32 ? 32 : 16) ? 128 : 0));
+            T.kind[k] = static_cast<uint8_t>((is_signed[i] ? 1 : 0) | (aligned(codes[i], 16) && aligned(out[i], 32) ? 128 : 0));
             T.first[k] = static_cast<uint32_t>(chunks);
             chunks += (T.n[k] + kReadBlocks * kBlock * kWarps - 1) / (kReadBlocks * kBlock * kWarps);
             if (chunks > 0xFFFFFFFFull - 65536) return cudaErrorInvalidValue;

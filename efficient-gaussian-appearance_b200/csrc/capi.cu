@@ -756,6 +756,7 @@ int fgs_adamw_step(const fgs_adamw_tensors* t, const fgs_adamw_hyper* hypers, in
             if (a.step < 1) return fail(FGS_ERR_INVALID_ARGUMENT, "step must be >= 1");
             if (!(a.beta1 >= 0.0 && a.beta1 < 1.0 && a.beta2 >= 0.0 && a.beta2 < 1.0)) return fail(FGS_ERR_INVALID_ARGUMENT, "betas must be in [0, 1)");
             if (!(a.eps >= 0.0)) return fail(FGS_ERR_INVALID_ARGUMENT, "eps must not be negative");
+            if (a.eps > 0.0 && a.eps < 1.2e-38) return fail(FGS_ERR_INVALID_ARGUMENT, "eps must be zero or a normal float (at least 1.2e-38)");
             fgs::AdamwHyper& h = H[static_cast<size_t>(i)];
             const double bc1 = 1.0 / (1.0 - std::pow(a.beta1, static_cast<double>(a.step)));
             for (int j = 0; j < 7; j++) {

@@ -116,7 +116,7 @@ cudaError_t launch_dp_shard_adam(const AdamSegment* segs, int n_segs, const floa
 enum { kDtypeF32 = 0, kDtypeBf16 = 1, kDtypeF16 = 2 };
 constexpr int kAdamwBlock = 256;     // elements of a tensor that share one exponent byte (8-bit moments)
 constexpr int kMaxAdamwHypers = 8;   // different (group, step) pairs of one launch
-constexpr int kNormPartials = 148 * 6;  // partial sums of one gradient-norm launch, one per CTA
+constexpr int kNormPartials = 148 * 64;  // partial sums of one gradient-norm launch at most, one per CTA
 struct AdamwHyper {
     float lr[7], decay[7];  // lr / (1 - b1^t) and 1 - lr wd per column
     int n_lr;

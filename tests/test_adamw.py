@@ -18,7 +18,7 @@ def _param(n=5, dtype=torch.float32, grad=True):
 
 @pytest.mark.parametrize('options,match', [
     ({'lr': -1.0}, 'learning rates'), ({'lr': [1e-3] * 8}, 'learning rates'), ({'lr': []}, 'learning rates'), ({'betas': (0.9, 1.0)}, 'betas'),
-    ({'betas': (0.9,)}, 'betas'), ({'eps': -1e-8}, 'eps'), ({'weight_decay': -0.1}, 'weight_decay'), ({'state_bits': 16}, 'state_bits'),
+    ({'betas': (0.9,)}, 'betas'), ({'eps': -1e-8}, 'eps'), ({'eps': 1e-39}, 'eps'), ({'weight_decay': -0.1}, 'weight_decay'), ({'state_bits': 16}, 'state_bits'),
     ({'max_grad_norm': 0.0}, 'max_grad_norm'), ({'max_grad_norm': float('nan')}, 'max_grad_norm'), ({'lr': float('nan')}, 'learning rates')])
 def test_options_refused(options, match):
     import FasterGSVDACudaBackend as F
@@ -108,7 +108,7 @@ def _abi_call(**change):
 @pytest.mark.parametrize('change,match', [
     ({'dtype': 3}, 'dtype'), ({'bits': 4}, 'state_bits'), ({'bits': 8}, 'exponents'), ({'n_hypers': 0}, 'NULL'),
     ({'hyper': {'step': 0}}, 'step'), ({'hyper': {'n_learning_rates': 8}}, 'learning rates'), ({'hyper': {'beta1': 1.0}}, 'betas'),
-    ({'hyper': {'beta2': float('nan')}}, 'betas'), ({'hyper': {'eps': -1.0}}, 'eps'), ({'partials': 64, 'max_norm': 1.0}, 'grad_norm'),
+    ({'hyper': {'beta2': float('nan')}}, 'betas'), ({'hyper': {'eps': -1.0}}, 'eps'), ({'hyper': {'eps': 1e-40}}, 'eps'), ({'partials': 64, 'max_norm': 1.0}, 'grad_norm'),
     ({'partials': 64, 'norm': 64}, 'max_norm'), ({'tensors': {'hyper': (ctypes.c_int32 * 1)(1)}}, 'index'),
     ({'tensors': {'grad': (ctypes.c_uint64 * 1)(0)}}, 'NULL'), ({'tensors': {'master': (ctypes.c_uint64 * 1)(64)}}, 'master')])
 def test_c_entry_refuses(change, match):

@@ -390,6 +390,28 @@ struct SumArgs {
 
 constexpr uint32_t kNone = 0xFFFFFFFFu;  // no key
 
+// loads of read-only data that are issued where they stand
+__device__ inline uint4 load_nc(const uint4* a) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(a));
+    return r;
+}
+__device__ inline uint2 load_nc(const uint2* a) {
+    uint2 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(a));
+    return r;
+}
+__device__ inline uint32_t load_nc(const uint32_t* a) {
+    uint32_t r;
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r) : "l"(a));
+    return r;
+}
+__device__ inline uint16_t load_nc(const uint16_t* a) {
+    uint16_t r;
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(r) : "l"(a));
+    return r;
+}
+
 template <typename P, int N>
 __device__ inline void write_row(P* grad, uint64_t row, uint32_t units, uint32_t col, const float (&acc)[N], float scale) {
     Pack<P, N> x;
@@ -475,9 +497,10 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(const P* __restrict__ 
             Pack<P, N> x[kAhead];
             uint32_t key[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; k++) {
-                key[k] = p + k < c1 ? keys[p + k] : a.rows;
-                if (key[k] < a.rows) x[k].raw = src[static_cast<uint64_t>(tokens[p + k]) * a.units];
+            for (int k = 0; k < kAhead; k++) {  // loaded in any case (every token has a gradient): none waits for another
+                const uint32_t q = p + k < c1 ? p + k : c1 - 1;
+                key[k] = keys[q];
+                x[k].raw = load_nc(src + static_cast<uint64_t>(tokens[q]) * a.units);
             }
 #pragma unroll
             for (int k = 0; k < kAhead; k++) {

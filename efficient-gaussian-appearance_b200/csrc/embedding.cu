@@ -205,29 +205,23 @@ constexpr int kRunStride = kDigits + 1;  // spreads the warps' counts of one dig
 constexpr uint32_t kClusterSortMax = kSortThreads * kMaxItems * kMaxCluster;
 
 size_t cluster_sort_smem(int items) {
-    return 2 * sizeof(uint64_t) * kSortThreads * static_cast<size_t>(items) + sizeof(uint32_t) * (kSortWarps * kRunStride + kMaxCluster * kDigits + 2 * kDigits);
+    return 2 * sizeof(uint64_t) * kSortThreads * static_cast<size_t>(items) + sizeof(uint32_t) * (kSortWarps * kRunStride + kMaxCluster * kDigits + 2 * kDigits + 16);
 }
 
 template <typename I, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads, 1) cluster_sort_kernel(const I* __restrict__ index, uint32_t tokens, int64_t rows, int64_t padding,
-                                                                       int end_bit, uint32_t* __restrict__ keys, uint32_t* __restrict__ vals,
-                                                                       uint4* __restrict__ clear, uint64_t clear_bytes) {
+                                                                       int end_bit, uint32_t* __restrict__ keys, uint32_t* __restrict__ vals) {
     namespace cg = cooperative_groups;
-    extern __shared__ uint64_t pairs[];  // two buffers of kSortThreads * ITEMS pairs: key in the high word
+    extern __shared__ uint64_t pairs[];  // two buffers of kSortThreads * ITEMS pairs, which receive in turn: key in the high word
     constexpr uint32_t kRun = kSortThreads * ITEMS;
     uint32_t* run = reinterpret_cast<uint32_t*>(pairs + 2 * kRun);  // [warp][digit]
     uint32_t* counts = run + kSortWarps * kRunStride;               // [CTA][digit]
     uint32_t* base = counts + kMaxCluster * kDigits;                // first place of this CTA's keys of each digit
-    uint32_t* totals = base + kDigits;
+    uint32_t* local = base + kDigits;                               // first place of each digit in the CTA's own order
+    uint32_t* totals = local + kDigits;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank(), ctas = cluster.num_blocks();
-    if (blockIdx.x >= ctas) {  // the other clusters clear the gradient while the first one sorts
-        const uint64_t n = clear_bytes / 16, stride = static_cast<uint64_t>(gridDim.x - ctas) * kSortThreads;
-        const uint64_t i0 = static_cast<uint64_t>(blockIdx.x - ctas) * kSortThreads + threadIdx.x;
-        for (uint64_t i = i0; i < n; i += stride) clear[i] = make_uint4(0, 0, 0, 0);
-        if (i0 < clear_bytes % 16) reinterpret_cast<uint8_t*>(clear + n)[i0] = 0;
-        return;
-    }
+    asm volatile("griddepcontrol.launch_dependents;");  // a clearing kernel may start beside this one
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const uint32_t first = rank * kRun + static_cast<uint32_t>(warp) * (32 * ITEMS) + lane;  // this thread's places: first + 32 j
     uint32_t key[ITEMS], val[ITEMS];
@@ -243,6 +237,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) cluster_sort_kernel(const I* 
     for (int pass = 0; pass < passes; pass++) {
         const int shift = pass * bits;
         uint64_t* to = pairs + (pass & 1) * kRun;
+        uint64_t* stage = pairs + (~pass & 1) * kRun;  // free until the next pass's pairs arrive, behind its first barrier
         for (int i = t; i < kSortWarps * kRunStride; i += kSortThreads) run[i] = 0;
         __syncthreads();
         uint32_t place[ITEMS];
@@ -252,11 +247,9 @@ __global__ void __launch_bounds__(kSortThreads, 1) cluster_sort_kernel(const I* 
             const uint32_t d = (key[j] >> shift) & mask;
             uint32_t same = 0xFFFFFFFFu;
 #pragma unroll
-            for (int b = 0; b < 8; b++) {
-                if (b >= bits) break;
-                const bool set = (d >> b) & 1u;
-                const uint32_t with = __ballot_sync(0xFFFFFFFFu, set);
-                same &= set ? with : ~with;
+            for (int b = 0; b < 8; b++) {  // bits above the pass's are zero in all
+                const uint32_t with = __ballot_sync(0xFFFFFFFFu, (d >> b) & 1u);
+                same &= with ^ (((d >> b) & 1u) - 1u);
             }
             const uint32_t before = __popc(same & ((1u << lane) - 1u));
             const uint32_t prior = mine[d];
@@ -297,27 +290,47 @@ __global__ void __launch_bounds__(kSortThreads, 1) cluster_sort_kernel(const I* 
                 before += r < rank ? c : 0u;
                 all += c;
             }
-            base[t] = before;
-            uint32_t incl = all;  // inclusive sum over the warp's digits
+            const uint32_t own = counts[rank * kDigits + t];
+            uint32_t incl = all, incl_own = own;  // inclusive sums over the warp's digits, of all CTAs and of this one
             for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-                if (lane >= o) incl += y;
+                const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, incl, o), z = __shfl_up_sync(0xFFFFFFFFu, incl_own, o);
+                if (lane >= o) {
+                    incl += y;
+                    incl_own += z;
+                }
             }
-            if (lane == 31) totals[warp] = incl;
-            base[t] += incl - all;
+            if (lane == 31) {
+                totals[warp] = incl;
+                totals[8 + warp] = incl_own;
+            }
+            base[t] = before + incl - all;
+            local[t] = incl_own - own;
         }
         __syncthreads();
         if (t < kDigits) {
-            uint32_t before = 0;
-            for (int w = 0; w < warp; w++) before += totals[w];
-            base[t] += before;
+            uint32_t before = 0, before_own = 0;
+            for (int w = 0; w < warp; w++) {
+                before += totals[w];
+                before_own += totals[8 + w];
+            }
+            local[t] += before_own;
+            base[t] += before - local[t];  // place of a digit's key less its place in the CTA's own order
+        }
+        __syncthreads();
+        // into digit order within the CTA, then to the owners: neighbours go to neighbouring places (pairs stored one by
+        // one straight to their places took 4.7k of a pass's 14k cycles)
+#pragma unroll
+        for (int j = 0; j < ITEMS; j++) {
+            const uint32_t d = (key[j] >> shift) & mask;
+            stage[local[d] + mine[d] + place[j]] = static_cast<uint64_t>(key[j]) << 32 | val[j];
         }
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < ITEMS; j++) {
-            const uint32_t d = (key[j] >> shift) & mask;
-            const uint32_t p = base[d] + mine[d] + place[j];
-            cluster.map_shared_rank(to, p / kRun)[p % kRun] = static_cast<uint64_t>(key[j]) << 32 | val[j];
+            const uint32_t i = j * kSortThreads + t;
+            const uint64_t x = stage[i];
+            const uint32_t p = base[(static_cast<uint32_t>(x >> 32) >> shift) & mask] + i;
+            cluster.map_shared_rank(to, p / kRun)[p % kRun] = x;
         }
         cluster.sync();
 #pragma unroll
@@ -338,8 +351,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) cluster_sort_kernel(const I* 
 }
 
 template <typename I, int ITEMS>
-cudaError_t launch_cluster_sort(const EmbeddingArgs& a, const void* index, int end_bit, uint32_t* keys, uint32_t* vals, void* clear, uint64_t clear_bytes,
-                                cudaStream_t s) {
+cudaError_t launch_cluster_sort(const EmbeddingArgs& a, const void* index, int end_bit, uint32_t* keys, uint32_t* vals, cudaStream_t s) {
     const uint32_t per = kSortThreads * ITEMS;
     uint32_t ctas = 1;
     while (ctas * per < static_cast<uint32_t>(a.tokens)) ctas *= 2;
@@ -347,10 +359,7 @@ cudaError_t launch_cluster_sort(const EmbeddingArgs& a, const void* index, int e
     cudaError_t e = cudaFuncSetAttribute(cluster_sort_kernel<I, ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t config{};
-    // 32 KB per clearing CTA, and no more of them than the SMs that the sort leaves
-    const uint64_t want = (clear_bytes + 32767) / 32768, room = 148 - ctas;
-    const uint32_t clearing = static_cast<uint32_t>((want < room ? want : room) / ctas * ctas);
-    config.gridDim = dim3(ctas + (clearing > 0 || clear_bytes == 0 ? clearing : ctas));
+    config.gridDim = dim3(ctas);
     config.blockDim = dim3(kSortThreads);
     config.dynamicSmemBytes = smem;
     config.stream = s;
@@ -361,18 +370,46 @@ cudaError_t launch_cluster_sort(const EmbeddingArgs& a, const void* index, int e
     config.attrs = &attribute;
     config.numAttrs = 1;
     return cudaLaunchKernelEx(&config, cluster_sort_kernel<I, ITEMS>, static_cast<const I*>(index), static_cast<uint32_t>(a.tokens), a.rows, a.padding,
-                              end_bit, keys, vals, static_cast<uint4*>(clear), clear_bytes);
+                              end_bit, keys, vals);
 }
 
 // as many CTAs as a cluster has before each takes more than 1024 indices
 template <typename I>
-cudaError_t cluster_sort(const EmbeddingArgs& a, const void* index, int end_bit, uint32_t* keys, uint32_t* vals, void* clear, uint64_t clear_bytes,
-                         cudaStream_t s) {
+cudaError_t cluster_sort(const EmbeddingArgs& a, const void* index, int end_bit, uint32_t* keys, uint32_t* vals, cudaStream_t s) {
     const uint32_t most = kSortThreads * kMaxCluster;
-    if (a.tokens <= most) return launch_cluster_sort<I, 1>(a, index, end_bit, keys, vals, clear, clear_bytes, s);
-    if (a.tokens <= 2 * most) return launch_cluster_sort<I, 2>(a, index, end_bit, keys, vals, clear, clear_bytes, s);
-    if (a.tokens <= 4 * most) return launch_cluster_sort<I, 4>(a, index, end_bit, keys, vals, clear, clear_bytes, s);
-    return launch_cluster_sort<I, 8>(a, index, end_bit, keys, vals, clear, clear_bytes, s);
+    if (a.tokens <= most) return launch_cluster_sort<I, 1>(a, index, end_bit, keys, vals, s);
+    if (a.tokens <= 2 * most) return launch_cluster_sort<I, 2>(a, index, end_bit, keys, vals, s);
+    if (a.tokens <= 4 * most) return launch_cluster_sort<I, 4>(a, index, end_bit, keys, vals, s);
+    return launch_cluster_sort<I, 8>(a, index, end_bit, keys, vals, s);
+}
+
+// Clears a gradient on the SMs that the sort before it leaves idle: launched as its programmatic dependent, so it starts
+// with the sort, and waits for the sort's end before its own.
+__global__ void __launch_bounds__(kThreads) clear_kernel(uint4* __restrict__ to, uint64_t bytes) {
+    const uint64_t n = bytes / 16, stride = static_cast<uint64_t>(gridDim.x) * kThreads;
+    const uint64_t i0 = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
+#pragma unroll 4
+    for (uint64_t i = i0; i < n; i += stride) to[i] = make_uint4(0, 0, 0, 0);
+    if (i0 < bytes % 16) reinterpret_cast<uint8_t*>(to + n)[i0] = 0;
+    asm volatile("griddepcontrol.launch_dependents;\n griddepcontrol.wait;" ::: "memory");
+}
+
+// Launches a kernel as the programmatic dependent of the one before it in the stream: it may start once every CTA of
+// that one has asked for it (griddepcontrol.launch_dependents) or ended, and waits for its results itself
+// (griddepcontrol.wait).
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, size_t smem, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = smem;
+    config.stream = s;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
 }
 
 struct SumArgs {
@@ -460,6 +497,7 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(const P* __restrict__ 
     extern __shared__ uint32_t staged[];  // the span's keys with one more on either side, and its tokens
     __shared__ float part[kThreads * N];
     __shared__ uint8_t full[kThreads];    // group: its head row goes on in the next group
+    asm volatile("griddepcontrol.launch_dependents;\n griddepcontrol.wait;" ::: "memory");
     const uint32_t sum_ctas = a.spans * a.parts;
     if (blockIdx.x >= sum_ctas) {
         clear_rows<P, N>(grad, a, blockIdx.x - sum_ctas, reinterpret_cast<uint8_t*>(part));
@@ -587,6 +625,7 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(const P* __restrict__ 
 template <typename P, int N>
 __global__ void __launch_bounds__(kThreads) join_kernel(P* __restrict__ grad, const SumArgs a) {
     __shared__ float part[kThreads * N];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t span = blockIdx.x;
     const uint64_t p0 = static_cast<uint64_t>(span) * a.span, p1 = p0 + a.span;
     if (p1 >= a.n) return;
@@ -634,6 +673,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(P* __restrict__ grad, co
     }
     if (slot == 0 && col < a.units) write_row<P, N>(grad, row, a.units, col, acc, a.scale);
 }
+
+constexpr uint64_t kClearBytes = 32ull << 20;
 
 struct GradBuffers {
     uint32_t *keys_a, *keys_b, *vals_a, *vals_b;
@@ -713,14 +754,9 @@ cudaError_t launch_sums(const EmbeddingArgs& a, const void* g, void* grad, SumAr
     const uint64_t ctas = static_cast<uint64_t>(S.spans) * S.parts + (S.cleared ? 0 : (static_cast<uint64_t>(a.rows) + zero_rows - 1) / zero_rows);
     if (ctas > 0x7FFFFFFFull || S.parts > 65535) return cudaErrorInvalidValue;
     const size_t smem = sizeof(uint32_t) * (2 * static_cast<size_t>(S.span) + 2);
-    sum_kernel<P, N><<<static_cast<unsigned>(ctas), kThreads, smem, s>>>(static_cast<const P*>(g), static_cast<P*>(grad), S);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    if (S.spans > 1) {
-        join_kernel<P, N><<<dim3(S.spans, S.parts), kThreads, 0, s>>>(static_cast<P*>(grad), S);
-        e = cudaGetLastError();
-    }
-    return e;
+    const cudaError_t e = launch_dependent(sum_kernel<P, N>, dim3(static_cast<unsigned>(ctas)), smem, s, static_cast<const P*>(g), static_cast<P*>(grad), S);
+    if (e != cudaSuccess || S.spans == 1) return e;
+    return launch_dependent(join_kernel<P, N>, dim3(S.spans, S.parts), 0, s, static_cast<P*>(grad), S);
 }
 
 }  // namespace
@@ -765,13 +801,12 @@ cudaError_t launch_embedding_grad(const EmbeddingArgs& a, const void* index, con
     SumArgs S{};
     cudaError_t e;
     if (tokens <= kClusterSortMax) {
-        // The sort keeps at most 8 SMs busy; the others clear the whole gradient meanwhile (rows that have tokens are
-        // written again, which costs less than looking for the others afterwards), unless its address is not aligned.
+        e = a.wide_index ? cluster_sort<int64_t>(a, index, end_bit, B.keys_a, B.vals_a, s) : cluster_sort<int32_t>(a, index, end_bit, B.keys_a, B.vals_a, s);
+        // The sort keeps at most 8 SMs busy: the others clear a large gradient meanwhile (rows that have tokens are written
+        // again, which costs less than looking for the others afterwards; a small one is not worth the launch).
         const uint64_t bytes = static_cast<uint64_t>(a.rows) * static_cast<uint64_t>(a.width) * static_cast<uint64_t>(size);
-        S.cleared = reinterpret_cast<uintptr_t>(grad) % 16 == 0;
-        const uint64_t clear = S.cleared ? bytes : 0;
-        e = a.wide_index ? cluster_sort<int64_t>(a, index, end_bit, B.keys_a, B.vals_a, grad, clear, s)
-                         : cluster_sort<int32_t>(a, index, end_bit, B.keys_a, B.vals_a, grad, clear, s);
+        S.cleared = bytes >= kClearBytes && reinterpret_cast<uintptr_t>(grad) % 16 == 0;
+        if (e == cudaSuccess && S.cleared) e = launch_dependent(clear_kernel, dim3(148 * 8), 0, s, static_cast<uint4*>(grad), bytes);
         if (e != cudaSuccess) return e;
         S.keys = B.keys_a;
         S.tokens = B.vals_a;

@@ -100,6 +100,17 @@ __device__ inline void store8(float* a, const float (&x)[8]) {
                  "f"(x[5]), "f"(x[6]), "f"(x[7])
                  : "memory");
 }
+// loads issued where they stand: the compiler would otherwise put some of them behind the use of others
+__device__ inline uint4 load16_rw(const void* a) {
+    uint4 r;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(a));
+    return r;
+}
+__device__ inline uint2 load8_rw(const void* a) {
+    uint2 r;
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(a));
+    return r;
+}
 __device__ inline void store32(void* a, const uint32_t (&x)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]),
                  "r"(x[6]), "r"(x[7])
@@ -146,7 +157,7 @@ __device__ inline void store_block(P* a, int lane, uint32_t left, const float (&
 template <bool VEC>
 __device__ inline void load_codes(const uint8_t* a, int lane, uint32_t left, uint32_t* q) {
     if (VEC) {
-        const uint2 r = *reinterpret_cast<const uint2*>(a + lane * 8);
+        const uint2 r = load8_rw(a + lane * 8);
         q[0] = r.x;
         q[1] = r.y;
     } else {
@@ -297,10 +308,10 @@ struct Loaded {
 template <typename P, bool EIGHT, bool MASTER, bool VEC>
 __device__ inline void load_all(const Chunk<P>& C, uint32_t at, uint32_t left, int lane, Loaded<P, EIGHT, MASTER>& L) {
     constexpr bool packed = VEC && sizeof(P) == 2;
-    if (packed) L.packed_g = *reinterpret_cast<const uint4*>(C.grad + at + lane * 8);
+    if (packed) L.packed_g = load16_rw(C.grad + at + lane * 8);
     else load_block<VEC>(C.grad + at, lane, left, L.g);
     if (MASTER) load_block<VEC>(C.master + at, lane, left, L.p);
-    else if (packed) L.packed_p = *reinterpret_cast<const uint4*>(C.param + at + lane * 8);
+    else if (packed) L.packed_p = load16_rw(C.param + at + lane * 8);
     else load_block<VEC>(C.param + at, lane, left, L.p);
     if (EIGHT) {
         load_codes<VEC>(static_cast<const uint8_t*>(C.m) + at, lane, left, L.qm);

@@ -698,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 5) grad_squares_kernel(const __grid_
 // ---------------------------------------------------------------------------------------------------
 // values of 8-bit moments
 
-constexpr int kReadTensors = 512;
+constexpr int kReadTensors = 768;
 struct ReadTable {
     uint32_t first[kReadTensors + 1];
     const uint8_t* codes[kReadTensors];

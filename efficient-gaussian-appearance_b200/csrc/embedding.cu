@@ -13,6 +13,7 @@
 // follow each other, so a row's sum stays in fp32 registers. Rows that cross chunks are put together in shared memory,
 // rows that cross spans leave one fp32 sum per span, which a second kernel adds up. Rows without a token are found by
 // binary search in the sorted list and cleared by further CTAs. Bound by HBM: g is read once, the gradient written once.
+#include <atomic>
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -356,8 +357,16 @@ cudaError_t launch_cluster_sort(const EmbeddingArgs& a, const void* index, int e
     uint32_t ctas = 1;
     while (ctas * per < static_cast<uint32_t>(a.tokens)) ctas *= 2;
     const size_t smem = cluster_sort_smem(ITEMS);
-    cudaError_t e = cudaFuncSetAttribute(cluster_sort_kernel<I, ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use so much shared memory
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(cluster_sort_kernel<I, ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(ctas);
     config.blockDim = dim3(kSortThreads);

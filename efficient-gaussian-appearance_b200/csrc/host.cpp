@@ -11,7 +11,9 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
@@ -97,7 +99,7 @@ void* address(const at::Tensor& t, const char* name, int code, int64_t count, in
 }
 
 const at::Tensor& tensor_of(PyObject* o, const char* name) {
-    if (!o || !THPVariable_Check(o)) refuse(std::string(name) + " must be a tensor");
+    if (!o || !(THPVariable_CheckExact(o) || THPVariable_Check(o))) refuse(std::string(name) + " must be a tensor");
     return THPVariable_Unpack(o);
 }
 
@@ -362,39 +364,55 @@ at::Tensor lookup(const at::Tensor& table, const at::Tensor& indices, double sca
     return out;
 }
 
-struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
-    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& table, const at::Tensor& indices, double scale, int64_t padding) {
-        ctx->save_for_backward({indices});
-        ctx->saved_data["shape"] = table.sizes().vec();
-        ctx->saved_data["type"] = static_cast<int64_t>(table.scalar_type());
-        ctx->saved_data["scale"] = scale;
-        ctx->saved_data["padding"] = padding;
-        return lookup(table, indices, scale, padding);
-    }
+// autograd node of a lookup: the table's gradient from its output's
+struct LookupBackward : torch::autograd::Node {
+    torch::autograd::SavedVariable indices;
+    std::vector<int64_t> shape;
+    at::ScalarType type;
+    double scale;
+    int64_t padding;
 
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-        const at::Tensor indices = ctx->get_saved_variables()[0];
-        const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
-        const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
-        const at::Tensor g = grads[0].detach().to(type).contiguous();
-        const c10::cuda::CUDAGuard guard(g.device());
-        at::Tensor grad = at::empty(shape, g.options());
-        int64_t width = 1;
-        for (size_t d = 1; d < shape.size(); d++) width *= shape[d];
-        size_t bytes = 0;
-        check(lib.workspace_bytes(indices.numel(), shape[0], width, &bytes));
-        const at::Tensor space = at::empty({static_cast<int64_t>(bytes)}, g.options().dtype(at::kByte));
-        check(lib.lookup_grad(indices.data_ptr(), indices.numel(), static_cast<int>(indices.element_size()), g.data_ptr(), type_code(g), shape[0], width,
-                              ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), grad.data_ptr(), space.data_ptr(), bytes,
-                              c10::cuda::getCurrentCUDAStream().stream()));
+    std::string name() const override { return "EmbeddingLookupBackward"; }
+    void release_variables() override { indices.reset_data(); }
+
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+        if (!grads[0].defined()) return {at::Tensor()};
+        const at::Tensor idx = indices.unpack();
+        at::Tensor grad;
+        {
+            const at::AutoGradMode no_graph(false);
+            const at::Tensor g = grads[0].to(type).contiguous();
+            const c10::cuda::CUDAGuard guard(g.device());
+            grad = at::empty(shape, g.options());
+            int64_t width = 1;
+            for (size_t d = 1; d < shape.size(); d++) width *= shape[d];
+            size_t bytes = 0;
+            check(lib.workspace_bytes(idx.numel(), shape[0], width, &bytes));
+            const at::Tensor space = at::empty({static_cast<int64_t>(bytes)}, g.options().dtype(at::kByte));
+            check(lib.lookup_grad(idx.data_ptr(), idx.numel(), static_cast<int>(idx.element_size()), g.data_ptr(), type_code(g), shape[0], width, scale,
+                                  padding, grad.data_ptr(), space.data_ptr(), bytes, c10::cuda::getCurrentCUDAStream().stream()));
+        }
         if (at::GradMode::is_enabled() && grads[0].requires_grad()) {  // asked for a graph of the gradient: an error if it is used
             grad.set_requires_grad(true);
             auto error = std::make_shared<torch::autograd::DelayedError>("embedding_lookup is differentiable once", 1);
-            grad = (*error)({grad})[0];
+            return (*error)({grad});
         }
-        return {grad, at::Tensor(), at::Tensor(), at::Tensor()};
+        return {grad};
     }
 };
+
+at::Tensor lookup_with_grad(const at::Tensor& table, const at::Tensor& indices, double scale, int64_t padding) {
+    std::shared_ptr<LookupBackward> node(new LookupBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(table));
+    node->indices = torch::autograd::SavedVariable(indices, false);
+    node->shape = table.sizes().vec();
+    node->type = table.scalar_type();
+    node->scale = scale;
+    node->padding = padding;
+    at::Tensor out = lookup(table, indices, scale, padding);
+    torch::autograd::set_history(out, node);
+    return out;
+}
 
 // embedding_lookup(table, indices, scale, padding index or None)
 PyObject* embedding_lookup(PyObject*, PyObject* args) {
@@ -419,7 +437,7 @@ PyObject* embedding_lookup(PyObject*, PyObject* args) {
             }
         }
         const at::Tensor indices = given.contiguous();
-        return THPVariable_Wrap(table.requires_grad() && at::GradMode::is_enabled() ? EmbeddingLookup::apply(table, indices, scale, padding)
+        return THPVariable_Wrap(table.requires_grad() && at::GradMode::is_enabled() ? lookup_with_grad(table, indices, scale, padding)
                                                                                    : lookup(table, indices, scale, padding));
     });
 }

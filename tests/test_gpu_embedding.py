@@ -226,6 +226,32 @@ def test_captured_and_replayed(cuda):
             _check_grad(grad, g, idx, 3.0)
 
 
+def test_saved_indices(cuda):
+    """The backward needs the indices of the forward: a changed or released copy is an error, not another gradient."""
+    import FasterGSVDACudaBackend as F
+    table = torch.randn(8, 4, device=cuda, requires_grad=True)
+    idx = torch.tensor([1, 2, 3], device=cuda)
+    out = F.embedding_lookup(table, idx)
+    idx += 1
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        out.sum().backward()
+    out = F.embedding_lookup(table, idx)
+    out.sum().backward()
+    with pytest.raises(RuntimeError, match='second time'):
+        out.sum().backward()
+    # gradients of several lookups of one table, one of them twice in the graph, add up
+    table.grad = None
+    a = F.embedding_lookup(table, idx, scale=2.0)
+    (a + a * F.embedding_lookup(table, idx[:1])).sum().backward()
+    ref = table.detach().double().cpu().requires_grad_(True)
+    b = 2.0 * ref[idx.cpu()]
+    (b + b * ref[idx[:1].cpu()]).sum().backward()
+    # sums and products of a few values: at most 16 roundings of the largest
+    assert (table.grad.double().cpu() - ref.grad).abs().max() <= 16 * E32 * ref.grad.abs().max()
+    no = F.embedding_lookup(table.detach(), idx)
+    assert not no.requires_grad and F.embedding_lookup(table, idx).grad_fn is not None
+
+
 def test_refusals(cuda):
     import FasterGSVDACudaBackend as F
     table, idx = torch.randn(8, 4, device=cuda), torch.zeros(3, dtype=torch.int64, device=cuda)

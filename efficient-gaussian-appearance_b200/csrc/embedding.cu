@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kUnits = 4;  // accesses per thread in the lookup
+constexpr uint32_t kLookupLanes = kThreads;
 
 __device__ inline float to_float(float x) { return x; }
 __device__ inline float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -60,6 +61,35 @@ __device__ inline uint32_t row_of(I index, int64_t rows, int64_t padding) {
     return i < rows ? static_cast<uint32_t>(i) : kBadRow;
 }
 
+// Loads of read-only data that are issued where they stand. KEEP: they may be read again soon, by another token of the
+// same row, and stay in L1; else they pass it by.
+template <bool KEEP>
+__device__ inline uint4 load_nc(const uint4* a) {
+    uint4 r;
+    if (KEEP) asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(a));
+    else asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(a));
+    return r;
+}
+template <bool KEEP>
+__device__ inline uint2 load_nc(const uint2* a) {
+    uint2 r;
+    if (KEEP) asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(a));
+    else asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(a));
+    return r;
+}
+template <bool KEEP>
+__device__ inline uint32_t load_nc(const uint32_t* a) {
+    uint32_t r;
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r) : "l"(a));
+    return r;
+}
+template <bool KEEP>
+__device__ inline uint16_t load_nc(const uint16_t* a) {
+    uint16_t r;
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(r) : "l"(a));
+    return r;
+}
+
 template <bool STREAM, typename A>
 __device__ inline void store(A* to, A x) {
     if (STREAM) __stcs(to, x);
@@ -75,7 +105,7 @@ __device__ inline void scale_pack(Pack<P, N>& x, uint32_t row, float scale) {
 
 // Short rows: a group of `lanes` lanes takes kUnits rows, whose loads are in flight together, and walks their columns.
 template <typename P, int N, typename I, bool STREAM>
-__global__ void __launch_bounds__(kThreads) lookup_kernel(const P* __restrict__ table, const I* __restrict__ index, P* __restrict__ out, int64_t rows,
+__global__ void __launch_bounds__(kThreads, 6) lookup_kernel(const P* __restrict__ table, const I* __restrict__ index, P* __restrict__ out, int64_t rows,
                                                           int64_t tokens, uint32_t units, uint32_t lanes, float scale, int64_t padding) {
     using A = typename Pack<P, N>::A;
     const uint32_t lane = threadIdx.x & (lanes - 1), groups = kThreads / lanes, group = threadIdx.x / lanes;
@@ -90,8 +120,8 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const P* __restrict__ 
     for (uint32_t c = lane; c < units; c += lanes) {
         Pack<P, N> x[kUnits];
 #pragma unroll
-        for (int k = 0; k < kUnits; k++)
-            if (row[k] < kBadRow) x[k].raw = reinterpret_cast<const A*>(table)[static_cast<uint64_t>(row[k]) * units + c];
+        for (int k = 0; k < kUnits; k++)  // the first row stands in for none: no load waits for a decision
+            if (rows > 0) x[k].raw = load_nc<true>(reinterpret_cast<const A*>(table) + static_cast<uint64_t>(row[k] < kBadRow ? row[k] : 0u) * units + c);
 #pragma unroll
         for (int k = 0; k < kUnits; k++) {
             const int64_t t = t0 + k * groups;
@@ -126,13 +156,15 @@ __global__ void __launch_bounds__(kThreads) lookup_long_kernel(const P* __restri
     }
 }
 
-// lanes of a group that walks rows of `units` accesses: the power of two up to 32 that leaves the fewest lanes idle
-uint32_t lanes_for(uint64_t units) {
+// Lanes of a group that walks rows of `units` accesses: the first power of two up to `most` that covers a row, or a smaller
+// one where that leaves an eighth fewer lanes idle (45 accesses: three steps of 16 lanes, not one of 64). Wide groups read
+// long stretches of a row at once: 32768 rows of 256 accesses by 32 lanes 47.7 us, by 256 lanes 41.2 us.
+uint32_t lanes_for(uint64_t units, uint32_t most) {
     uint32_t best = 1;
-    while (best < 32 && best < units) best *= 2;
+    while (best < most && best < units) best *= 2;
     for (uint32_t l = best / 2; l >= 4; l /= 2) {
-        const uint64_t steps = (units + l - 1) / l * l, least = (units + best - 1) / best * best;
-        if (steps < least) best = l;
+        const uint64_t with = (units + l - 1) / l * l, now = (units + best - 1) / best * best;
+        if (8 * with <= 7 * now) best = l;
     }
     return best;
 }
@@ -155,7 +187,7 @@ cudaError_t launch_lookup_as(const EmbeddingArgs& a, const void* table, const vo
         lookup_long_kernel<P, N, I, STREAM><<<dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>(parts)), kThreads, 0, s>>>(
             t, i, o, a.rows, static_cast<uint32_t>(units), a.scale, a.padding);
     } else {
-        const uint32_t lanes = lanes_for(units);
+        const uint32_t lanes = lanes_for(units, kLookupLanes);
         const uint64_t per = static_cast<uint64_t>(kThreads / lanes) * kUnits;
         lookup_kernel<P, N, I, STREAM><<<static_cast<unsigned>((static_cast<uint64_t>(a.tokens) + per - 1) / per), kThreads, 0, s>>>(
             t, i, o, a.rows, a.tokens, static_cast<uint32_t>(units), lanes, a.scale, a.padding);
@@ -436,28 +468,6 @@ struct SumArgs {
 
 constexpr uint32_t kNone = 0xFFFFFFFFu;  // no key
 
-// loads of read-only data that are issued where they stand
-__device__ inline uint4 load_nc(const uint4* a) {
-    uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(a));
-    return r;
-}
-__device__ inline uint2 load_nc(const uint2* a) {
-    uint2 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(a));
-    return r;
-}
-__device__ inline uint32_t load_nc(const uint32_t* a) {
-    uint32_t r;
-    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r) : "l"(a));
-    return r;
-}
-__device__ inline uint16_t load_nc(const uint16_t* a) {
-    uint16_t r;
-    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(r) : "l"(a));
-    return r;
-}
-
 template <typename P, int N>
 __device__ inline void write_row(P* grad, uint64_t row, uint32_t units, uint32_t col, const float (&acc)[N], float scale) {
     Pack<P, N> x;
@@ -547,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(const P* __restrict__ 
             for (int k = 0; k < kAhead; k++) {  // loaded in any case (every token has a gradient): none waits for another
                 const uint32_t q = p + k < c1 ? p + k : c1 - 1;
                 key[k] = keys[q];
-                x[k].raw = load_nc(src + static_cast<uint64_t>(tokens[q]) * a.units);
+                x[k].raw = load_nc<false>(src + static_cast<uint64_t>(tokens[q]) * a.units);
             }
 #pragma unroll
             for (int k = 0; k < kAhead; k++) {
@@ -704,7 +714,7 @@ int bits_of(uint64_t x) {
 // How the sorted tokens are cut: enough groups to give each of 148 x 2048 threads a column, 8 to 64 positions each, and
 // at most 4096 positions (their keys and tokens are staged in shared memory) per CTA.
 void cut(uint64_t tokens, uint64_t units, SumArgs* S) {
-    S->lanes = lanes_for(units);
+    S->lanes = lanes_for(units, 32);
     S->parts = static_cast<uint32_t>((units + S->lanes - 1) / S->lanes);
     const uint32_t groups = kThreads / S->lanes;
     const uint64_t want = tokens * units / (148ull * 2048ull);

@@ -17,6 +17,7 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include "embedding.cuh"
 #include "launch.h"
 
 namespace fgs {
@@ -51,15 +52,6 @@ struct Pack {
     };
     __device__ Pack() {}
 };
-
-// row of an index: the row itself, kNoRow (padding) or kBadRow (past the table)
-constexpr uint32_t kNoRow = 0xFFFFFFFFu, kBadRow = 0xFFFFFFFEu;
-template <typename I>
-__device__ inline uint32_t row_of(I index, int64_t rows, int64_t padding) {
-    const int64_t i = static_cast<int64_t>(index);
-    if (i < 0 || i == padding) return kNoRow;
-    return i < rows ? static_cast<uint32_t>(i) : kBadRow;
-}
 
 // Loads of read-only data that are issued where they stand. KEEP: they may be read again soon, by another token of the
 // same row, and stay in L1; else they pass it by.
@@ -211,22 +203,6 @@ int access_elements(const EmbeddingArgs& a, int size, const void* p, const void*
 // ---------------------------------------------------------------------------------------------------
 // gradient
 
-// The indices as sort keys: the row, or `rows` for tokens that add to none.
-template <typename I>
-__device__ inline uint32_t key_of(I index, int64_t rows, int64_t padding) {
-    const uint32_t r = row_of(index, rows, padding);
-    return r < kBadRow ? r : static_cast<uint32_t>(rows);
-}
-
-template <typename I>
-__global__ void __launch_bounds__(kThreads) keys_kernel(const I* __restrict__ index, uint32_t tokens, int64_t rows, int64_t padding,
-                                                        uint32_t* __restrict__ keys, uint32_t* __restrict__ vals) {
-    const uint32_t t = blockIdx.x * kThreads + threadIdx.x;
-    if (t >= tokens) return;
-    keys[t] = key_of(index[t], rows, padding);
-    vals[t] = t;
-}
-
 // Stable radix sort of up to 65536 indices in one launch: a cluster of up to 8 CTAs holds all (key, token) pairs in its
 // shared memory, each CTA a run of 1024 x ITEMS positions. Per pass of at most 8 bits: every warp ranks its keys by
 // ballots (a warp owns consecutive positions, so the order of equal digits is kept), the CTAs tell one another their
@@ -262,7 +238,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) cluster_sort_kernel(const I* 
     for (int j = 0; j < ITEMS; j++) {
         const uint32_t p = first + 32 * j;
         val[j] = p;
-        key[j] = p < tokens ? key_of(index[p], rows, padding) : 0xFFFFFFFFu;  // sorts behind all others, which came before it
+        key[j] = p < tokens ? row_key(index[p], rows, padding) : 0xFFFFFFFFu;  // sorts behind all others, which came before it
     }
     const int passes = (end_bit + 7) / 8, bits = (end_bit + passes - 1) / passes;
     const uint32_t mask = (1u << bits) - 1u;
@@ -746,7 +722,7 @@ size_t carve(void* ws, uint64_t tokens, uint64_t rows, uint64_t width, int size,
     b.vals_a = reinterpret_cast<uint32_t*>(take(4 * tokens));
     b.keys_b = reinterpret_cast<uint32_t*>(take(small ? 0 : 4 * tokens));
     b.vals_b = reinterpret_cast<uint32_t*>(take(small ? 0 : 4 * tokens));
-    b.sort_bytes = small ? 0 : tile_sort_temp_bytes(tokens, 32, true);
+    b.sort_bytes = small ? 0 : row_sort_temp_bytes(tokens);
     b.sort_temp = take(b.sort_bytes);
     // narrower accesses (misaligned addresses) make more units and longer chunks, never more spans
     uint64_t spans = 1;
@@ -830,15 +806,9 @@ cudaError_t launch_embedding_grad(const EmbeddingArgs& a, const void* index, con
         S.keys = B.keys_a;
         S.tokens = B.vals_a;
     } else {
-        const unsigned ctas = (tokens + kThreads - 1) / kThreads;
-        if (a.wide_index) keys_kernel<<<ctas, kThreads, 0, s>>>(static_cast<const int64_t*>(index), tokens, a.rows, a.padding, B.keys_a, B.vals_a);
-        else keys_kernel<<<ctas, kThreads, 0, s>>>(static_cast<const int32_t*>(index), tokens, a.rows, a.padding, B.keys_a, B.vals_a);
-        e = cudaGetLastError();
+        e = row_sort(index, a.wide_index, a.rows, a.padding, tokens, end_bit, B.keys_a, B.keys_b, B.vals_a, B.vals_b, B.sort_temp, B.sort_bytes, &S.keys,
+                     &S.tokens, s);
         if (e != cudaSuccess) return e;
-        const void* keys = nullptr;
-        e = tile_sort(B.keys_a, B.keys_b, B.vals_a, B.vals_b, tokens, end_bit, true, B.sort_temp, B.sort_bytes, &keys, &S.tokens, s);
-        if (e != cudaSuccess) return e;
-        S.keys = static_cast<const uint32_t*>(keys);
     }
     S.head = B.head;
     S.tail = B.tail;

@@ -32,6 +32,11 @@ cudaError_t depth_sort(PrimBuffers& B, uint32_t n_visible, cudaStream_t s);  // 
 size_t tile_sort_temp_bytes(uint64_t n_instances, int end_bit, bool wide);
 cudaError_t tile_sort(void* keys_a, void* keys_b, uint32_t* vals_a, uint32_t* vals_b, uint64_t n, int end_bit, bool wide,
                       void* temp, size_t temp_bytes, const void** keys_out, const uint32_t** vals_out, cudaStream_t s);
+// rows of embedding indices with their positions (stable); the result lies in one of the two pairs of buffers
+size_t row_sort_temp_bytes(uint64_t n);
+cudaError_t row_sort(const void* index, bool wide, int64_t rows, int64_t padding, uint64_t n, int end_bit, uint32_t* keys_a, uint32_t* keys_b,
+                     uint32_t* vals_a, uint32_t* vals_b, void* temp, size_t temp_bytes, const uint32_t** keys_out, const uint32_t** vals_out,
+                     cudaStream_t s);
 cudaError_t exclusive_scan_u32(uint32_t* data, uint32_t n, void* temp, size_t temp_bytes, cudaStream_t s);
 size_t exclusive_scan_temp_bytes(uint32_t n);
 

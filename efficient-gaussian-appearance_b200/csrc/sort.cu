@@ -13,6 +13,7 @@
 //     run contiguously to its global offset (digit base from the scanned totals + the tile's row offset).
 // Positions are 32-bit: a sort takes fewer than 2^32 - 4096 keys.
 // Traffic per pass: keys read twice, keys and values read and written once.
+#include "embedding.cuh"
 #include "launch.h"
 
 namespace fgs {
@@ -25,7 +26,28 @@ constexpr int kSortItems = 16;                          // keys per thread
 constexpr int kSortTile = kSortThreads * kSortItems;    // 4096 keys per tile
 constexpr int kRadix = 256;
 
-uint32_t n_tiles_of(uint64_t n) { return static_cast<uint32_t>((n + kSortTile - 1) / kSortTile); }
+uint32_t n_tiles_of(uint64_t n, int items = kSortItems) {
+    const uint64_t tile = static_cast<uint64_t>(kSortThreads) * items;
+    return static_cast<uint32_t>((n + tile - 1) / tile);
+}
+
+// where a pass reads its keys and values: arrays, or (first pass of the sort of table rows) the indices themselves
+template <typename K>
+struct ArraySource {
+    using Key = K;
+    const K* keys;
+    const uint32_t* vals;
+    __device__ K key(uint32_t i) const { return keys[i]; }
+    __device__ uint32_t val(uint32_t i) const { return vals[i]; }
+};
+template <typename I>
+struct IndexSource {
+    using Key = uint32_t;
+    const I* index;
+    int64_t rows, padding;
+    __device__ uint32_t key(uint32_t i) const { return row_key(index[i], rows, padding); }
+    __device__ uint32_t val(uint32_t i) const { return i; }
+};
 
 // exclusive scan of one value per thread over a 256-thread block; returns the block total in *total
 __device__ inline uint32_t block_exclusive_scan(uint32_t x, uint32_t* warp_tot, uint32_t* total) {
@@ -55,22 +77,22 @@ __device__ inline uint32_t block_exclusive_scan(uint32_t x, uint32_t* warp_tot, 
     return r;
 }
 
-template <typename K>
-__global__ void __launch_bounds__(kSortThreads) radix_upsweep(const K* __restrict__ keys, uint32_t n, int shift, uint32_t mask,
-                                                              uint32_t* __restrict__ hist, uint32_t n_tiles) {
+template <typename S, int ITEMS>
+__global__ void __launch_bounds__(kSortThreads) radix_upsweep(const S src, uint32_t n, int shift, uint32_t mask, uint32_t* __restrict__ hist,
+                                                              uint32_t n_tiles) {
     __shared__ uint32_t cnt[kRadix];
     cnt[threadIdx.x] = 0;
-    const uint32_t base = blockIdx.x * kSortTile + threadIdx.x;
+    const uint32_t base = blockIdx.x * (kSortThreads * ITEMS) + threadIdx.x;
     // all loads first (the shared atomics below would otherwise keep each load waiting behind the previous one)
-    uint32_t d[kSortItems];
+    uint32_t d[ITEMS];
 #pragma unroll
-    for (int j = 0; j < kSortItems; j++) {
+    for (int j = 0; j < ITEMS; j++) {
         const uint32_t i = base + j * kSortThreads;
-        d[j] = i < n ? (static_cast<uint32_t>(keys[i]) >> shift) & mask : kRadix;
+        d[j] = i < n ? (static_cast<uint32_t>(src.key(i)) >> shift) & mask : kRadix;
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kSortItems; j++)
+    for (int j = 0; j < ITEMS; j++)
         if (d[j] < kRadix) atomicAdd(&cnt[d[j]], 1u);
     __syncthreads();
     hist[threadIdx.x * n_tiles + blockIdx.x] = cnt[threadIdx.x];
@@ -106,17 +128,19 @@ __device__ inline uint32_t digit_peers(uint32_t d, int bits, bool valid) {
     return m;
 }
 
-template <typename K>
-__global__ void __launch_bounds__(kSortThreads, 3) radix_downsweep(const K* __restrict__ kin, K* __restrict__ kout, const uint32_t* __restrict__ vin,
-                                                                uint32_t* __restrict__ vout, uint32_t n, int shift, int bits, uint32_t mask,
+template <typename S, int ITEMS>
+__global__ void __launch_bounds__(kSortThreads, 3) radix_downsweep(const S src, typename S::Key* __restrict__ kout, uint32_t* __restrict__ vout,
+                                                                uint32_t n, int shift, int bits, uint32_t mask,
                                                                 const uint32_t* __restrict__ hist, const uint32_t* __restrict__ totals,
                                                                 uint32_t n_tiles) {
+    using K = typename S::Key;
+    constexpr int kTile = kSortThreads * ITEMS;
     __shared__ uint32_t run[kSortWarps][kRadix];  // per-warp digit counts (then exclusive offsets within the tile)
     __shared__ uint32_t tile_off[kRadix];         // first tile-local position of each digit
     __shared__ uint32_t glob_off[kRadix];         // first global position of each digit for this tile
     __shared__ uint32_t warp_tot[kSortWarps];
-    __shared__ K skey[kSortTile];
-    __shared__ uint32_t sval[kSortTile];
+    __shared__ K skey[kTile];
+    __shared__ uint32_t sval[kTile];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
 #pragma unroll
     for (int w = 0; w < kSortWarps; w++) run[w][t] = 0;
@@ -126,26 +150,24 @@ __global__ void __launch_bounds__(kSortThreads, 3) radix_downsweep(const K* __re
         glob_off[t] = base + hist[t * n_tiles + blockIdx.x];
     }
     __syncthreads();
-    // warp chunk: keys [tile + warp * 512, + 512), 16 rounds of 32 consecutive keys
-    const uint32_t chunk = blockIdx.x * kSortTile + warp * (kSortItems * 32);
+    // warp chunk: ITEMS rounds of 32 consecutive keys (with 16: keys [tile + warp * 512, + 512))
+    const uint32_t chunk = blockIdx.x * kTile + warp * (ITEMS * 32);
     const uint32_t left = n > chunk ? n - chunk : 0u;  // keys of this warp's chunk that exist
-    const K* kc = kin + chunk;
-    const uint32_t* vc = vin + chunk;
-    K key[kSortItems];
-    uint32_t val[kSortItems], rank[kSortItems];
+    K key[ITEMS];
+    uint32_t val[ITEMS], rank[ITEMS];
     uint32_t valid_bits = 0;
     const uint32_t lt = (1u << lane) - 1u;
     // all loads first: the ranking rounds below are serialised through the shared counters and must not wait on
     // one global load each
 #pragma unroll
-    for (int j = 0; j < kSortItems; j++) {
+    for (int j = 0; j < ITEMS; j++) {
         const uint32_t i = j * 32 + lane;
         const bool valid = i < left;
-        key[j] = valid ? kc[i] : K(0);
+        key[j] = valid ? src.key(chunk + i) : K(0);
         valid_bits |= valid ? (1u << j) : 0u;
     }
 #pragma unroll
-    for (int j = 0; j < kSortItems; j++) {
+    for (int j = 0; j < ITEMS; j++) {
         const bool valid = (valid_bits >> j) & 1u;
         const uint32_t d = valid ? (static_cast<uint32_t>(key[j]) >> shift) & mask : kRadix;  // kRadix: no digit
         const uint32_t peers = digit_peers(d, bits, valid);
@@ -157,7 +179,7 @@ __global__ void __launch_bounds__(kSortThreads, 3) radix_downsweep(const K* __re
     }
     // values are only needed for the scatter: their loads overlap the offset scan
 #pragma unroll
-    for (int j = 0; j < kSortItems; j++) val[j] = (valid_bits >> j) & 1u ? vc[j * 32 + lane] : 0u;
+    for (int j = 0; j < ITEMS; j++) val[j] = (valid_bits >> j) & 1u ? src.val(chunk + j * 32 + lane) : 0u;
     __syncthreads();
     // tile-local offsets: digit-major, warps in order within a digit (the chunks are consecutive in the input)
     {
@@ -172,7 +194,7 @@ __global__ void __launch_bounds__(kSortThreads, 3) radix_downsweep(const K* __re
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kSortItems; j++) {
+    for (int j = 0; j < ITEMS; j++) {
         if (!((valid_bits >> j) & 1u)) continue;
         const uint32_t d = (static_cast<uint32_t>(key[j]) >> shift) & mask;
         const uint32_t p = tile_off[d] + run[warp][d] + rank[j];
@@ -181,8 +203,8 @@ __global__ void __launch_bounds__(kSortThreads, 3) radix_downsweep(const K* __re
     }
     __syncthreads();
     // write out in tile-local order: consecutive positions of a digit go to consecutive global positions
-    const uint32_t tile_base = blockIdx.x * kSortTile;
-    const uint32_t count = n - tile_base < static_cast<uint32_t>(kSortTile) ? n - tile_base : kSortTile;
+    const uint32_t tile_base = blockIdx.x * kTile;
+    const uint32_t count = n - tile_base < static_cast<uint32_t>(kTile) ? n - tile_base : kTile;
     for (uint32_t p = t; p < count; p += kSortThreads) {
         const K k = skey[p];
         const uint32_t d = (static_cast<uint32_t>(k) >> shift) & mask;
@@ -197,14 +219,24 @@ struct SortTemp {
     uint32_t* totals;  // [kRadix]
 };
 
-SortTemp carve_sort_temp(void* temp, uint64_t n) {
+SortTemp carve_sort_temp(void* temp, uint64_t n, int items = kSortItems) {
     SortTemp T;
     T.hist = static_cast<uint32_t*>(temp);
-    T.totals = T.hist + static_cast<uint64_t>(kRadix) * n_tiles_of(n);
+    T.totals = T.hist + static_cast<uint64_t>(kRadix) * n_tiles_of(n, items);
     return T;
 }
 
-size_t sort_temp_bytes(uint64_t n) { return (static_cast<uint64_t>(kRadix) * n_tiles_of(n) + kRadix) * sizeof(uint32_t); }
+size_t sort_temp_bytes(uint64_t n, int items = kSortItems) { return (static_cast<uint64_t>(kRadix) * n_tiles_of(n, items) + kRadix) * sizeof(uint32_t); }
+
+// one pass over the digit [shift, shift + bits)
+template <int ITEMS, typename S>
+cudaError_t radix_pass(const S& src, typename S::Key* kout, uint32_t* vout, uint64_t n, int shift, int bits, const SortTemp& T, cudaStream_t s) {
+    const uint32_t tiles = n_tiles_of(n, ITEMS), mask = (1u << bits) - 1u;
+    radix_upsweep<S, ITEMS><<<tiles, kSortThreads, 0, s>>>(src, static_cast<uint32_t>(n), shift, mask, T.hist, tiles);
+    radix_row_scan<<<kRadix, kSortThreads, 0, s>>>(T.hist, tiles, T.totals);
+    radix_downsweep<S, ITEMS><<<tiles, kSortThreads, 0, s>>>(src, kout, vout, static_cast<uint32_t>(n), shift, bits, mask, T.hist, T.totals, tiles);
+    return cudaGetLastError();
+}
 
 // sorts bits [0, end_bit) of the keys; the result ends in (ka, va) or (kb, vb), reported through *kout / *vout
 template <typename K>
@@ -216,20 +248,14 @@ cudaError_t radix_sort_pairs(K* ka, K* kb, uint32_t* va, uint32_t* vb, uint64_t 
     if (temp_bytes < sort_temp_bytes(n)) return cudaErrorInvalidValue;
     if (n > 0xFFFFFFFFull - kSortTile) return cudaErrorInvalidValue;  // positions are 32-bit
     const SortTemp T = carve_sort_temp(temp, n);
-    const uint32_t tiles = n_tiles_of(n);
     const int passes = (end_bit + 7) / 8;
     const int bits = (end_bit + passes - 1) / passes;
-    const uint32_t mask = (1u << bits) - 1u;
     K* kin = ka;
     K* kx = kb;
     uint32_t* vin = va;
     uint32_t* vx = vb;
     for (int p = 0; p < passes; p++) {
-        const int shift = p * bits;
-        radix_upsweep<K><<<tiles, kSortThreads, 0, s>>>(kin, static_cast<uint32_t>(n), shift, mask, T.hist, tiles);
-        radix_row_scan<<<kRadix, kSortThreads, 0, s>>>(T.hist, tiles, T.totals);
-        radix_downsweep<K><<<tiles, kSortThreads, 0, s>>>(kin, kx, vin, vx, static_cast<uint32_t>(n), shift, bits, mask, T.hist, T.totals, tiles);
-        cudaError_t e = cudaGetLastError();
+        const cudaError_t e = radix_pass<kSortItems>(ArraySource<K>{kin, vin}, kx, vx, n, p * bits, bits, T, s);
         if (e != cudaSuccess) return e;
         K* tk = kin; kin = kx; kx = tk;
         uint32_t* tv = vin; vin = vx; vx = tv;
@@ -237,6 +263,50 @@ cudaError_t radix_sort_pairs(K* ka, K* kb, uint32_t* va, uint32_t* vb, uint64_t 
     *kout = kin;
     *vout = vin;
     return cudaSuccess;
+}
+
+// sorts the rows of indices (and the positions 0 .. n - 1): the first pass reads the indices themselves
+template <int ITEMS, typename I>
+cudaError_t sort_rows_as(const I* index, int64_t rows, int64_t padding, uint64_t n, int end_bit, uint32_t* ka, uint32_t* kb, uint32_t* va, uint32_t* vb,
+                         void* temp, uint32_t** kout, uint32_t** vout, cudaStream_t s) {
+    const SortTemp T = carve_sort_temp(temp, n, ITEMS);
+    const int passes = (end_bit + 7) / 8;
+    const int bits = (end_bit + passes - 1) / passes;
+    cudaError_t e = radix_pass<ITEMS>(IndexSource<I>{index, rows, padding}, ka, va, n, 0, bits, T, s);
+    for (int p = 1; p < passes && e == cudaSuccess; p++) {
+        e = radix_pass<ITEMS>(ArraySource<uint32_t>{ka, va}, kb, vb, n, p * bits, bits, T, s);
+        uint32_t* k = ka; ka = kb; kb = k;
+        uint32_t* v = va; va = vb; vb = v;
+    }
+    *kout = ka;
+    *vout = va;
+    return e;
+}
+
+// Keys per thread: three CTAs run on an SM at once, so a pass takes as many rounds as it has groups of 444 tiles, each of a
+// time that grows with the tile (about as items + 4). 2M keys: a downsweep of 489 tiles of 16 x 256 keys takes two rounds,
+// 20.3 us, one of 782 tiles of 10 x 256 too, 17.7 us.
+int row_sort_items(uint64_t n) {
+    int best = 16;
+    uint64_t least = ~0ull;
+    for (const int items : {16, 10, 4}) {
+        const uint64_t cost = (n_tiles_of(n, items) + 443) / 444 * (items + 4);
+        if (cost < least) {
+            least = cost;
+            best = items;
+        }
+    }
+    return best;
+}
+
+template <typename I>
+cudaError_t sort_rows(const I* index, int64_t rows, int64_t padding, uint64_t n, int end_bit, uint32_t* ka, uint32_t* kb, uint32_t* va, uint32_t* vb,
+                      void* temp, uint32_t** kout, uint32_t** vout, cudaStream_t s) {
+    switch (row_sort_items(n)) {
+        case 4: return sort_rows_as<4>(index, rows, padding, n, end_bit, ka, kb, va, vb, temp, kout, vout, s);
+        case 10: return sort_rows_as<10>(index, rows, padding, n, end_bit, ka, kb, va, vb, temp, kout, vout, s);
+        default: return sort_rows_as<16>(index, rows, padding, n, end_bit, ka, kb, va, vb, temp, kout, vout, s);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -337,6 +407,20 @@ cudaError_t tile_sort(void* keys_a, void* keys_b, uint32_t* vals_a, uint32_t* va
         *keys_out = kout;
     }
     *vals_out = vout;
+    return e;
+}
+
+size_t row_sort_temp_bytes(uint64_t n) { return sort_temp_bytes(n, row_sort_items(n)); }
+
+cudaError_t row_sort(const void* index, bool wide, int64_t rows, int64_t padding, uint64_t n, int end_bit, uint32_t* keys_a, uint32_t* keys_b,
+                     uint32_t* vals_a, uint32_t* vals_b, void* temp, size_t temp_bytes, const uint32_t** keys_out, const uint32_t** vals_out,
+                     cudaStream_t s) {
+    if (n == 0 || end_bit <= 0 || temp_bytes < row_sort_temp_bytes(n) || n > 0xFFFFFFFFull - kSortTile) return cudaErrorInvalidValue;
+    uint32_t *k = nullptr, *v = nullptr;
+    const cudaError_t e = wide ? sort_rows(static_cast<const int64_t*>(index), rows, padding, n, end_bit, keys_a, keys_b, vals_a, vals_b, temp, &k, &v, s)
+                               : sort_rows(static_cast<const int32_t*>(index), rows, padding, n, end_bit, keys_a, keys_b, vals_a, vals_b, temp, &k, &v, s);
+    *keys_out = k;
+    *vals_out = v;
     return e;
 }
 

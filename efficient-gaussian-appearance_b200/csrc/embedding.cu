@@ -452,6 +452,30 @@ __device__ inline void write_row(P* grad, uint64_t row, uint32_t units, uint32_t
     reinterpret_cast<typename Pack<P, N>::A*>(grad)[row * units + col] = x.raw;
 }
 
+// N consecutive partial sums (aligned to their size, up to 16 bytes)
+template <int N>
+__device__ inline void load_part(const float* a, float (&x)[N]) {
+    if constexpr (N >= 4) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(x + j) = *reinterpret_cast<const float4*>(a + j);
+    } else if constexpr (N == 2) {
+        *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(a);
+    } else {
+        x[0] = a[0];
+    }
+}
+template <int N>
+__device__ inline void store_part(float* a, const float (&x)[N]) {
+    if constexpr (N >= 4) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(a + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+    } else if constexpr (N == 2) {
+        *reinterpret_cast<float2*>(a) = make_float2(x[0], x[1]);
+    } else {
+        a[0] = x[0];
+    }
+}
+
 // clears the rows without a token among `zero_rows` rows
 template <typename P, int N>
 __device__ inline void clear_rows(P* grad, const SumArgs& a, uint32_t cta, uint8_t* used) {
@@ -487,7 +511,7 @@ __device__ inline void clear_rows(P* grad, const SumArgs& a, uint32_t cta, uint8
 // Within a group a row's sum stays in registers; rows that cross chunk borders are put together in shared memory, by
 // doubling along the groups that lie whole within the row.
 template <typename P, int N>
-__global__ void __launch_bounds__(kThreads, 4) sum_kernel(const P* __restrict__ g, P* __restrict__ grad, const SumArgs a) {
+__global__ void __launch_bounds__(kThreads, N * sizeof(P) == 4 ? 6 : 4) sum_kernel(const P* __restrict__ g, P* __restrict__ grad, const SumArgs a) {
     using A = typename Pack<P, N>::A;
     extern __shared__ uint32_t staged[];  // the span's keys with one more on either side, and its tokens
     __shared__ float part[kThreads * N];
@@ -603,15 +627,15 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(const P* __restrict__ 
             leaves = full[group + 1];
         }
         if (leaves) {
-#pragma unroll
-            for (int j = 0; j < N; j++) a.tail[static_cast<uint64_t>(span) * width + col * N + j] = acc[j];
+            store_part<N>(a.tail + static_cast<uint64_t>(span) * width + col * N, acc);
         } else {
             write_row<P, N>(grad, row, a.units, col, acc, a.scale);
         }
     }
     if (group == 0 && first) {
 #pragma unroll
-        for (int j = 0; j < N; j++) a.head[static_cast<uint64_t>(span) * width + col * N + j] = part[j * kThreads + threadIdx.x];
+        for (int j = 0; j < N; j++) acc[j] = part[j * kThreads + threadIdx.x];
+        store_part<N>(a.head + static_cast<uint64_t>(span) * width + col * N, acc);
     }
 }
 
@@ -640,14 +664,21 @@ __global__ void __launch_bounds__(kThreads) join_kernel(P* __restrict__ grad, co
 #pragma unroll
     for (int j = 0; j < N; j++) acc[j] = 0.0f;
     if (col < a.units) {
-        if (slot == 0) {
+        if (slot == 0) load_part<N>(a.tail + static_cast<uint64_t>(span) * width + col * N, acc);
+        constexpr int kBatch = N >= 8 ? 4 : 8;  // spans in flight
+        for (uint32_t c0 = span + 1 + slot; c0 <= last; c0 += kBatch * slots) {
+            float x[kBatch][N];
 #pragma unroll
-            for (int j = 0; j < N; j++) acc[j] = a.tail[static_cast<uint64_t>(span) * width + col * N + j];
-        }
-#pragma unroll 4
-        for (uint32_t c = span + 1 + slot; c <= last; c += slots) {
+            for (int k = 0; k < kBatch; k++) {
+                const uint32_t c = c0 + k * slots;
+                load_part<N>(a.head + static_cast<uint64_t>(c <= last ? c : last) * width + col * N, x[k]);
+            }
 #pragma unroll
-            for (int j = 0; j < N; j++) acc[j] += a.head[static_cast<uint64_t>(c) * width + col * N + j];
+            for (int k = 0; k < kBatch; k++) {
+                if (c0 + k * slots > last) break;
+#pragma unroll
+                for (int j = 0; j < N; j++) acc[j] += x[k][j];
+            }
         }
     }
     uint32_t busy = slots;  // slots that may hold a sum

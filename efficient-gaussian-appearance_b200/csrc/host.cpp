@@ -51,6 +51,24 @@ struct Ref {
 
 struct PythonError {};  // the interpreter's error is set
 
+// Looks parameters up in the optimizer's state dict. It is in the parameters' order as a rule, so the entry behind the
+// last one is tried first, by identity: a lookup hashes the tensor, which calls into the interpreter.
+struct StateCursor {
+    PyObject* dict;
+    Py_ssize_t at = 0;
+    PyObject* find(PyObject* param) {
+        PyObject *key, *value;
+        Py_ssize_t next = at;
+        if (PyDict_Next(dict, &next, &key, &value) && key == param) {
+            at = next;
+            return value;
+        }
+        value = PyDict_GetItemWithError(dict, param);
+        if (!value && PyErr_Occurred()) throw PythonError();
+        return value;
+    }
+};
+
 PyObject* must(PyObject* o) {
     if (!o) throw PythonError();
     return o;
@@ -167,6 +185,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
         const double max_norm = limit == Py_None ? 0.0 : number(limit);
         if (limit != Py_None && !(max_norm > 0.0)) refuse("max_grad_norm must be positive (or None for no clipping)");
         Job jobs[3][2][2];
+        StateCursor states{all_state};
         std::vector<fgs_adamw_hyper> hypers;
         std::vector<Py_ssize_t> hyper_group;
         std::vector<std::pair<PyObject*, int64_t>> counted;  // states and their new step counts (borrowed)
@@ -197,8 +216,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                 const int64_t n = p.numel();
                 job.param.push_back(address(p, "a parameter", code, n, device));
                 job.grad.push_back(address(g, "a gradient", code, n, device));
-                PyObject* state = PyDict_GetItemWithError(all_state, o);
-                if (!state && PyErr_Occurred()) throw PythonError();
+                PyObject* state = states.find(o);
                 if (!state || (PyDict_Check(state) && PyDict_GET_SIZE(state) == 0)) {
                     Ref made(must(PyObject_CallFunction(new_state, "Oii", o, static_cast<int>(bits), static_cast<int>(master))));
                     if (PyList_Append(fresh.p, o) || PyList_Append(fresh.p, made.p)) throw PythonError();
@@ -282,9 +300,15 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                 }
         for (Py_ssize_t i = 0; i < PyList_GET_SIZE(fresh.p); i += 2)
             if (PyDict_SetItem(all_state, PyList_GET_ITEM(fresh.p, i), PyList_GET_ITEM(fresh.p, i + 1))) throw PythonError();
+        Ref count;  // most parameters have the same step count
+        int64_t counts = -1;
         for (const auto& c : counted) {
-            Ref t(must(PyLong_FromLongLong(c.second)));
-            if (PyDict_SetItem(c.first, names.step, t.p)) throw PythonError();
+            if (c.second != counts) {
+                Py_XDECREF(count.p);
+                count.p = nullptr;
+                count.p = must(PyLong_FromLongLong(counts = c.second));
+            }
+            if (PyDict_SetItem(c.first, names.step, count.p)) throw PythonError();
         }
         if (!norm.defined()) Py_RETURN_NONE;
         return THPVariable_Wrap(norm.select(0, 0));
@@ -304,12 +328,12 @@ PyObject* read_moments(PyObject*, PyObject* args) {
         std::vector<uint8_t> is_signed;
         std::vector<int64_t> counts;
         int device = -1, out_code = -1;
+        StateCursor states{all_state};
         std::vector<std::pair<at::Tensor, at::Tensor>> copies;  // moments in 32 bits; an undefined source: zeros
         for (Py_ssize_t i = 0; i < n; i++) {
             PyObject* o = PyList_GET_ITEM(params, i);
             const int64_t count = tensor_of(o, "a parameter").numel();
-            PyObject* state = PyDict_GetItemWithError(all_state, o);
-            if (!state && PyErr_Occurred()) throw PythonError();
+            PyObject* state = states.find(o);
             const bool none = !state || !PyDict_Check(state) || PyDict_GET_SIZE(state) == 0;
             for (int k = 0; k < 2; k++) {
                 const at::Tensor& out = tensor_of(PyList_GET_ITEM(outs[k], i), "an output");

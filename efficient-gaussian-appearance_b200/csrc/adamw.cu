@@ -20,6 +20,7 @@
 // decodes to NaN throughout.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include "dependent.cuh"
 #include "launch.h"
 
 namespace fgs {
@@ -67,6 +68,7 @@ struct Table {
     int n_partials;
     double max_norm;
     float* norm_out;
+    bool dependent;  // launched as the programmatic dependent of the kernel before it
 };
 constexpr uint32_t kMaxRun = 8;  // blocks of a warp's run (at most 32: one lane each)
 
@@ -466,6 +468,8 @@ __device__ inline float clip_factor(double norm, double max_norm) {
 __global__ void __launch_bounds__(kThreads) clip_kernel(const double* __restrict__ partials, int n_partials, double max_norm, float* __restrict__ factor,
                                                         float* __restrict__ norm_out) {
     __shared__ double scratch[kWarps];
+    allow_dependent();
+    wait_dependency();
     double x = 0.0;
     for (int i = threadIdx.x; i < n_partials; i += kThreads) x += partials[i];
     const double norm = sqrt(block_sum(x, scratch));
@@ -479,6 +483,7 @@ template <typename P, bool EIGHT, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<P, EIGHT, MASTER>()) adamw_kernel(const __grid_constant__ Table<CAP> T) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float clip = 1.0f;
+    if (T.partials) wait_dependency();
     if (T.factor) {
         clip = *T.factor;
     } else if (T.partials) {  // every CTA adds the partial sums in the same order: no further launch, no atomics
@@ -530,6 +535,8 @@ cudaError_t launch_table(const Table<CAP>& T, int sms, cudaStream_t s) {
     // Long steps: CTAs of four chunks each, which the hardware hands out as SMs become free. Equal shares of one resident
     // grid ended at 123k to 172k cycles on different SMs (20M elements, 8-bit moments).
     if (long_step(T.chunks, T.blocks, sms)) grid = EIGHT ? units : (units + 3) / 4;
+    // a clipped step overlaps the end of the norm's (or factor's) kernel, which its first instruction waits for
+    if (T.dependent) return launch_dependent(adamw_kernel<P, EIGHT, MASTER, CAP>, dim3(grid), kThreads, 0, s, T);
     adamw_kernel<P, EIGHT, MASTER, CAP><<<grid, kThreads, 0, s>>>(T);
     return cudaGetLastError();
 }
@@ -608,8 +615,12 @@ cudaError_t launch_all(const AdamwTensors& A, const AdamwHyper* hypers, int dtyp
         T.max_norm = clip.max_norm;
         T.norm_out = clip.norm_out;
         T.factor = nullptr;
+        T.dependent = clip.partials != nullptr;
         if (clip.partials && long_step(T.chunks, T.blocks, sms)) {
-            if (!factor_made) clip_kernel<<<1, kThreads, 0, s>>>(clip.partials, clip.n_partials, clip.max_norm, clip.factor, clip.norm_out);
+            if (!factor_made) {
+                const cudaError_t e = launch_dependent(clip_kernel, dim3(1), kThreads, 0, s, clip.partials, clip.n_partials, clip.max_norm, clip.factor, clip.norm_out);
+                if (e != cudaSuccess) return e;
+            }
             factor_made = true;
             T.factor = clip.factor;
         }
@@ -676,6 +687,7 @@ __device__ inline float chunk_squares(const P* g, uint64_t left, bool vec) {
 
 __global__ void __launch_bounds__(kThreads, 5) grad_squares_kernel(const __grid_constant__ NormTable T) {
     __shared__ double scratch[kWarps];
+    allow_dependent();
     double total = 0.0;
     const uint32_t first = share_of(T.chunks, blockIdx.x, gridDim.x), end = share_of(T.chunks, blockIdx.x + 1, gridDim.x);
     int t = owner(T, first);

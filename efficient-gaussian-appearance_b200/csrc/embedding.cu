@@ -17,6 +17,7 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include "dependent.cuh"
 #include "embedding.cuh"
 #include "launch.h"
 
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) cluster_sort_kernel(const I* 
     uint32_t* totals = local + kDigits;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank(), ctas = cluster.num_blocks();
-    asm volatile("griddepcontrol.launch_dependents;");  // a clearing kernel may start beside this one
+    allow_dependent();  // a clearing kernel may start beside this one
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const uint32_t first = rank * kRun + static_cast<uint32_t>(warp) * (32 * ITEMS) + lane;  // this thread's places: first + 32 j
     uint32_t key[ITEMS], val[ITEMS];
@@ -408,25 +409,8 @@ __global__ void __launch_bounds__(kThreads) clear_kernel(uint4* __restrict__ to,
 #pragma unroll 4
     for (uint64_t i = i0; i < n; i += stride) to[i] = make_uint4(0, 0, 0, 0);
     if (i0 < bytes % 16) reinterpret_cast<uint8_t*>(to + n)[i0] = 0;
-    asm volatile("griddepcontrol.launch_dependents;\n griddepcontrol.wait;" ::: "memory");
-}
-
-// Launches a kernel as the programmatic dependent of the one before it in the stream: it may start once every CTA of
-// that one has asked for it (griddepcontrol.launch_dependents) or ended, and waits for its results itself
-// (griddepcontrol.wait).
-template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, size_t smem, cudaStream_t s, Args... args) {
-    cudaLaunchConfig_t config{};
-    config.gridDim = grid;
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = smem;
-    config.stream = s;
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+    allow_dependent();
+    wait_dependency();
 }
 
 struct SumArgs {
@@ -516,7 +500,8 @@ __global__ void __launch_bounds__(kThreads, N * sizeof(P) == 4 ? 6 : 4) sum_kern
     extern __shared__ uint32_t staged[];  // the span's keys with one more on either side, and its tokens
     __shared__ float part[kThreads * N];
     __shared__ uint8_t full[kThreads];    // group: its head row goes on in the next group
-    asm volatile("griddepcontrol.launch_dependents;\n griddepcontrol.wait;" ::: "memory");
+    allow_dependent();
+    wait_dependency();
     const uint32_t sum_ctas = a.spans * a.parts;
     if (blockIdx.x >= sum_ctas) {
         clear_rows<P, N>(grad, a, blockIdx.x - sum_ctas, reinterpret_cast<uint8_t*>(part));
@@ -644,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, N * sizeof(P) == 4 ? 6 : 4) sum_kern
 template <typename P, int N>
 __global__ void __launch_bounds__(kThreads) join_kernel(P* __restrict__ grad, const SumArgs a) {
     __shared__ float part[kThreads * N];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    wait_dependency();
     const uint32_t span = blockIdx.x;
     const uint64_t p0 = static_cast<uint64_t>(span) * a.span, p1 = p0 + a.span;
     if (p1 >= a.n) return;
@@ -780,9 +765,9 @@ cudaError_t launch_sums(const EmbeddingArgs& a, const void* g, void* grad, SumAr
     const uint64_t ctas = static_cast<uint64_t>(S.spans) * S.parts + (S.cleared ? 0 : (static_cast<uint64_t>(a.rows) + zero_rows - 1) / zero_rows);
     if (ctas > 0x7FFFFFFFull || S.parts > 65535) return cudaErrorInvalidValue;
     const size_t smem = sizeof(uint32_t) * (2 * static_cast<size_t>(S.span) + 2);
-    const cudaError_t e = launch_dependent(sum_kernel<P, N>, dim3(static_cast<unsigned>(ctas)), smem, s, static_cast<const P*>(g), static_cast<P*>(grad), S);
+    const cudaError_t e = launch_dependent(sum_kernel<P, N>, dim3(static_cast<unsigned>(ctas)), kThreads, smem, s, static_cast<const P*>(g), static_cast<P*>(grad), S);
     if (e != cudaSuccess || S.spans == 1) return e;
-    return launch_dependent(join_kernel<P, N>, dim3(S.spans, S.parts), 0, s, static_cast<P*>(grad), S);
+    return launch_dependent(join_kernel<P, N>, dim3(S.spans, S.parts), kThreads, 0, s, static_cast<P*>(grad), S);
 }
 
 }  // namespace
@@ -832,7 +817,7 @@ cudaError_t launch_embedding_grad(const EmbeddingArgs& a, const void* index, con
         // again, which costs less than looking for the others afterwards; a small one is not worth the launch).
         const uint64_t bytes = static_cast<uint64_t>(a.rows) * static_cast<uint64_t>(a.width) * static_cast<uint64_t>(size);
         S.cleared = bytes >= kClearBytes && reinterpret_cast<uintptr_t>(grad) % 16 == 0;
-        if (e == cudaSuccess && S.cleared) e = launch_dependent(clear_kernel, dim3(148 * 8), 0, s, static_cast<uint4*>(grad), bytes);
+        if (e == cudaSuccess && S.cleared) e = launch_dependent(clear_kernel, dim3(148 * 8), kThreads, 0, s, static_cast<uint4*>(grad), bytes);
         if (e != cudaSuccess) return e;
         S.keys = B.keys_a;
         S.tokens = B.vals_a;

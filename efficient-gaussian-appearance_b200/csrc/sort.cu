@@ -13,6 +13,7 @@
 //     run contiguously to its global offset (digit base from the scanned totals + the tile's row offset).
 // Positions are 32-bit: a sort takes fewer than 2^32 - 4096 keys.
 // Traffic per pass: keys read twice, keys and values read and written once.
+#include "dependent.cuh"
 #include "embedding.cuh"
 #include "launch.h"
 
@@ -81,6 +82,8 @@ template <typename S, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) radix_upsweep(const S src, uint32_t n, int shift, uint32_t mask, uint32_t* __restrict__ hist,
                                                               uint32_t n_tiles) {
     __shared__ uint32_t cnt[kRadix];
+    allow_dependent();
+    wait_dependency();
     cnt[threadIdx.x] = 0;
     const uint32_t base = blockIdx.x * (kSortThreads * ITEMS) + threadIdx.x;
     // all loads first (the shared atomics below would otherwise keep each load waiting behind the previous one)
@@ -101,6 +104,8 @@ __global__ void __launch_bounds__(kSortThreads) radix_upsweep(const S src, uint3
 // row d of hist: exclusive offsets over the tiles; totals[d] = the row sum
 __global__ void __launch_bounds__(kSortThreads) radix_row_scan(uint32_t* __restrict__ hist, uint32_t n_tiles, uint32_t* __restrict__ totals) {
     __shared__ uint32_t warp_tot[kSortWarps];
+    allow_dependent();
+    wait_dependency();
     uint32_t* row = hist + static_cast<uint64_t>(blockIdx.x) * n_tiles;
     uint32_t carry = 0;
     for (uint32_t c0 = 0; c0 < n_tiles; c0 += kSortThreads) {
@@ -144,6 +149,8 @@ __global__ void __launch_bounds__(kSortThreads, 3) radix_downsweep(const S src, 
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
 #pragma unroll
     for (int w = 0; w < kSortWarps; w++) run[w][t] = 0;
+    allow_dependent();
+    wait_dependency();
     // global base of every digit: exclusive scan of the digit totals, plus this tile's row offset
     {
         const uint32_t base = block_exclusive_scan(totals[t], warp_tot, nullptr);
@@ -238,6 +245,24 @@ cudaError_t radix_pass(const S& src, typename S::Key* kout, uint32_t* vout, uint
     return cudaGetLastError();
 }
 
+// the same pass with its launches overlapped (`first`: its first kernel is launched in the ordinary way)
+template <int ITEMS, typename S>
+cudaError_t radix_pass_dependent(const S& src, typename S::Key* kout, uint32_t* vout, uint64_t n, int shift, int bits, const SortTemp& T, bool first,
+                                 cudaStream_t s) {
+    const uint32_t tiles = n_tiles_of(n, ITEMS), mask = (1u << bits) - 1u, count = static_cast<uint32_t>(n);
+    cudaError_t e = cudaSuccess;
+    if (first) {
+        radix_upsweep<S, ITEMS><<<tiles, kSortThreads, 0, s>>>(src, count, shift, mask, T.hist, tiles);
+        e = cudaGetLastError();
+    } else {
+        e = launch_dependent(radix_upsweep<S, ITEMS>, dim3(tiles), kSortThreads, 0, s, src, count, shift, mask, T.hist, tiles);
+    }
+    if (e == cudaSuccess) e = launch_dependent(radix_row_scan, dim3(kRadix), kSortThreads, 0, s, T.hist, tiles, T.totals);
+    if (e == cudaSuccess)
+        e = launch_dependent(radix_downsweep<S, ITEMS>, dim3(tiles), kSortThreads, 0, s, src, kout, vout, count, shift, bits, mask, T.hist, T.totals, tiles);
+    return e;
+}
+
 // sorts bits [0, end_bit) of the keys; the result ends in (ka, va) or (kb, vb), reported through *kout / *vout
 template <typename K>
 cudaError_t radix_sort_pairs(K* ka, K* kb, uint32_t* va, uint32_t* vb, uint64_t n, int end_bit, void* temp, size_t temp_bytes, K** kout,
@@ -272,9 +297,9 @@ cudaError_t sort_rows_as(const I* index, int64_t rows, int64_t padding, uint64_t
     const SortTemp T = carve_sort_temp(temp, n, ITEMS);
     const int passes = (end_bit + 7) / 8;
     const int bits = (end_bit + passes - 1) / passes;
-    cudaError_t e = radix_pass<ITEMS>(IndexSource<I>{index, rows, padding}, ka, va, n, 0, bits, T, s);
+    cudaError_t e = radix_pass_dependent<ITEMS>(IndexSource<I>{index, rows, padding}, ka, va, n, 0, bits, T, true, s);
     for (int p = 1; p < passes && e == cudaSuccess; p++) {
-        e = radix_pass<ITEMS>(ArraySource<uint32_t>{ka, va}, kb, vb, n, p * bits, bits, T, s);
+        e = radix_pass_dependent<ITEMS>(ArraySource<uint32_t>{ka, va}, kb, vb, n, p * bits, bits, T, false, s);
         uint32_t* k = ka; ka = kb; kb = k;
         uint32_t* v = va; va = vb; vb = v;
     }

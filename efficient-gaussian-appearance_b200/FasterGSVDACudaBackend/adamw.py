@@ -27,7 +27,8 @@ class FusedAdamW(torch.optim.Optimizer):
       master_weights=True: half-precision parameters keep a float32 copy in the state ('master'), which is updated; the
         parameter is its rounding. Float32 parameters need none.
     `max_grad_norm` (for all groups together): gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) as they are
-    read, p.grad stays as it is, and `grad_norm` then holds the norm (a 0-dim device tensor, a new one at each step). An
+    read, p.grad stays as it is, and `grad_norm` then holds the norm (a 0-dim device tensor, a new one at each step; None
+    after a step without clipping or gradients). An
     infinite or NaN gradient makes the norm infinite or NaN: the step is then not skipped, what it scales by 0 or NaN
     becomes so.
 
@@ -84,9 +85,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        norm = host.adamw_step(self.state, self.param_groups, self._new_state, self.max_grad_norm)
-        if norm is not None:
-            self.grad_norm = norm
+        self.grad_norm = host.adamw_step(self.state, self.param_groups, self._new_state, self.max_grad_norm)
         return loss
 
     @torch.no_grad()
@@ -105,9 +104,13 @@ class FusedAdamW(torch.optim.Optimizer):
         return exp_avgs, exp_avg_sqs
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As torch's, but the state keeps its own types (torch's casts it to the parameters' type)."""
+        """As torch's, but the state keeps its own types (torch's casts it to the parameters' type). Groups saved by another
+        AdamW take this one's options where they lack them (its moments are float32: state_bits=32)."""
         saved = state_dict['state']
         super().load_state_dict({**state_dict, 'state': {}})
+        for group in self.param_groups:
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
         self.state.clear()
         for group, mine in zip(state_dict['param_groups'], self.param_groups):
             for key, p in zip(group['params'], mine['params']):

@@ -13,6 +13,6 @@ def embedding_lookup(table: torch.Tensor, indices: torch.Tensor, scale: float = 
     not read: its output is NaN, and it adds to no gradient (nothing is copied to the host to raise an error).
 
     Differentiable in `table` (once). The gradient is dense, scale * the sum of the output gradients of each row's
-    indices: summed in float32 in an order that depends only on the inputs, so the same inputs give the same bits. Both
-    directions may be captured into CUDA graphs."""
+    indices: summed in float32 in an order that depends only on the inputs (and the alignment of the gradient's address),
+    so the same inputs give the same bits. Both directions may be captured into CUDA graphs."""
     return host.embedding_lookup(table, indices, scale, padding_index)

@@ -155,6 +155,21 @@ def test_state_keeps_its_types_over_save_and_load():
     assert again.max_grad_norm == 1.0 and next(iter(again.state.values()))['exp_avg'].dtype == torch.uint8
 
 
+def test_state_of_another_adamw_loads():
+    """A checkpoint of torch's AdamW: its step counts are tensors and its groups lack this optimizer's options."""
+    import FasterGSVDACudaBackend as F
+    p = _param(6)
+    ref = torch.optim.AdamW([p], lr=0.02, betas=(0.8, 0.95))
+    for _ in range(3):
+        ref.step()
+    opt = F.FusedAdamW([p], state_bits=32, master_weights=True)
+    opt.load_state_dict(ref.state_dict())
+    group, state = opt.param_groups[0], opt.state[p]
+    assert group['lr'] == 0.02 and tuple(group['betas']) == (0.8, 0.95) and group['state_bits'] == 32 and group['master_weights'] is True
+    assert state['step'] == 3 and isinstance(state['step'], int) and torch.equal(state['exp_avg'], ref.state[p]['exp_avg'])
+    assert state['exp_avg'].data_ptr() != ref.state[p]['exp_avg'].data_ptr()
+
+
 def test_code_values():
     """Every code's value survives coding in a block of its own exponent, whatever the threshold: it needs no rounding."""
     for signed in (True, False):

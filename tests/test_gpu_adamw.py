@@ -336,3 +336,100 @@ def test_moments_into_given_tensors(cuda):
         opt.read_moments([to[0][0][:5], to[0][1]], to[1])
     with pytest.raises(RuntimeError):
         opt.read_moments([x.half() for x in to[0]], [x.half() for x in to[1]])
+
+
+def test_closure_hooks_and_schedulers(cuda):
+    """What torch's optimizers offer around a step: a closure with gradients enabled, hooks, and learning-rate schedulers."""
+    import FasterGSVDACudaBackend as F
+    p = torch.nn.Parameter(torch.ones(300, device=cuda))
+    opt = F.FusedAdamW([p], lr=0.1, max_grad_norm=2.0)
+    schedule = torch.optim.lr_scheduler.StepLR(opt, step_size=1, gamma=0.5)
+    seen = []
+    opt.register_step_post_hook(lambda *a: seen.append('after'))
+
+    def closure():
+        opt.zero_grad()
+        loss = (p ** 2).sum()
+        loss.backward()
+        return loss
+
+    with torch.no_grad():
+        before = _snapshot(opt)
+        loss = opt.step(closure)
+    assert float(loss.detach()) == 300.0 and seen == ['after']
+    norm = 2.0 * np.sqrt(300.0)
+    assert abs(float(opt.grad_norm) - norm) <= 18 * 2.0 ** -24 * norm
+    _check(opt, before, 2.0 / (norm + 1e-6), True)
+    schedule.step()
+    assert opt.param_groups[0]['lr'] == 0.05
+    opt.max_grad_norm = None
+    before = _snapshot(opt)
+    opt.step()
+    assert opt.grad_norm is None
+    _check(opt, before)
+
+
+def test_two_optimizers_at_once(cuda):
+    """Steps of two optimizers on two streams do not share anything: the bits of each by itself."""
+    import FasterGSVDACudaBackend as F
+
+    def make(seed):
+        params = _params([(400_000,), (9,)], torch.float32, cuda, seed=seed)
+        _grads(params, 1, seed)
+        return params, F.FusedAdamW(params, state_bits=8, max_grad_norm=0.5)
+
+    alone = []
+    for seed in (0, 1):
+        params, opt = make(seed)
+        for _ in range(4):
+            opt.step()
+        alone.append(([p.detach().clone() for p in params], opt.grad_norm.clone()))
+    both = [make(0), make(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for (params, opt), s in zip(both, streams):
+            with torch.cuda.stream(s):
+                opt.step()
+    torch.cuda.synchronize()
+    for (params, opt), (ref, norm) in zip(both, alone):
+        assert all(torch.equal(p, q) for p, q in zip(params, ref)) and torch.equal(opt.grad_norm, norm)
+
+
+def test_more_than_2_31_elements(cuda):
+    """One tensor whose offsets pass 32 bits, looked at around its begin, 2^31 and its end."""
+    import FasterGSVDACudaBackend as F
+    n = 2 ** 31 + 1000
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device=cuda))
+    p.grad = torch.zeros(n, dtype=torch.bfloat16, device=cuda)
+    places = [slice(0, 512), slice(2 ** 31 - 512, 2 ** 31 + 256), slice(n - 1000, n)]
+    r = torch.Generator().manual_seed(0)
+    for k in places:
+        p.grad[k] = torch.randn(k.stop - k.start, generator=r).bfloat16().to(cuda)
+    opt = F.FusedAdamW([p], lr=0.5, state_bits=8, weight_decay=0.0)
+    opt.step()
+    s = opt.state[p]
+    for k in places:
+        g = _np(p.grad[k])
+        w, _, _ = O.step64(np.zeros_like(g), np.zeros_like(g), np.zeros_like(g), g, 1, 0.5, (0.9, 0.999), 1e-8, 0.0)
+        assert (np.abs(_np(p[k]) - w) <= (2.0 ** -8 + 2.0 ** -19) * np.abs(w) + 2.0 ** -134).all()
+        m32, v32 = O.moments32(np.zeros_like(g), np.zeros_like(g), g, (0.9, 0.999))
+        first = k.start  # a multiple of 256, but for the thresholds' element numbers, which are the tensor's
+        assert first % 256 == 0 or k.stop == n
+        first = first // 256 * 256
+        lead = k.start - first
+        for name, x, signed in (('exp_avg', m32, True), ('exp_avg_sq', v32, False)):
+            full = np.zeros(k.stop - first, np.float32)
+            full[lead:] = x
+            turn = first * O.TURN
+            shift = O.thresholds(full.size, 1, signed)
+            wrapped = (shift + turn) & 0xFFFFFFFF
+            keep = O.thresholds
+            O.thresholds = lambda *a: wrapped
+            try:
+                q, e = O.encode(full, 1, signed)
+            finally:
+                O.thresholds = keep
+            np.testing.assert_array_equal(s[name][first:k.stop].cpu().numpy(), q)
+            np.testing.assert_array_equal(s[name + '_exponent'][first // 256:first // 256 + e.size].cpu().numpy(), e)

@@ -176,6 +176,70 @@ def test_gradient_against_differences(cuda):
             assert abs(got - float(table.grad[i, j])) <= 4 * 2 * 3 * E32 * 64 * float(w.abs().max()) / step
 
 
+@pytest.mark.parametrize('dtype', DTYPES, ids=['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('tokens', [65_536, 65_537, 200_000])
+def test_around_and_beyond_one_cluster(cuda, tokens, dtype):
+    """The longest list that one cluster sorts, the next longer one, and one of several tiles; an odd width; rows in use
+    and out of use; absent tokens whose gradients are NaN."""
+    import FasterGSVDACudaBackend as F
+    for rows, width, kind in ((1000, 7, 'skewed'), (300_000, 4, 'even'), (2, 16, 'even')):
+        table, idx, g = _inputs(cuda, rows, width, tokens, dtype, kind, torch.int64)
+        g = (g.float() * 0.01).to(dtype)
+        g[(idx < 0) | (idx >= rows)] = float('nan')
+        table.requires_grad_(True)
+        out = F.embedding_lookup(table, idx, scale=0.25)
+        _check_rows(out, table, idx, 0.25)
+        out.backward(g)
+        _check_grad(table.grad, g, idx, 0.25)
+        none = torch.full_like(idx, -1)
+        none[tokens // 2] = rows - 1
+        grad, = torch.autograd.grad(F.embedding_lookup(table, none), table, torch.ones_like(g))
+        assert (grad[rows - 1] == 1).all() and not grad[:rows - 1].any()
+
+
+def test_extreme_indices_and_tables_of_one_dimension(cuda):
+    import FasterGSVDACudaBackend as F
+    table = torch.randn(9, device=cuda, requires_grad=True)
+    idx = torch.tensor([[2 ** 40, -2 ** 40, 8], [0, 2 ** 32 + 1, 9], [-1, 3, 3]], device=cuda)
+    out = F.embedding_lookup(table, idx, scale=2.0)
+    assert out.shape == (3, 3)
+    _check_rows(out.reshape(-1, 1), table.reshape(-1, 1), idx.reshape(-1), 2.0)
+    out.nan_to_num().sum().backward()
+    want = torch.zeros(9)
+    want[8], want[0], want[3] = 2.0, 2.0, 4.0
+    assert torch.equal(table.grad.cpu(), want)
+    with torch.inference_mode():
+        assert torch.equal(F.embedding_lookup(table, idx[2]), torch.stack([table.new_zeros(()), table[3], table[3]]))
+    big = torch.tensor([2 ** 31 - 1, -2 ** 31, 4], dtype=torch.int32, device=cuda)
+    out = F.embedding_lookup(table.detach(), big)
+    assert out[0].isnan() and out[1] == 0 and out[2] == table[4]
+
+
+def test_more_than_2_31_elements(cuda):
+    """A table, an output and a gradient whose offsets pass 32 bits."""
+    import FasterGSVDACudaBackend as F
+    rows, width = 2 ** 21 + 5, 1032
+    table = torch.zeros(rows, width, dtype=torch.bfloat16, device=cuda)
+    at = torch.tensor([0, 2 ** 21 - 3, 2 ** 21 + 4, 2 ** 21 + 4, 77], device=cuda)
+    r = torch.Generator().manual_seed(0)
+    table[at] = torch.randn(5, width, generator=r).bfloat16().to(cuda)
+    table.requires_grad_(True)
+    out = F.embedding_lookup(table, at, scale=3.0)
+    _check_rows(out, table.detach()[at], torch.arange(5), 3.0)
+    g = torch.randn(5, width, generator=r).bfloat16().to(cuda)
+    grad, = torch.autograd.grad(out, table, g)
+    want = torch.zeros(3, width, dtype=torch.float64)
+    want[0], want[1], want[2] = g[0].double().cpu(), g[1].double().cpu(), (g[2].double() + g[3].double()).cpu()
+    got = grad[at[:3]].double().cpu()
+    assert ((got - 3.0 * want).abs() <= 2.0 ** -7 * (3.0 * want).abs() + 2.0 ** -20).all()
+    assert int(torch.count_nonzero(grad).item()) == int(torch.count_nonzero(grad[at[[0, 1, 2, 4]]]).item())
+    del out, grad
+    short = table.detach()[:1000]
+    many = torch.arange(2 ** 21 + 5, device=cuda) % 1000
+    out = F.embedding_lookup(short, many)
+    assert torch.equal(out[-3:], short[many[-3:]]) and torch.equal(out[2 ** 21 - 2], short[many[2 ** 21 - 2]])
+
+
 def test_same_bits_on_any_stream(cuda):
     import FasterGSVDACudaBackend as F
     table, idx, g = _inputs(cuda, 90, 40, 20_000, torch.float32, 'skewed', torch.int64)
@@ -191,10 +255,11 @@ def test_same_bits_on_any_stream(cuda):
     assert all(torch.equal(first, x) for x in grads)
 
 
-def test_captured_and_replayed(cuda):
+@pytest.mark.parametrize('rows,tokens', [(200, 5000), (200, 70_000), (400_000, 5000)], ids=['short', 'radix passes', 'cleared beside the sort'])
+def test_captured_and_replayed(cuda, rows, tokens):
     """Both directions in one graph, replayed on other indices and gradients; a second graph lives beside it."""
     import FasterGSVDACudaBackend as F
-    table, idx, g = _inputs(cuda, 200, 48, 5000, torch.bfloat16, 'even', torch.int64)
+    table, idx, g = _inputs(cuda, rows, 48, tokens, torch.bfloat16, 'even', torch.int64)
     table.requires_grad_(True)
 
     def both():
@@ -213,7 +278,7 @@ def test_captured_and_replayed(cuda):
             outs = both()
         graphs.append((graph, outs))
     for seed, kind in ((1, 'one'), (2, 'skewed')):
-        t2, i2, g2 = _inputs(cuda, 200, 48, 5000, torch.bfloat16, kind, torch.int64, seed)
+        t2, i2, g2 = _inputs(cuda, rows, 48, tokens, torch.bfloat16, kind, torch.int64, seed)
         idx.copy_(i2)
         g.copy_(g2)
         with torch.no_grad():

@@ -31,12 +31,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBlock = kAdamwBlock;  // elements per warp and round; also the elements that share an exponent
 static_assert(kBlock == 32 * 8, "eight elements per lane");
-// resident CTAs per SM that the registers are bounded for: with 8-bit moments 3 (80 registers; 4 spill 100 bytes and take
-// 143 instead of 129 us for 40M bf16 elements)
-template <typename P, bool EIGHT, bool MASTER>
-constexpr int ctas_per_sm() {
-    return EIGHT ? 3 : 4;
-}
+constexpr int kCtasPerSm = 4;  // 64 registers per thread
 constexpr uint32_t kTurn = 0x9e3779b9u;  // 2^32 / golden ratio: the thresholds' step from element to element
 
 struct Hyper {
@@ -192,6 +187,39 @@ __device__ inline float quotient(float x, float y) {
     return x * r;
 }
 
+// value of one code of a block with any exponent
+template <bool SIGNED>
+__device__ inline float decode1(uint32_t code, int exponent) {
+    constexpr int top = SIGNED ? 127 : 255;
+    const int base = 8 * (exponent + 1) - top;
+    const int c = static_cast<int>(code & top);
+    const int k = c + base;
+    uint32_t bits = c > 0 && k > 0 ? static_cast<uint32_t>(k) << 20 : 0u;
+    if (exponent == 255) bits = 0x7fc00000u;
+    if (SIGNED) bits |= (code & 128u) << 24;
+    return __uint_as_float(bits);
+}
+
+// code of one element, `u` its threshold, in a block whose largest exponent is `high`
+template <bool SIGNED>
+__device__ inline uint32_t encode1(float x, uint32_t u, int high) {
+    constexpr int top = SIGNED ? 127 : 255;
+    const int base = 8 * (high + 1) - top;
+    const int floor = base > 0 ? base : 0;
+    const uint32_t least = static_cast<uint32_t>(floor + 1) << 20;
+    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+    int c = static_cast<int>((b + (u >> 12)) >> 20) - base;
+    if (b < least) {  // under the smallest code in use
+        const float share = __uint_as_float(least) * 5.9604644775390625e-8f;  // least / 2^24
+        const bool keep = SIGNED ? __uint_as_float(b) > static_cast<float>(u >> 8) * share : b > 0;
+        c = keep ? floor + 1 - base : 0;
+    }
+    const int cap = top < 0x7f7 - base ? top : 0x7f7 - base;  // no code past the largest finite float
+    c = c < cap ? c : cap;
+    const uint32_t code = static_cast<uint32_t>(c) & 255u;
+    return SIGNED ? (code & 127u) | (x < 0.0f ? 128u : 0u) : code;
+}
+
 // Values of two codes, as bf16 (which holds them exactly), from the halves of x: (q + base) << 4, zero for q = 0. Two
 // codes per instruction, and products in the place of shifts and selections, which run at half the rate: the 8-bit step
 // is bound by them. For blocks with base >= 0, where every nonzero code is a normal float.
@@ -221,21 +249,13 @@ __device__ inline void decode(const uint32_t* q, int exponent, float (&x)[8]) {
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const uint32_t code = PACKED ? (q[j / 4] >> (8 * (j & 3))) & 255u : q[j];
-        const int c = static_cast<int>(code & top);
-        const int k = c + base;
-        uint32_t bits = c > 0 && k > 0 ? static_cast<uint32_t>(k) << 20 : 0u;
-        if (exponent == 255) bits = 0x7fc00000u;
-        if (SIGNED) bits |= (code & 128u) << 24;
-        x[j] = __uint_as_float(bits);
-    }
+    for (int j = 0; j < 8; j++) x[j] = decode1<SIGNED>(PACKED ? (q[j / 4] >> (8 * (j & 3))) & 255u : q[j], exponent);
 }
 
-// codes of a block (all 32 lanes; elements that do not exist are zero), packed (VEC) or one per register; returns the
-// exponent byte. `u0`: the threshold of element 0 of the block.
-template <bool SIGNED, bool VEC>
-__device__ inline uint32_t encode(const float (&x)[8], uint32_t u0, int lane, uint32_t* q) {
+// packed codes of a whole block (all 32 lanes, eight consecutive elements each); returns the exponent byte. `u0`: the
+// threshold of element 0 of the block.
+template <bool SIGNED>
+__device__ inline uint32_t encode(const float (&x)[8], uint32_t u0, int lane, uint32_t (&q)[2]) {
     constexpr int top = SIGNED ? 127 : 255;
     uint32_t b[8];  // bits of the magnitudes (the second moment has no sign; that of a NaN is cut off below)
 #pragma unroll
@@ -250,8 +270,8 @@ __device__ inline uint32_t encode(const float (&x)[8], uint32_t u0, int lane, ui
     const int base = 8 * (static_cast<int>(high) + 1) - top;
     const int floor = base > 0 ? base : 0;
     const uint32_t least = static_cast<uint32_t>(floor + 1) << 20;
-    const uint32_t u = u0 + place<VEC>(lane, 0) * kTurn;
-    if (VEC && high < 254 && small >= least) {  // the usual case: nothing under the smallest code or near the largest float
+    const uint32_t u = u0 + place<true>(lane, 0) * kTurn;
+    if (high < 254 && small >= least) {  // the usual case: nothing under the smallest code or near the largest float
 #pragma unroll
         for (int w = 0; w < 2; w++) {
             uint32_t k[4];  // the code in bits 24..31
@@ -267,25 +287,9 @@ __device__ inline uint32_t encode(const float (&x)[8], uint32_t u0, int lane, ui
         }
         return high;
     }
-    const int low = floor + 1 - base;                         // the smallest code in use
-    const int cap = top < 0x7f7 - base ? top : 0x7f7 - base;  // no code past the largest finite float
-    const float share = __uint_as_float(least) * 5.9604644775390625e-8f;  // least / 2^24
-    if (VEC) q[0] = q[1] = 0;
+    q[0] = q[1] = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const uint32_t uj = u + (VEC ? j : 32 * j) * kTurn;
-        const uint32_t bj = b[j] & 0x7fffffffu;
-        int c = static_cast<int>((bj + (uj >> 12)) >> 20) - base;
-        if (bj < least) {
-            const bool keep = SIGNED ? __uint_as_float(bj) > static_cast<float>(uj >> 8) * share : bj > 0;
-            c = keep ? low : 0;
-        }
-        c = c < cap ? c : cap;
-        uint32_t code = static_cast<uint32_t>(c) & 255u;
-        if (SIGNED) code = (code & 127u) | (x[j] < 0.0f ? 128u : 0u);
-        if (VEC) q[j / 4] |= code << (8 * (j & 3));
-        else q[j] = code;
-    }
+    for (int j = 0; j < 8; j++) q[j / 4] |= encode1<SIGNED>(x[j], u + j * kTurn, static_cast<int>(high)) << (8 * (j & 3));
     return high;
 }
 
@@ -361,17 +365,13 @@ __device__ inline void store_all(const Chunk<P>& C, const Hyper& H, uint64_t sta
                                  float (&v)[8], uint32_t& em, uint32_t& ev) {
     if (MASTER) store_block<VEC>(C.master + at, lane, left, p);
     store_block<VEC>(C.param + at, lane, left, p);
-    if (EIGHT) {
-        if (!VEC) {  // places past the end take no part in the block's exponent (nor in anything else)
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (place<VEC>(lane, j) >= left) m[j] = v[j] = 0.0f;
-        }
-        uint32_t q[VEC ? 2 : 8];
+    if constexpr (EIGHT) {
+        static_assert(VEC, "cut blocks of 8-bit moments: cut_block");
+        uint32_t q[2];
         const uint32_t u = static_cast<uint32_t>(start) * kTurn;
-        em = encode<true, VEC>(m, u + H.dither_m, lane, q);
+        em = encode<true>(m, u + H.dither_m, lane, q);
         store_codes<VEC>(static_cast<uint8_t*>(C.m) + at, lane, left, q);
-        ev = encode<false, VEC>(v, u + H.dither_v, lane, q);
+        ev = encode<false>(v, u + H.dither_v, lane, q);
         store_codes<VEC>(static_cast<uint8_t*>(C.v) + at, lane, left, q);
     } else {
         store_block<VEC>(static_cast<float*>(C.m) + at, lane, left, m);
@@ -414,6 +414,45 @@ __device__ inline Chunk<P> chunk_at(const TAB& T, int t, uint64_t start) {
                     static_cast<char*>(T.v[t]) + start * (EIGHT ? 1 : 4), MASTER ? T.master[t] + start : nullptr};
 }
 
+// A block that is cut or not aligned, one element of a lane after the other: rolled up, with the new moments in local
+// memory, so that the whole blocks keep their registers (with both unrolled 80 registers and 117 us for 40M bf16 elements).
+template <typename P, bool MASTER>
+__device__ inline void cut_block(const Chunk<P>& C, const Hyper& H, uint64_t start, uint32_t at, uint32_t left, float clip, int lane, uint32_t& em,
+                                 uint32_t& ev) {
+    float m[8], v[8];
+    uint32_t high_m = 0, high_v = 0;
+#pragma unroll 1
+    for (int j = 0; j < 8; j++) {
+        const uint32_t i = place<false>(lane, j);
+        m[j] = v[j] = 0.0f;  // places past the end take no part in the block's exponent (nor in anything else)
+        if (i < left) {
+            const float gc = clip * to_float(C.grad[at + i]);
+            m[j] = H.beta1 * decode1<true>(static_cast<const uint8_t*>(C.m)[at + i], static_cast<int>(em)) + H.rest1 * gc;
+            v[j] = H.beta2 * decode1<false>(static_cast<const uint8_t*>(C.v)[at + i], static_cast<int>(ev)) + H.rest2 * gc * gc;
+            const uint32_t c = H.n_lr == 1 ? 0u : static_cast<uint32_t>((start + i) % static_cast<uint32_t>(H.n_lr));
+            float p;
+            if (MASTER) p = C.master[at + i];
+            else p = to_float(C.param[at + i]);
+            p = fmaf(-H.lr[c], quotient(m[j], fmaf(root(v[j]), H.root_rcp, H.eps)), p * H.decay[c]);
+            if (MASTER) C.master[at + i] = p;
+            from_float(p, C.param[at + i]);
+        }
+        const uint32_t bm = __float_as_uint(m[j]) & 0x7fffffffu, bv = __float_as_uint(v[j]) & 0x7fffffffu;
+        high_m = bm > high_m ? bm : high_m;
+        high_v = bv > high_v ? bv : high_v;
+    }
+    em = __reduce_max_sync(0xffffffffu, high_m) >> 23;
+    ev = __reduce_max_sync(0xffffffffu, high_v) >> 23;
+#pragma unroll 1
+    for (int j = 0; j < 8; j++) {
+        const uint32_t i = place<false>(lane, j);
+        if (i >= left) break;
+        const uint32_t u = (static_cast<uint32_t>(start) + i) * kTurn;
+        static_cast<uint8_t*>(C.m)[at + i] = static_cast<uint8_t>(encode1<true>(m[j], u + H.dither_m, static_cast<int>(em)));
+        static_cast<uint8_t*>(C.v)[at + i] = static_cast<uint8_t>(encode1<false>(v[j], u + H.dither_v, static_cast<int>(ev)));
+    }
+}
+
 // A warp's run of blocks with 8-bit moments: lane b keeps the exponents of block b, read and written with one access per
 // run. (One byte load and store per block, from different warps, made every read of a sector wait for the partial writes
 // to it: 59M elements took 385 us, against 185 us without them.)
@@ -437,16 +476,13 @@ __device__ inline void update_run(const Table<CAP>& T, uint32_t run, float clip,
     for (uint32_t b = 0; b < blocks; b++) {
         const uint32_t at = b * kBlock;
         uint32_t em_b = __shfl_sync(0xffffffffu, em, b), ev_b = __shfl_sync(0xffffffffu, ev, b);
-        Loaded<P, true, MASTER> L;
         if (vec && have - at >= kBlock) {
+            Loaded<P, true, MASTER> L;
             load_all<P, true, MASTER, true>(C, at, kBlock, lane, L);
             update<P, true, MASTER, true>(H, start + at, clip, lane, L, em_b, ev_b);
             store_all<P, true, MASTER, true>(C, H, start + at, at, kBlock, lane, L.p, L.m, L.v, em_b, ev_b);
         } else {
-            const uint32_t n = have - at < kBlock ? have - at : kBlock;
-            load_all<P, true, MASTER, false>(C, at, n, lane, L);
-            update<P, true, MASTER, false>(H, start + at, clip, lane, L, em_b, ev_b);
-            store_all<P, true, MASTER, false>(C, H, start + at, at, n, lane, L.p, L.m, L.v, em_b, ev_b);
+            cut_block<P, MASTER>(C, H, start + at, at, have - at < kBlock ? have - at : kBlock, clip, lane, em_b, ev_b);
         }
         if (lane == b) {
             em = em_b;
@@ -480,7 +516,7 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const double* __restrict
 }
 
 template <typename P, bool EIGHT, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm<P, EIGHT, MASTER>()) adamw_kernel(const __grid_constant__ Table<CAP> T) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __grid_constant__ Table<CAP> T) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float clip = 1.0f;
     if (T.partials) wait_dependency();
@@ -529,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<P, EIGHT, MASTER>()) ada
 
 template <typename P, bool EIGHT, bool MASTER, int CAP>
 cudaError_t launch_table(const Table<CAP>& T, int sms, cudaStream_t s) {
-    const uint32_t resident = static_cast<uint32_t>(sms) * ctas_per_sm<P, EIGHT, MASTER>();
+    const uint32_t resident = static_cast<uint32_t>(sms) * kCtasPerSm;
     const uint32_t units = EIGHT ? (T.chunks + kWarps - 1) / kWarps : T.chunks;
     uint32_t grid = units < resident ? units : resident;
     // Long steps: CTAs of four chunks each, which the hardware hands out as SMs become free. Equal shares of one resident

@@ -3,7 +3,10 @@
 //   g <- c g;  m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g g
 //   p <- p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // all in fp32 (products and sums rounded one by one: this file is built without contraction), p rounded once to its own type.
-// Bound by HBM: every parameter, gradient and moment is read once and written once.
+// Bound by HBM: every parameter, gradient and moment is read once and written once (28 bytes per fp32 element, 16 with
+// 8-bit moments, 10 in bf16 with them). Measured on a B200 (6.56 TB/s copy): 59M fp32 elements 244 us (6.8 TB/s), with
+// 8-bit moments 159 us (5.9 TB/s); 40M bf16 elements in 300 tensors with fp32 copies 171 us (6.6 TB/s), with 8-bit moments
+// and no copies 102 us (3.9 TB/s: 63 instructions per element at 76 % of the issue slots).
 //
 // Moments in 8 bits. 256 consecutive elements of a tensor (one warp's share) have one exponent byte E, the largest
 // exponent among them. A code q != 0 stands for the float with the bits (q + 8 (E + 1) - top) << 20: three mantissa
@@ -515,6 +518,8 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const double* __restrict
     }
 }
 
+// The step. With fp32 moments a CTA's warps share chunks of 2048 elements, with 8-bit ones each warp takes a run of blocks.
+// Aligned whole blocks move eight elements per lane (32-byte accesses in fp32).
 template <typename P, bool EIGHT, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __grid_constant__ Table<CAP> T) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -672,7 +677,9 @@ cudaError_t launch_all(const AdamwTensors& A, const AdamwHyper* hypers, int dtyp
 }
 
 // ---------------------------------------------------------------------------------------------------
-// sum of squared gradients: per-thread fp32 sums over 32 elements, added up in fp64; one partial sum per CTA
+// Sum of squared gradients: per-thread fp32 sums over 32 elements, added up in fp64; one partial sum per CTA, added in a
+// fixed order by the step (or clip_kernel). Bound by HBM: 80 MB of bf16 in 17 us (4.7 TB/s; with one load in flight per
+// thread 31 us).
 
 constexpr int kNormTensors = 1024;
 constexpr uint32_t kNormChunk = kThreads * 8 * 4;
@@ -744,7 +751,8 @@ __global__ void __launch_bounds__(kThreads, 5) grad_squares_kernel(const __grid_
 }
 
 // ---------------------------------------------------------------------------------------------------
-// values of 8-bit moments
+// Values of 8-bit moments: one byte in, two (bf16, exact) or four out. Bound by HBM: both moments of 59M elements to bf16
+// in 62 us (5.7 TB/s; with 16-byte instead of 32-byte stores 76 us).
 
 constexpr int kReadTensors = 768;
 struct ReadTable {

@@ -537,17 +537,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __gri
     }
     const uint32_t first = share_of(T.chunks, blockIdx.x, gridDim.x), end = share_of(T.chunks, blockIdx.x + 1, gridDim.x);
     if (first == end) return;
-    // with clipping the norm has just walked the same shares front to back: their ends are still in L2
-    const bool back = T.partials != nullptr;
     if constexpr (EIGHT) {
-        for (uint32_t i = first + warp; i < end; i += kWarps) update_run<P, MASTER>(T, back ? first + end - 1 - i : i, clip, lane);
+        for (uint32_t run = first + warp; run < end; run += kWarps) update_run<P, MASTER>(T, run, clip, lane);
     } else {
         const uint32_t at = static_cast<uint32_t>(warp) * kBlock;
-        int t = owner(T, back ? end - 1 : first);
-        for (uint32_t i = first; i < end; i++) {
-            const uint32_t chunk = back ? first + end - 1 - i : i;
+        int t = owner(T, first);
+        for (uint32_t chunk = first; chunk < end; chunk++) {
             while (chunk >= T.first[t + 1]) t++;
-            while (chunk < T.first[t]) t--;
             const Hyper& H = T.h[T.hyper[t] & 127];
             const uint64_t start = static_cast<uint64_t>(chunk - T.first[t]) * (kWarps * kBlock);
             const uint64_t left = T.n[t] - start;

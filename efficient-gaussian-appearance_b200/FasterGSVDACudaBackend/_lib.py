@@ -129,24 +129,28 @@ for _name, (_res, _args) in PROTOTYPES.items():
     _fn.argtypes = _args
 
 
-_HOST_PATH = _LIB_PATH.with_name('_fgs_host.so')
+_host = None
 
 
-def _load_host():
-    """The module of csrc/host.cpp (the host side of the many-tensor operators), bound to this library's entry points."""
-    if not _HOST_PATH.exists():
-        raise ImportError(f'{_HOST_PATH} not found; build it with `python efficient-gaussian-appearance_b200/build.py` (or __graft_entry__.build())')
-    import torch  # noqa: F401  (its libraries have to be loaded first)
-    spec = importlib.util.spec_from_file_location('_fgs_host', _HOST_PATH)
-    module = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(module)
-    module.bind(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
-        'fgs_last_error', 'fgs_adamw_step', 'fgs_grad_squares_capacity', 'fgs_grad_squares', 'fgs_adamw_read_moments', 'fgs_embedding_lookup',
-        'fgs_embedding_workspace_bytes', 'fgs_embedding_grad')))
-    return module
-
-
-host = _load_host()
+def host():
+    """The module of csrc/host.cpp (the host side of the many-tensor operators, built against the installed torch), bound to
+    this library's entry points. Loaded at its first use; raises ImportError if it is missing."""
+    global _host
+    if _host is None:
+        beside, own = _LIB_PATH.with_name('_fgs_host.so'), Path(__file__).resolve().parent / 'lib' / '_fgs_host.so'
+        path = beside if beside.exists() else own
+        if not path.exists():
+            raise ImportError(f'_fgs_host.so not found at {path}; build it with `python efficient-gaussian-appearance_b200/build.py` '
+                              f'(or __graft_entry__.build())')
+        import torch  # noqa: F401  (its libraries have to be loaded first)
+        spec = importlib.util.spec_from_file_location('_fgs_host', path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in (
+            'fgs_last_error', 'fgs_adamw_step', 'fgs_grad_squares_capacity', 'fgs_grad_squares', 'fgs_adamw_read_moments', 'fgs_embedding_lookup',
+            'fgs_embedding_workspace_bytes', 'fgs_embedding_grad')))
+        _host = module
+    return _host
 
 
 def check(rc: int) -> None:

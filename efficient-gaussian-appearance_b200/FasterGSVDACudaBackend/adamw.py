@@ -26,8 +26,8 @@ class FusedAdamW(torch.optim.Optimizer):
         changes are kept; the same inputs give the same codes). read_moments() gives their values.
       master_weights=True: half-precision parameters keep a float32 copy in the state ('master'), which is updated; the
         parameter is its rounding. Float32 parameters need none.
-    `max_grad_norm` (for all groups together): gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) as they are
-    read, p.grad stays as it is, and `grad_norm` then holds the norm (a 0-dim device tensor, a new one at each step; None
+    `max_grad_norm` (for all groups together; inf only measures): gradients are scaled by min(1, max_grad_norm /
+    (norm + 1e-6)) as they are read, p.grad stays as it is, and `grad_norm` then holds the norm (a 0-dim device tensor, a new one at each step; None
     after a step without clipping or gradients). An
     infinite or NaN gradient makes the norm infinite or NaN: the step is then not skipped, what it scales by 0 or NaN
     becomes so.
@@ -85,7 +85,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        self.grad_norm = host.adamw_step(self.state, self.param_groups, self._new_state, self.max_grad_norm)
+        self.grad_norm = host().adamw_step(self.state, self.param_groups, self._new_state, self.max_grad_norm)
         return loss
 
     @torch.no_grad()
@@ -100,7 +100,7 @@ class FusedAdamW(torch.optim.Optimizer):
             exp_avgs, exp_avg_sqs = ([torch.empty(p.shape, dtype=dtype, device=p.device) for p in params] for _ in range(2))
         if len(exp_avgs) != len(params) or len(exp_avg_sqs) != len(params):
             raise ValueError('one tensor per parameter is needed')
-        host.read_moments(self.state, params, list(exp_avgs), list(exp_avg_sqs))
+        host().read_moments(self.state, params, list(exp_avgs), list(exp_avg_sqs))
         return exp_avgs, exp_avg_sqs
 
     def load_state_dict(self, state_dict: dict) -> None:

@@ -15,4 +15,4 @@ def embedding_lookup(table: torch.Tensor, indices: torch.Tensor, scale: float = 
     Differentiable in `table` (once). The gradient is dense, scale * the sum of the output gradients of each row's
     indices: summed in float32 in an order that depends only on the inputs (and the alignment of the gradient's address),
     so the same inputs give the same bits. Both directions may be captured into CUDA graphs."""
-    return host.embedding_lookup(table, indices, scale, padding_index)
+    return host().embedding_lookup(table, indices, scale, padding_index)

@@ -74,7 +74,7 @@ PyObject* must(PyObject* o) {
     return o;
 }
 
-// Runs f() for Python: C++ exceptions become Python ones.
+// Runs f() for Python: every C++ exception becomes a Python one.
 template <typename F>
 PyObject* guarded(F&& f) {
     try {
@@ -87,6 +87,8 @@ PyObject* guarded(F&& f) {
         PyErr_SetString(PyExc_ValueError, e.what());
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {
+        PyErr_SetString(PyExc_RuntimeError, "unknown error in _fgs_host");
     }
     return nullptr;
 }

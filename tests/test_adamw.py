@@ -70,7 +70,7 @@ def test_layouts_refused():
 
 def test_entries_of_the_host_module_refuse():
     import FasterGSVDACudaBackend as F
-    host = F._lib.host
+    host = F._lib.host()
     with pytest.raises(TypeError):
         host.adamw_step([], [], None, None)
     for groups, match in (([3], 'dicts'), ([{}], 'params'), ([{'params': ()}], 'list'), ([{'params': [3], 'state_bits': 8, 'master_weights': 0}], 'tensor'),

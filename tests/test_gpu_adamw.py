@@ -118,13 +118,14 @@ def test_steps_against_the_formula(cuda, dtype, master, bits, clip, misalign):
 
 def test_norm_below_the_limit_changes_nothing(cuda):
     import FasterGSVDACudaBackend as F
-    a, b = _params(SHAPES, torch.float32, cuda), _params(SHAPES, torch.float32, cuda)
-    one, two = F.FusedAdamW(a), F.FusedAdamW(b, max_grad_norm=1e9)
-    for params, opt in ((a, one), (b, two)):
+    a, b, c = (_params(SHAPES, torch.float32, cuda) for _ in range(3))
+    one, two, three = F.FusedAdamW(a), F.FusedAdamW(b, max_grad_norm=1e9), F.FusedAdamW(c, max_grad_norm=float('inf'))
+    for params, opt in ((a, one), (b, two), (c, three)):
         _grads(params, 1)
         opt.step()
-    for p, q in zip(a, b):
-        assert torch.equal(p, q)
+    for p, q, r in zip(a, b, c):
+        assert torch.equal(p, q) and torch.equal(p, r)
+    assert torch.equal(two.grad_norm, three.grad_norm)
     assert one.grad_norm is None and two.grad_norm.shape == ()
 
 

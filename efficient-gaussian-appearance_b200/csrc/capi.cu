@@ -733,7 +733,7 @@ int fgs_adam_step(const fgs_adam_segment* segs, int n, void* stream) {
     return FGS_OK;
 }
 
-int fgs_adamw_step(const fgs_adamw_tensors* t, const fgs_adamw_hyper* hypers, int n_hypers, int dtype, int state_bits, const double* partials,
+int fgs_adamw_step(const fgs_adamw_tensors* t, const fgs_adamw_hyper* hypers, int n_hypers, int dtype, int state_bits, double* partials,
                    int n_partials, double max_norm, float* grad_norm, void* stream) {
     static_assert(FGS_ADAMW_BLOCK == fgs::kAdamwBlock && FGS_DTYPE_F32 == int(fgs::kDtypeF32) && FGS_DTYPE_BF16 == int(fgs::kDtypeBf16) &&
                       FGS_DTYPE_F16 == int(fgs::kDtypeF16),
@@ -782,7 +782,7 @@ int fgs_adamw_step(const fgs_adamw_tensors* t, const fgs_adamw_hyper* hypers, in
         }
         const fgs::AdamwTensors A{static_cast<int>(t->count), t->param, t->grad, t->exp_avg, t->exp_avg_sq, t->exp_avg_exponent,
                                   t->exp_avg_sq_exponent, t->master, t->n_elements, t->hyper};
-        const fgs::AdamwClip clip{partials, n_partials, max_norm, grad_norm ? grad_norm + 1 : nullptr, grad_norm};
+        const fgs::AdamwClip clip{partials, n_partials, max_norm, reinterpret_cast<float*>(partials + (partials ? n_partials : 0)), grad_norm};
         ProfScope p_("adamw", static_cast<cudaStream_t>(stream));
         FGS_CUDA(fgs::launch_adamw(A, H.data(), dtype, eight, master, clip, static_cast<cudaStream_t>(stream)), "adamw");
     } catch (const std::exception& e) {
@@ -793,7 +793,7 @@ int fgs_adamw_step(const fgs_adamw_tensors* t, const fgs_adamw_hyper* hypers, in
 
 int fgs_grad_squares_capacity(int64_t count, int* out) {
     if (!out || count < 0 || count > 0x7FFFFF) return fail(FGS_ERR_INVALID_ARGUMENT, "bad argument");
-    *out = fgs::grad_squares_launches(static_cast<int>(count)) * fgs::kNormPartials;
+    *out = fgs::grad_squares_launches(static_cast<int>(count)) * fgs::kNormPartials + 1;  // one for the clip factor
     return FGS_OK;
 }
 

@@ -274,7 +274,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                         room += need;
                     }
             partials = at::empty({room}, on.dtype(at::kDouble));
-            norm = at::empty({2}, on.dtype(at::kFloat));  // the norm, and room for the clip factor
+            norm = at::empty({}, on.dtype(at::kFloat));
             double* to = partials.data_ptr<double>();
             for (int code = 0; code < 3; code++)
                 for (auto& by_bits : jobs[code])
@@ -313,7 +313,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
             if (PyDict_SetItem(c.first, names.step, count.p)) throw PythonError();
         }
         if (!norm.defined()) Py_RETURN_NONE;
-        return THPVariable_Wrap(norm.select(0, 0));
+        return THPVariable_Wrap(norm);
     });
 }
 

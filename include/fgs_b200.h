@@ -221,12 +221,13 @@ typedef struct {
     const int64_t* n_elements;
     const int32_t* hyper;           /* index into the hyperparameter sets */
 } fgs_adamw_tensors;
-/* `partials`: the n_partials values of fgs_grad_squares (any number of its calls, one after another in one array), or
- * NULL for no clipping; grad_norm (needed with partials): two device floats, which receive the norm and the clip factor. */
+/* `partials`: the n_partials values of fgs_grad_squares (any number of its calls, one after another in one array) with room
+ * for one value behind them, or NULL for no clipping; grad_norm (needed with partials): one device float, which receives
+ * the norm. */
 int fgs_adamw_step(const fgs_adamw_tensors* tensors, const fgs_adamw_hyper* hypers, int n_hypers, int dtype, int state_bits,
-                   const double* partials, int n_partials, double max_norm, float* grad_norm, void* stream);
+                   double* partials, int n_partials, double max_norm, float* grad_norm, void* stream);
 /* partial sums of the squared elements of `count` tensors (types may differ), in a fixed order; *n_partials receives
- * their number, at most the capacity that fgs_grad_squares_capacity returns for the same count */
+ * their number, less than the capacity that fgs_grad_squares_capacity returns for the same count */
 int fgs_grad_squares_capacity(int64_t count, int* out);
 int fgs_grad_squares(const void* const* grads, const int64_t* n_elements, const uint8_t* dtypes, int64_t count, double* partials, int capacity,
                      int* n_partials, void* stream);

@@ -72,7 +72,8 @@ constexpr uint32_t kMaxRun = 8;  // blocks of a warp's run (at most 32: one lane
 
 // whether the hardware hands out the CTAs as SMs become free (else: one resident grid, equal shares)
 inline bool long_step(uint32_t chunks, uint32_t blocks, int sms) { return static_cast<uint64_t>(chunks) * blocks > static_cast<uint64_t>(sms) * 4 * kWarps * 8; }
-constexpr int kFewTensors = 24, kManyTensors = 384;
+// Tables of three sizes: a launch copies the whole table, and 28 KB of it took 3 us more of the host than 2 KB.
+constexpr int kFewTensors = 24, kSomeTensors = 96, kManyTensors = 384;
 static_assert(sizeof(Table<kManyTensors>) <= 32764, "kernel parameter limit");
 
 __device__ inline float to_float(float x) { return x; }
@@ -680,16 +681,17 @@ cudaError_t launch_all(const AdamwTensors& A, const AdamwHyper* hypers, int dtyp
 constexpr int kNormTensors = 1024;
 constexpr uint32_t kNormChunk = kThreads * 8 * 4;
 
+template <int CAP>
 struct NormTable {
-    uint32_t first[kNormTensors + 1];
-    const void* grad[kNormTensors];
-    uint64_t n[kNormTensors];
-    uint8_t kind[kNormTensors];  // dtype; bit 7: aligned for whole-lane loads
+    uint32_t first[CAP + 1];
+    const void* grad[CAP];
+    uint64_t n[CAP];
+    uint8_t kind[CAP];  // dtype; bit 7: aligned for whole-lane loads
     int n_tensors;
     uint32_t chunks;
     double* partials;
 };
-static_assert(sizeof(NormTable) <= 32764, "kernel parameter limit");
+static_assert(sizeof(NormTable<kNormTensors>) <= 32764, "kernel parameter limit");
 
 // 16 bytes, issued where it stands: the compiler would otherwise wait for each load before it issues the next one
 __device__ inline uint4 load16(const void* a) {
@@ -724,7 +726,8 @@ __device__ inline float chunk_squares(const P* g, uint64_t left, bool vec) {
     return s;
 }
 
-__global__ void __launch_bounds__(kThreads, 5) grad_squares_kernel(const __grid_constant__ NormTable T) {
+template <int CAP>
+__global__ void __launch_bounds__(kThreads, 5) grad_squares_kernel(const __grid_constant__ NormTable<CAP> T) {
     __shared__ double scratch[kWarps];
     allow_dependent();
     double total = 0.0;
@@ -751,17 +754,18 @@ __global__ void __launch_bounds__(kThreads, 5) grad_squares_kernel(const __grid_
 // in 62 us (5.7 TB/s; with 16-byte instead of 32-byte stores 76 us).
 
 constexpr int kReadTensors = 768;
+template <int CAP>
 struct ReadTable {
-    uint32_t first[kReadTensors + 1];
-    const uint8_t* codes[kReadTensors];
-    const uint8_t* exps[kReadTensors];
-    void* out[kReadTensors];
-    uint64_t n[kReadTensors];
-    uint8_t kind[kReadTensors];  // bit 0: signed, bit 7: aligned
+    uint32_t first[CAP + 1];
+    const uint8_t* codes[CAP];
+    const uint8_t* exps[CAP];
+    void* out[CAP];
+    uint64_t n[CAP];
+    uint8_t kind[CAP];  // bit 0: signed, bit 7: aligned
     int n_tensors;
     uint32_t chunks;
 };
-static_assert(sizeof(ReadTable) <= 32764, "kernel parameter limit");
+static_assert(sizeof(ReadTable<kReadTensors>) <= 32764, "kernel parameter limit");
 
 constexpr uint32_t kReadBlocks = 4;  // blocks of a warp's run
 
@@ -805,8 +809,8 @@ __device__ inline void read_blocks(const uint8_t* codes, const uint8_t* exps, O*
     }
 }
 
-template <typename O>
-__global__ void __launch_bounds__(kThreads) read_moments_kernel(const __grid_constant__ ReadTable T) {
+template <typename O, int CAP>
+__global__ void __launch_bounds__(kThreads) read_moments_kernel(const __grid_constant__ ReadTable<CAP> T) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t first = share_of(T.chunks, blockIdx.x, gridDim.x), end = share_of(T.chunks, blockIdx.x + 1, gridDim.x);
     int t = owner(T, first);
@@ -826,18 +830,20 @@ __global__ void __launch_bounds__(kThreads) read_moments_kernel(const __grid_con
 
 cudaError_t launch_adamw(const AdamwTensors& A, const AdamwHyper* hypers, int dtype, bool eight, bool master, const AdamwClip& clip, cudaStream_t s) {
     if (A.count <= kFewTensors) return launch_all<kFewTensors>(A, hypers, dtype, eight, master, clip, s);
+    if (A.count <= kSomeTensors) return launch_all<kSomeTensors>(A, hypers, dtype, eight, master, clip, s);
     return launch_all<kManyTensors>(A, hypers, dtype, eight, master, clip, s);
 }
 
-cudaError_t launch_grad_squares(const void* const* grads, const int64_t* n_elements, const uint8_t* dtypes, int count, double* partials,
+template <int CAP>
+static cudaError_t grad_squares_by(const void* const* grads, const int64_t* n_elements, const uint8_t* dtypes, int count, double* partials,
                                 int* n_partials, cudaStream_t s) {
     *n_partials = 0;
     int i = 0;
     while (i < count) {
-        NormTable T;
+        NormTable<CAP> T;
         int k = 0;
         uint64_t chunks = 0;
-        for (; i < count && k < kNormTensors; i++) {
+        for (; i < count && k < CAP; i++) {
             if (n_elements[i] <= 0) continue;
             T.grad[k] = grads[i];
             T.n[k] = static_cast<uint64_t>(n_elements[i]);
@@ -854,7 +860,7 @@ cudaError_t launch_grad_squares(const void* const* grads, const int64_t* n_eleme
         // one resident grid, or CTAs of two chunks that the hardware hands out as SMs become free
         const uint64_t resident = 148 * 5;
         const int grid = static_cast<int>(chunks < resident ? chunks : chunks < 2 * resident ? resident : chunks < 2 * kNormPartials ? chunks / 2 : kNormPartials);
-        grad_squares_kernel<<<grid, kThreads, 0, s>>>(T);
+        grad_squares_kernel<CAP><<<grid, kThreads, 0, s>>>(T);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return e;
         *n_partials += grid;
@@ -862,17 +868,24 @@ cudaError_t launch_grad_squares(const void* const* grads, const int64_t* n_eleme
     return cudaSuccess;
 }
 
+cudaError_t launch_grad_squares(const void* const* grads, const int64_t* n_elements, const uint8_t* dtypes, int count, double* partials,
+                                int* n_partials, cudaStream_t s) {
+    if (count <= kSomeTensors) return grad_squares_by<kSomeTensors>(grads, n_elements, dtypes, count, partials, n_partials, s);
+    return grad_squares_by<kNormTensors>(grads, n_elements, dtypes, count, partials, n_partials, s);
+}
+
 int grad_squares_launches(int count) { return (count + kNormTensors - 1) / kNormTensors; }
 
-cudaError_t launch_read_moments(const uint8_t* const* codes, const uint8_t* const* exps, const uint8_t* is_signed, const int64_t* n_elements, int count,
+template <int CAP>
+static cudaError_t read_moments_by(const uint8_t* const* codes, const uint8_t* const* exps, const uint8_t* is_signed, const int64_t* n_elements, int count,
                                 void* const* out, int dtype, cudaStream_t s) {
     const uint32_t cap = static_cast<uint32_t>(sm_count()) * 8;
     int i = 0;
     while (i < count) {
-        ReadTable T;
+        ReadTable<CAP> T;
         int k = 0;
         uint64_t chunks = 0;
-        for (; i < count && k < kReadTensors; i++) {
+        for (; i < count && k < CAP; i++) {
             if (n_elements[i] <= 0) continue;
             T.codes[k] = codes[i];
             T.exps[k] = exps[i];
@@ -888,12 +901,18 @@ cudaError_t launch_read_moments(const uint8_t* const* codes, const uint8_t* cons
         T.first[k] = T.chunks = static_cast<uint32_t>(chunks);
         T.n_tensors = k;
         const uint32_t grid = T.chunks < cap ? T.chunks : cap;
-        if (dtype == kDtypeF32) read_moments_kernel<float><<<grid, kThreads, 0, s>>>(T);
-        else read_moments_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(T);
+        if (dtype == kDtypeF32) read_moments_kernel<float, CAP><<<grid, kThreads, 0, s>>>(T);
+        else read_moments_kernel<__nv_bfloat16, CAP><<<grid, kThreads, 0, s>>>(T);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
+}
+
+cudaError_t launch_read_moments(const uint8_t* const* codes, const uint8_t* const* exps, const uint8_t* is_signed, const int64_t* n_elements, int count,
+                                void* const* out, int dtype, cudaStream_t s) {
+    if (count <= kSomeTensors) return read_moments_by<kSomeTensors>(codes, exps, is_signed, n_elements, count, out, dtype, s);
+    return read_moments_by<kReadTensors>(codes, exps, is_signed, n_elements, count, out, dtype, s);
 }
 
 }  // namespace fgs

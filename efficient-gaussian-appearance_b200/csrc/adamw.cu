@@ -166,16 +166,7 @@ __device__ inline void load_codes(const uint8_t* a, int lane, uint32_t left, uin
         for (int j = 0; j < 8; j++) q[j] = place<VEC>(lane, j) < left ? a[place<VEC>(lane, j)] : 0u;
     }
 }
-template <bool VEC>
-__device__ inline void store_codes(uint8_t* a, int lane, uint32_t left, const uint32_t* q) {
-    if (VEC) {
-        *reinterpret_cast<uint2*>(a + lane * 8) = make_uint2(q[0], q[1]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (place<VEC>(lane, j) < left) a[place<VEC>(lane, j)] = static_cast<uint8_t>(q[j]);
-    }
-}
+__device__ inline void store_codes(uint8_t* a, int lane, const uint32_t (&q)[2]) { *reinterpret_cast<uint2*>(a + lane * 8) = make_uint2(q[0], q[1]); }
 
 // Square root within 2^-23 of the value, reciprocal too: with the product 5 roundings of half a step on an update that is
 // itself a small part of the parameter; the exact ones took half of the 8-bit step's instructions. The reciprocal takes
@@ -312,7 +303,7 @@ template <typename P, bool EIGHT, bool MASTER>
 struct Loaded {
     float p[8], g[8], m[8], v[8];
     uint4 packed_p, packed_g;
-    uint32_t qm[8], qv[8];
+    uint32_t qm[2], qv[2];
 };
 
 template <typename P, bool EIGHT, bool MASTER, bool VEC>
@@ -323,9 +314,10 @@ __device__ inline void load_all(const Chunk<P>& C, uint32_t at, uint32_t left, i
     if (MASTER) load_block<VEC>(C.master + at, lane, left, L.p);
     else if (packed) L.packed_p = load16_rw(C.param + at + lane * 8);
     else load_block<VEC>(C.param + at, lane, left, L.p);
-    if (EIGHT) {
-        load_codes<VEC>(static_cast<const uint8_t*>(C.m) + at, lane, left, L.qm);
-        load_codes<VEC>(static_cast<const uint8_t*>(C.v) + at, lane, left, L.qv);
+    if constexpr (EIGHT) {
+        static_assert(VEC, "cut blocks of 8-bit moments: cut_block");
+        load_codes<true>(static_cast<const uint8_t*>(C.m) + at, lane, left, L.qm);
+        load_codes<true>(static_cast<const uint8_t*>(C.v) + at, lane, left, L.qv);
     } else {
         load_block<VEC>(static_cast<const float*>(C.m) + at, lane, left, L.m);
         load_block<VEC>(static_cast<const float*>(C.v) + at, lane, left, L.v);
@@ -339,9 +331,9 @@ __device__ inline void update(const Hyper& H, uint64_t start, float clip, int la
         unpack8<P>(L.packed_g, L.g);
         if (!MASTER) unpack8<P>(L.packed_p, L.p);
     }
-    if (EIGHT) {
-        decode<true, VEC>(L.qm, static_cast<int>(em), L.m);
-        decode<false, VEC>(L.qv, static_cast<int>(ev), L.v);
+    if constexpr (EIGHT) {
+        decode<true, true>(L.qm, static_cast<int>(em), L.m);
+        decode<false, true>(L.qv, static_cast<int>(ev), L.v);
     }
     // the moments decide the codes, so their products and sums are rounded one by one; the update is not coded
 #pragma unroll
@@ -370,13 +362,12 @@ __device__ inline void store_all(const Chunk<P>& C, const Hyper& H, uint64_t sta
     if (MASTER) store_block<VEC>(C.master + at, lane, left, p);
     store_block<VEC>(C.param + at, lane, left, p);
     if constexpr (EIGHT) {
-        static_assert(VEC, "cut blocks of 8-bit moments: cut_block");
         uint32_t q[2];
         const uint32_t u = static_cast<uint32_t>(start) * kTurn;
         em = encode<true>(m, u + H.dither_m, lane, q);
-        store_codes<VEC>(static_cast<uint8_t*>(C.m) + at, lane, left, q);
+        store_codes(static_cast<uint8_t*>(C.m) + at, lane, q);
         ev = encode<false>(v, u + H.dither_v, lane, q);
-        store_codes<VEC>(static_cast<uint8_t*>(C.v) + at, lane, left, q);
+        store_codes(static_cast<uint8_t*>(C.v) + at, lane, q);
     } else {
         store_block<VEC>(static_cast<float*>(C.m) + at, lane, left, m);
         store_block<VEC>(static_cast<float*>(C.v) + at, lane, left, v);

@@ -32,7 +32,8 @@ class FusedAdamW(torch.optim.Optimizer):
     infinite or NaN gradient makes the norm infinite or NaN: the step is then not skipped, what it scales by 0 or NaN
     becomes so.
 
-    Parameters, gradients and state must be contiguous CUDA tensors on one device. The step count is a host value, so a
+    Parameters, gradients and state must be contiguous CUDA tensors on one device, and no two parameters may share
+    memory. The step count is a host value, so a
     step cannot be captured into a CUDA graph (RuntimeError). Anything refused is refused before a kernel is launched
     and leaves parameters, state and step counts as they were.
     """

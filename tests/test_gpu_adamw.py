@@ -1,6 +1,7 @@
 """FusedAdamW on the GPU against its formula in 64 bits (tolerances counted in roundings: oracle/adamw.py bounds) and, for
 8-bit moments, bit for bit against the restatement of the block format."""
 import copy
+import warnings
 
 import numpy as np
 import pytest
@@ -434,3 +435,26 @@ def test_more_than_2_31_elements(cuda):
                 O.thresholds = keep
             np.testing.assert_array_equal(s[name][first:k.stop].cpu().numpy(), q)
             np.testing.assert_array_equal(s[name + '_exponent'][first // 256:first // 256 + e.size].cpu().numpy(), e)
+
+
+def test_parameters_of_one_memory_are_refused(cuda):
+    """The same parameter twice, or two that overlap, would be updated by two threads at once; neighbours are not touched."""
+    import FasterGSVDACudaBackend as F
+    flat = torch.ones(1024, device=cuda)
+    a, b = (torch.nn.Parameter(flat[s]) for s in (slice(0, 512), slice(512, 1024)))
+    c = torch.nn.Parameter(flat[500:600])
+    half = torch.nn.Parameter(flat[508:512].view(torch.bfloat16))
+    empty = torch.nn.Parameter(flat[100:100])
+    for p in (a, b, c, half, empty):
+        p.grad = torch.ones_like(p)
+    with warnings.catch_warnings():
+        warnings.simplefilter('ignore')
+        twice = F.FusedAdamW([b, a, b])
+    for opt in (twice, F.FusedAdamW([a, c]), F.FusedAdamW([c, b]), F.FusedAdamW([half, b, a])):
+        with pytest.raises(RuntimeError, match='share memory'):
+            opt.step()
+        assert all(not opt.state[p] for p in (a, b, c, half))
+    torch.cuda.synchronize()
+    assert (flat == 1).all()
+    F.FusedAdamW([b, empty, a]).step()
+    assert (flat < 1).all()

@@ -124,6 +124,11 @@ const at::Tensor& tensor_of(PyObject* o, const char* name) {
     return THPVariable_Unpack(o);
 }
 
+// Tells autograd of a change in place: a graph that saved the tensor before raises an error in its backward.
+void changed(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // names of the state and of the group options, made once
 struct Names {
     PyObject *params, *lr, *betas, *eps, *weight_decay, *state_bits, *master_weights, *step, *exp_avg, *exp_avg_sq, *exp_avg_exponent,
@@ -208,6 +213,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
         std::vector<fgs_adamw_hyper> hypers;
         std::vector<Py_ssize_t> hyper_group;
         std::vector<std::pair<PyObject*, int64_t>> counted;  // states and their new step counts (borrowed)
+        std::vector<PyObject*> updated;                      // borrowed
         Ref fresh(must(PyList_New(0)));                      // parameter, state, parameter, state ...
         int device = -1;
         bool any = false;
@@ -262,6 +268,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                 }
                 if (master) job.master.push_back(static_cast<float*>(address(state_tensor(state, names.master), "master", FGS_DTYPE_F32, n, device)));
                 job.count.push_back(n);
+                updated.push_back(o);
                 size_t h = hypers.size();
                 while (h > 0 && hyper_group[h - 1] == gi && hypers[h - 1].step != t) h--;
                 if (h == 0 || hyper_group[h - 1] != gi) {
@@ -318,6 +325,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                                          n_partials ? partials.data_ptr<double>() : nullptr, n_partials, max_norm,
                                          n_partials ? norm.data_ptr<float>() : nullptr, stream));
                 }
+        for (PyObject* o : updated) changed(THPVariable_Unpack(o));
         for (Py_ssize_t i = 0; i < PyList_GET_SIZE(fresh.p); i += 2)
             if (PyDict_SetItem(all_state, PyList_GET_ITEM(fresh.p, i), PyList_GET_ITEM(fresh.p, i + 1))) throw PythonError();
         Ref count;  // most parameters have the same step count
@@ -387,6 +395,8 @@ PyObject* read_moments(PyObject*, PyObject* args) {
         }
         check(lib.read_moments(codes.data(), exponents.data(), is_signed.data(), counts.data(), static_cast<int64_t>(codes.size()), to.data(), out_code,
                                c10::cuda::getCurrentCUDAStream().stream()));
+        for (PyObject* list : outs)
+            for (Py_ssize_t i = 0; i < n; i++) changed(THPVariable_Unpack(PyList_GET_ITEM(list, i)));
         Py_RETURN_NONE;
     });
 }

@@ -458,3 +458,23 @@ def test_parameters_of_one_memory_are_refused(cuda):
     assert (flat == 1).all()
     F.FusedAdamW([b, empty, a]).step()
     assert (flat < 1).all()
+
+
+@pytest.mark.parametrize('clip', [None, 1.0])
+def test_a_step_is_a_change_in_place_for_autograd(cuda, clip):
+    """A graph that saved a parameter before the step must not go on with the new values; read moments neither."""
+    import FasterGSVDACudaBackend as F
+    p, idle = _params([(40, 6), (8,)], torch.float32, cuda)
+    opt = F.FusedAdamW([p, idle], max_grad_norm=clip)
+    loss, other = (p * p).sum(), (idle * idle).sum()
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    other.backward()  # not updated: as it was
+    outs = [[torch.zeros(40, 6, device=cuda), torch.zeros(8, device=cuda)] for _ in range(2)]
+    x = torch.ones(40, 6, device=cuda, requires_grad=True)
+    loss = (x * outs[0][0]).sum()
+    opt.read_moments(*outs)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()

@@ -429,8 +429,19 @@ struct LookupBackward : torch::autograd::Node {
     std::string name() const override { return "EmbeddingLookupBackward"; }
     void release_variables() override { indices.reset_data(); }
 
+    // A leaf's accumulation runs on the stream on which its first living graph was made. If that is the default stream
+    // and this backward is being captured, the engine would have the default stream wait for a captured event.
+    void refuse_uncapturable() const {
+        const auto& leaf = next_edge(0).function;
+        if (!leaf || leaf->num_outputs() != 0) return;
+        const auto at = leaf->stream();
+        if (at && at->id() == 0 && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+            refuse("the backward of embedding_lookup cannot be captured while a graph of the table made on the default stream lives: release it first");
+    }
+
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         if (!grads[0].defined()) return {at::Tensor()};
+        refuse_uncapturable();
         const at::Tensor idx = indices.unpack();
         at::Tensor grad;
         {

@@ -291,6 +291,28 @@ def test_captured_and_replayed(cuda, rows, tokens):
             _check_grad(grad, g, idx, 3.0)
 
 
+def test_capture_beside_an_eager_graph(cuda):
+    """A graph of the table that lives on the default stream: a captured backward is refused, an eager one is not."""
+    import FasterGSVDACudaBackend as F
+    table, idx, g = _inputs(cuda, 30, 16, 100, torch.float32, 'even', torch.int64)
+    table.requires_grad_(True)
+    eager = F.embedding_lookup(table, idx)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match='release it first'):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(F.embedding_lookup(table, idx), table, g)
+    torch.cuda.synchronize()
+    grad, = torch.autograd.grad(eager, table, g)
+    _check_grad(grad, g, idx, 1.0)
+    del eager, grad
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grad, = torch.autograd.grad(F.embedding_lookup(table, idx), table, g)
+    graph.replay()
+    torch.cuda.synchronize()
+    _check_grad(grad, g, idx, 1.0)
+
+
 def test_saved_indices(cuda):
     """The backward needs the indices of the forward: a changed or released copy is an error, not another gradient."""
     import FasterGSVDACudaBackend as F

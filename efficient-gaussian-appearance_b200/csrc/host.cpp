@@ -489,6 +489,7 @@ PyObject* embedding_lookup(PyObject*, PyObject* args) {
         const int code = type_code(table);
         if (table.layout() != at::kStrided || !table.is_cuda() || code < 0 || code > FGS_DTYPE_F16 || table.dim() < 1 || !table.is_contiguous())
             refuse("table must be a contiguous CUDA float32, bfloat16 or float16 tensor [rows, ...]");
+        if (table._fw_grad(0).defined()) refuse("embedding_lookup has no forward-mode derivative");
         const at::Tensor& given = tensor_of(indices_o, "indices");
         if (given.layout() != at::kStrided || (given.scalar_type() != at::kLong && given.scalar_type() != at::kInt) || given.device() != table.device())
             refuse("indices must be an int64 or int32 tensor on the device of the table");

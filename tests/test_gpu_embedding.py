@@ -355,3 +355,16 @@ def test_refusals(cuda):
     grad, = torch.autograd.grad(F.embedding_lookup(table, idx).sum(), table, create_graph=True)
     with pytest.raises(RuntimeError):
         grad.sum().backward()
+
+
+def test_forward_mode_is_refused(cuda):
+    import FasterGSVDACudaBackend as F
+    from torch.autograd import forward_ad
+    table, idx = torch.randn(8, 4, device=cuda), torch.zeros(3, dtype=torch.int64, device=cuda)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(table, torch.ones_like(table))
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            F.embedding_lookup(dual, idx)
+        assert torch.equal(F.embedding_lookup(table, idx), table[idx])
+    with pytest.raises(RuntimeError):  # tensors of a function transform have no memory of their own
+        torch.func.vmap(lambda t: F.embedding_lookup(t, idx))(table[None].expand(2, 8, 4).contiguous())

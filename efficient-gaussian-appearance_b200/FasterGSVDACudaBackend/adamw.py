@@ -29,15 +29,14 @@ class FusedAdamW(torch.optim.Optimizer):
       master_weights=True: half-precision parameters keep a float32 copy in the state ('master'), which is updated; the
         parameter is its rounding. Float32 parameters need none.
     `max_grad_norm` (for all groups together; inf only measures): gradients are scaled by min(1, max_grad_norm /
-    (norm + 1e-6)) as they are read, p.grad stays as it is, and `grad_norm` then holds the norm (a 0-dim device tensor, a new one at each step; None
-    after a step without clipping or gradients). An
-    infinite or NaN gradient makes the norm infinite or NaN: the step is then not skipped, what it scales by 0 or NaN
+    (norm + 1e-6)) as they are read, p.grad stays as it is, and `grad_norm` then holds the norm (a 0-dim device tensor, a
+    new one at each step; None after a step without clipping or gradients). An infinite or NaN gradient makes the norm infinite or NaN: the step is then not skipped, what it scales by 0 or NaN
     becomes so.
 
     Parameters, gradients and state must be contiguous CUDA tensors on one device, and no two parameters may share
     memory. The step count is a host value, so a
     step cannot be captured into a CUDA graph (RuntimeError). Anything refused is refused before a kernel is launched
-    and leaves parameters, state and step counts as they were.
+    and leaves parameters, state and step counts as they were. For autograd a step is a change in place.
     """
 
     grad_norm = None

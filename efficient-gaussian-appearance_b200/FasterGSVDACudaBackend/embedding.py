@@ -12,8 +12,8 @@ def embedding_lookup(table: torch.Tensor, indices: torch.Tensor, scale: float = 
     device. A negative index, or `padding_index`, stands for no row: zeros, and no gradient. An index past the table is
     not read: its output is NaN, and it adds to no gradient (nothing is copied to the host to raise an error).
 
-    Differentiable in `table` (once, backward only). The gradient is dense, scale * the sum of the output gradients of each row's
-    indices: summed in float32 in an order that depends only on the inputs (and the alignment of the gradient's address),
-    so the same inputs give the same bits. Both directions may be captured into CUDA graphs (the backward not
-    while an eager graph of the table, made on the default stream, lives: RuntimeError)."""
+    Differentiable in `table` (once, backward only). The gradient is dense, scale * the sum of the output gradients of
+    each row's indices: summed in float32 in an order that depends only on the inputs (and the alignment of the
+    gradient's address), so the same inputs give the same bits. Both directions may be captured into CUDA graphs (the
+    backward not while an eager graph of the table, made on the default stream, lives: RuntimeError)."""
     return host().embedding_lookup(table, indices, scale, padding_index)

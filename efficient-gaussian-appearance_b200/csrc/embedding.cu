@@ -435,8 +435,8 @@ cudaError_t cluster_sort(const EmbeddingArgs& a, const void* index, int end_bit,
     return launch_cluster_sort<I, 8>(a, index, end_bit, keys, vals, s);
 }
 
-// Clears a gradient (102 MB in 22 us beside the sort) on the SMs that the sort before it leaves idle: launched as its programmatic dependent, so it starts
-// with the sort, and waits for the sort's end before its own.
+// Clears a gradient (102 MB in 22 us beside the sort) on the SMs that the sort before it leaves idle: launched as its
+// programmatic dependent, so it starts with the sort, and waits for the sort's end before its own.
 __global__ void __launch_bounds__(kThreads) clear_kernel(uint4* __restrict__ to, uint64_t bytes) {
     const uint64_t n = bytes / 16, stride = static_cast<uint64_t>(gridDim.x) * kThreads;
     const uint64_t i0 = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;

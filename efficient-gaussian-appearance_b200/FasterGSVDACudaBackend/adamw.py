@@ -35,7 +35,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     Parameters, gradients and state must be contiguous CUDA tensors on one device, and no two parameters may share
     memory. The step count is a host value, so a
-    step cannot be captured into a CUDA graph (RuntimeError). Anything refused is refused before a kernel is launched
+    step cannot be captured into a CUDA graph, nor recorded by a tracer (RuntimeError). Anything refused is refused before a kernel is launched
     and leaves parameters, state and step counts as they were. For autograd a step is a change in place.
     """
 

@@ -15,5 +15,8 @@ def embedding_lookup(table: torch.Tensor, indices: torch.Tensor, scale: float = 
     Differentiable in `table` (once, backward only). The gradient is dense, scale * the sum of the output gradients of
     each row's indices: summed in float32 in an order that depends only on the inputs (and the alignment of the
     gradient's address), so the same inputs give the same bits. Both directions may be captured into CUDA graphs (the
-    backward not while an eager graph of the table, made on the default stream, lives: RuntimeError)."""
+    backward not while an eager graph of the table, made on the default stream, lives: RuntimeError).
+
+    Tracers (torch.jit.trace, torch.fx, torch.export), fake tensors and function transforms are refused (RuntimeError): they
+    would not see what the kernels write. torch.compile leaves the call out of its graph."""
     return host().embedding_lookup(table, indices, scale, padding_index)

@@ -8,6 +8,7 @@
 #include <stdexcept>
 #include <string>
 #include <vector>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
@@ -17,6 +18,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
 #include "../../include/fgs_b200.h"
@@ -107,8 +109,28 @@ int type_code(const at::Tensor& t) {
     }
 }
 
+// The kernels work on memory, past torch's dispatcher: whatever records calls there would see an allocation and none of the
+// writes to it, and give uninitialised memory when it is run again.
+void refuse_recorded(const char* what) {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    using Key = c10::impl::TorchDispatchModeKey;
+    if (torch::jit::tracer::isTracing()) refuse(std::string(what) + " cannot be traced by torch.jit.trace");
+    if (!Modes::any_modes_set()) return;
+    for (const Key k : {Key::FAKE, Key::PROXY, Key::FUNCTIONAL})
+        if (Modes::get_mode(k).has_value()) refuse(std::string(what) + " cannot be traced by torch.fx or run on fake tensors");
+}
+
+// refuses tensors that do not own their value's memory: fake ones, wrappers of function transforms, other subclasses that
+// dispatch to Python
+void refuse_wrapped(const at::Tensor& t, const char* name) {
+    constexpr c10::DispatchKeySet wrappers({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                            c10::DispatchKey::Functionalize, c10::DispatchKey::ZeroTensor});
+    if (t.key_set().has_any(wrappers)) refuse(std::string(name) + " must be a plain tensor: fake tensors and tensors of function transforms have no memory");
+}
+
 // data address of a contiguous CUDA tensor of the given type and element count on `device` (-1: any, and sets it)
 void* address(const at::Tensor& t, const char* name, int code, int64_t count, int& device) {
+    refuse_wrapped(t, name);
     if (t.layout() != at::kStrided || type_code(t) != code || !t.is_contiguous())
         refuse(std::string(name) + " must be a contiguous " + kTypeNames[code] + " tensor");
     if (!t.is_cuda()) refuse(std::string(name) + " must be a CUDA tensor");
@@ -205,6 +227,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
     PyObject *all_state, *groups, *new_state, *limit;
     if (!PyArg_ParseTuple(args, "O!O!OO", &PyDict_Type, &all_state, &PyList_Type, &groups, &new_state, &limit)) return nullptr;
     return guarded([&]() -> PyObject* {
+        refuse_recorded("FusedAdamW.step");
         const double max_norm = limit == Py_None ? 0.0 : number(limit);
         if (limit != Py_None && !(max_norm > 0.0)) refuse("max_grad_norm must be positive (or None for no clipping)");
         Job jobs[3][2][2];
@@ -350,6 +373,7 @@ PyObject* read_moments(PyObject*, PyObject* args) {
     if (!PyArg_ParseTuple(args, "O!O!O!O!", &PyDict_Type, &all_state, &PyList_Type, &params, &PyList_Type, &outs[0], &PyList_Type, &outs[1]))
         return nullptr;
     return guarded([&]() -> PyObject* {
+        refuse_recorded("FusedAdamW.read_moments");
         const Py_ssize_t n = PyList_GET_SIZE(params);
         if (PyList_GET_SIZE(outs[0]) != n || PyList_GET_SIZE(outs[1]) != n) refuse("one tensor per parameter is needed");
         const at::NoGradGuard no_graph;
@@ -419,6 +443,7 @@ at::Tensor lookup(const at::Tensor& table, const at::Tensor& indices, double sca
         width *= table.size(d);
     }
     at::Tensor out = at::empty(shape, table.options().requires_grad(false));
+    refuse_wrapped(out, "the output");
     check(lib.lookup(table.data_ptr(), table.size(0), width, type_code(table), indices.data_ptr(), indices.numel(),
                      static_cast<int>(indices.element_size()), scale, padding, out.data_ptr(), c10::cuda::getCurrentCUDAStream().stream()));
     return out;
@@ -447,6 +472,7 @@ struct LookupBackward : torch::autograd::Node {
 
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         if (!grads[0].defined()) return {at::Tensor()};
+        refuse_recorded("the backward of embedding_lookup");
         refuse_uncapturable();
         const at::Tensor idx = indices.unpack();
         at::Tensor grad;
@@ -455,6 +481,8 @@ struct LookupBackward : torch::autograd::Node {
             const at::Tensor g = grads[0].to(type).contiguous();
             const c10::cuda::CUDAGuard guard(g.device());
             grad = at::empty(shape, g.options());
+            refuse_wrapped(g, "the gradient of a lookup");
+            refuse_wrapped(grad, "the table's gradient");
             int64_t width = 1;
             for (size_t d = 1; d < shape.size(); d++) width *= shape[d];
             size_t bytes = 0;
@@ -491,12 +519,15 @@ PyObject* embedding_lookup(PyObject*, PyObject* args) {
     double scale;
     if (!PyArg_ParseTuple(args, "OOdO", &table_o, &indices_o, &scale, &padding_o)) return nullptr;
     return guarded([&]() -> PyObject* {
+        refuse_recorded("embedding_lookup");
         const at::Tensor& table = tensor_of(table_o, "table");
+        refuse_wrapped(table, "table");
         const int code = type_code(table);
         if (table.layout() != at::kStrided || !table.is_cuda() || code < 0 || code > FGS_DTYPE_F16 || table.dim() < 1 || !table.is_contiguous())
             refuse("table must be a contiguous CUDA float32, bfloat16 or float16 tensor [rows, ...]");
         if (table._fw_grad(0).defined()) refuse("embedding_lookup has no forward-mode derivative");
         const at::Tensor& given = tensor_of(indices_o, "indices");
+        refuse_wrapped(given, "indices");
         if (given.layout() != at::kStrided || (given.scalar_type() != at::kLong && given.scalar_type() != at::kInt) || given.device() != table.device())
             refuse("indices must be an int64 or int32 tensor on the device of the table");
         int64_t padding = -1;

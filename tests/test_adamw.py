@@ -219,3 +219,42 @@ def test_small_values_are_kept():
     x[0], x[1] = 1.0, 0.0
     v = O.decode(*O.encode(x, 5, False), False)
     assert v[1] == 0.0 and (v[2:] == np.float32(1.25 * 2.0 ** -31)).all()
+
+
+@pytest.mark.parametrize('kind', ['jit.trace', 'real', 'fake', 'symbolic'])
+def test_tracers_refused(kind):
+    """A tracer would record none of the kernel's writes."""
+    import FasterGSVDACudaBackend as F
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    p = _param()
+    opt = F.FusedAdamW([p])
+
+    def step(x):
+        opt.step()
+        return x + p.detach()
+
+    def read(x):
+        opt.read_moments([torch.zeros(5)], [torch.zeros(5)])
+        return x + 1.0
+
+    for f in (step, read):
+        with pytest.raises(RuntimeError, match='cannot be traced'):
+            if kind == 'jit.trace':
+                torch.jit.trace(f, (torch.zeros(5),))
+            elif kind == 'fake':
+                with FakeTensorMode(allow_non_fake_inputs=True):
+                    f(torch.zeros(5))
+            else:
+                make_fx(f, tracing_mode=kind)(torch.zeros(5))
+    assert not opt.state
+
+
+def test_tensors_without_memory_refused():
+    import FasterGSVDACudaBackend as F
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode() as mode:
+        p = torch.nn.Parameter(mode.from_tensor(torch.ones(5)))
+        p.grad = mode.from_tensor(torch.ones(5))
+    with pytest.raises(RuntimeError, match='plain tensor'):
+        F.FusedAdamW([p]).step()

@@ -33,3 +33,37 @@ def test_workspace_size():
         check(lib.fgs_embedding_grad(64, 100, 8, 64, 0, 50, 8, 1.0, -1, 64, 64, need - 1, None))
     with pytest.raises(RuntimeError, match='indices'):
         size_out(lib.fgs_embedding_workspace_bytes, -1, 50, 8)
+
+
+def _trace(kind, f, *args):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    if kind == 'jit.trace':
+        return torch.jit.trace(f, args)
+    if kind == 'fake':
+        with FakeTensorMode(allow_non_fake_inputs=True):
+            return f(*args)
+    return make_fx(f, tracing_mode=kind)(*args)
+
+
+@pytest.mark.parametrize('kind', ['jit.trace', 'real', 'fake', 'symbolic'])
+def test_tracers_refused(kind):
+    """A tracer would record the allocation of the output and none of the kernel's writes to it."""
+    import FasterGSVDACudaBackend as F
+    table, idx = torch.zeros(4, 3), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match='cannot be traced'):
+        _trace(kind, lambda t, i: F.embedding_lookup(t, i) + 1.0, table, idx)
+
+
+def test_tensors_without_memory_refused():
+    """Fake tensors out of their mode, and tensors of function transforms."""
+    import FasterGSVDACudaBackend as F
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    table, idx = torch.zeros(4, 3), torch.zeros(2, dtype=torch.int64)
+    with FakeTensorMode() as mode:
+        fake = mode.from_tensor(table)
+    for call in (lambda: F.embedding_lookup(fake, idx), lambda: torch.func.grad(lambda t: F.embedding_lookup(t, idx).sum())(table),
+                 lambda: torch.func.vmap(lambda t: F.embedding_lookup(t, idx))(table[None]),
+                 lambda: torch.func.functionalize(lambda t: F.embedding_lookup(t, idx))(table)):
+        with pytest.raises(RuntimeError, match='plain tensor'):
+            call()

@@ -368,3 +368,24 @@ def test_forward_mode_is_refused(cuda):
         assert torch.equal(F.embedding_lookup(table, idx), table[idx])
     with pytest.raises(RuntimeError):  # tensors of a function transform have no memory of their own
         torch.func.vmap(lambda t: F.embedding_lookup(t, idx))(table[None].expand(2, 8, 4).contiguous())
+
+
+def test_tracers_are_refused(cuda):
+    """What a tracer would record, run on other inputs, would give the memory of an allocation: refused in both directions. A
+    mode that only watches is none of them."""
+    import FasterGSVDACudaBackend as F
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    table, idx, g = _inputs(cuda, 30, 16, 100, torch.float32, 'even', torch.int64)
+    for trace in (lambda f: torch.jit.trace(f, (table, idx)), lambda f: make_fx(f)(table, idx), lambda f: make_fx(f, tracing_mode='fake')(table, idx)):
+        with pytest.raises(RuntimeError, match='cannot be traced'):
+            trace(lambda t, i: F.embedding_lookup(t, i, scale=2.0) + 1.0)
+    table.requires_grad_(True)
+    out = F.embedding_lookup(table, idx)
+    with pytest.raises(RuntimeError, match='cannot be traced'):
+        make_fx(lambda x: torch.autograd.grad(out, table, x, retain_graph=True)[0] + 1.0)(g)
+    with FlopCounterMode(display=False):
+        out = F.embedding_lookup(table, idx, scale=0.5)
+        out.backward(g)
+    _check_rows(out, table, idx, 0.5)
+    _check_grad(table.grad, g, idx, 0.5)

@@ -131,6 +131,7 @@ void refuse_wrapped(const at::Tensor& t, const char* name) {
 // data address of a contiguous CUDA tensor of the given type and element count on `device` (-1: any, and sets it)
 void* address(const at::Tensor& t, const char* name, int code, int64_t count, int& device) {
     refuse_wrapped(t, name);
+    if (t.is_neg()) refuse(std::string(name) + " must not be a lazily negated view: its memory holds the negative");
     if (t.layout() != at::kStrided || type_code(t) != code || !t.is_contiguous())
         refuse(std::string(name) + " must be a contiguous " + kTypeNames[code] + " tensor");
     if (!t.is_cuda()) refuse(std::string(name) + " must be a CUDA tensor");
@@ -436,6 +437,7 @@ PyObject* read_moments(PyObject*, PyObject* args) {
 
 at::Tensor lookup(const at::Tensor& table, const at::Tensor& indices, double scale, int64_t padding) {
     const c10::cuda::CUDAGuard guard(table.device());
+    const at::Tensor values = table.is_neg() ? table.detach().resolve_neg() : table;
     std::vector<int64_t> shape = indices.sizes().vec();
     int64_t width = 1;
     for (int64_t d = 1; d < table.dim(); d++) {
@@ -444,7 +446,7 @@ at::Tensor lookup(const at::Tensor& table, const at::Tensor& indices, double sca
     }
     at::Tensor out = at::empty(shape, table.options().requires_grad(false));
     refuse_wrapped(out, "the output");
-    check(lib.lookup(table.data_ptr(), table.size(0), width, type_code(table), indices.data_ptr(), indices.numel(),
+    check(lib.lookup(values.data_ptr(), table.size(0), width, type_code(table), indices.data_ptr(), indices.numel(),
                      static_cast<int>(indices.element_size()), scale, padding, out.data_ptr(), c10::cuda::getCurrentCUDAStream().stream()));
     return out;
 }
@@ -478,7 +480,7 @@ struct LookupBackward : torch::autograd::Node {
         at::Tensor grad;
         {
             const at::AutoGradMode no_graph(false);
-            const at::Tensor g = grads[0].to(type).contiguous();
+            const at::Tensor g = grads[0].to(type).contiguous().resolve_neg();
             const c10::cuda::CUDAGuard guard(g.device());
             grad = at::empty(shape, g.options());
             refuse_wrapped(g, "the gradient of a lookup");
@@ -539,7 +541,7 @@ PyObject* embedding_lookup(PyObject*, PyObject* args) {
                 throw PythonError();
             }
         }
-        const at::Tensor indices = given.contiguous();
+        const at::Tensor indices = given.contiguous().resolve_neg();
         return THPVariable_Wrap(table.requires_grad() && at::GradMode::is_enabled() ? lookup_with_grad(table, indices, scale, padding)
                                                                                    : lookup(table, indices, scale, padding));
     });

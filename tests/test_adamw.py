@@ -258,3 +258,12 @@ def test_tensors_without_memory_refused():
         p.grad = mode.from_tensor(torch.ones(5))
     with pytest.raises(RuntimeError, match='plain tensor'):
         F.FusedAdamW([p]).step()
+
+
+def test_lazily_negated_tensors_refused():
+    """Their memory holds the negative of their values (the imaginary part of a conjugate, for one)."""
+    import FasterGSVDACudaBackend as F
+    p = torch.nn.Parameter(torch.complex(torch.ones(1), torch.ones(1)).conj().imag)
+    p.grad = torch.ones(1)
+    with pytest.raises(RuntimeError, match='parameter must not be a lazily negated view'):
+        F.FusedAdamW([p]).step()

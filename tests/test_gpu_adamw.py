@@ -496,3 +496,18 @@ def test_moments_into_shared_memory_are_refused(cuda, bits):
     assert (flat == 7).all()
     opt.read_moments([whole], [apart])
     assert (flat != 7).all()
+
+
+def test_lazily_negated_gradients_are_refused(cuda):
+    import FasterGSVDACudaBackend as F
+    p = torch.nn.Parameter(torch.ones(300, device=cuda))
+    p.grad = torch._neg_view(torch.ones(300, device=cuda))
+    opt = F.FusedAdamW([p])
+    with pytest.raises(RuntimeError, match='a gradient must not be a lazily negated view'):
+        opt.step()
+    assert (p == 1).all()
+    p.grad = p.grad.resolve_neg()
+    opt.step()
+    assert (p > 1 - 1e-2).all() and not (p == 1).any()
+    with pytest.raises(RuntimeError, match='an output must not be a lazily negated view'):
+        opt.read_moments([torch._neg_view(torch.empty(300, device=cuda))], [torch.empty(300, device=cuda)])

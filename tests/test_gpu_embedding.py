@@ -389,3 +389,15 @@ def test_tracers_are_refused(cuda):
         out.backward(g)
     _check_rows(out, table, idx, 0.5)
     _check_grad(table.grad, g, idx, 0.5)
+
+
+def test_lazily_negated_tensors(cuda):
+    """Tensors whose memory holds the negative of their values (torch's views of conjugates' imaginary parts)."""
+    import FasterGSVDACudaBackend as F
+    table, idx, g = _inputs(cuda, 30, 16, 100, torch.float32, 'even', torch.int64)
+    leaf = table.clone().requires_grad_(True)
+    out = F.embedding_lookup(torch._neg_view(leaf), torch._neg_view(idx), scale=2.0)
+    assert torch._neg_view(idx).is_neg() and torch._neg_view(leaf).is_neg()
+    _check_rows(out, -table, -idx, 2.0)
+    out.backward(torch._neg_view(g))
+    _check_grad(leaf.grad, g, -idx, 2.0)  # negated twice: by the view of the table and by that of the gradient

@@ -52,8 +52,9 @@ class FusedAdamW(torch.optim.Optimizer):
     def __getstate__(self) -> dict:
         return {**super().__getstate__(), 'max_grad_norm': self.max_grad_norm}
 
-    def add_param_group(self, param_group: dict) -> None:
-        options = {**self.defaults, **param_group}
+    @staticmethod
+    def _check_options(options: dict) -> None:
+        """Raises ValueError for options of a group that a step cannot follow, those of other AdamWs among them."""
         lrs = options['lr'] if isinstance(options['lr'], (list, tuple)) else [options['lr']]
         if not 1 <= len(lrs) <= 7:
             raise ValueError('between 1 and 7 learning rates are supported')
@@ -67,6 +68,14 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError('eps must be zero or a normal float32 (at least 1.2e-38)')
         if options['state_bits'] not in (8, 32):
             raise ValueError('state_bits must be 8 or 32')
+        for name in ('maximize', 'amsgrad', 'differentiable'):
+            if options.get(name, False):
+                raise ValueError(f'{name} is not supported')
+        if not options.get('decoupled_weight_decay', True) and float(options['weight_decay']) != 0.0:
+            raise ValueError('weight decay is always decoupled: that of Adam (decoupled_weight_decay=False) is not supported')
+
+    def add_param_group(self, param_group: dict) -> None:
+        self._check_options({**self.defaults, **param_group})
         super().add_param_group(param_group)
 
     @staticmethod
@@ -108,7 +117,10 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict: dict) -> None:
         """As torch's, but the state keeps its own types (torch's casts it to the parameters' type). Groups saved by another
-        AdamW take this one's options where they lack them (its moments are float32: state_bits=32)."""
+        AdamW take this one's options where they lack them (its moments are float32: state_bits=32); what this one cannot
+        follow (maximize, amsgrad, differentiable, weight decay that is not decoupled) is refused, and nothing is changed."""
+        for group in state_dict['param_groups']:
+            self._check_options({**self.defaults, **group})
         saved = state_dict['state']
         super().load_state_dict({**state_dict, 'state': {}})
         for group in self.param_groups:

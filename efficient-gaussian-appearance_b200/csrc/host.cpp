@@ -155,7 +155,7 @@ void changed(const at::Tensor& t) {
 // names of the state and of the group options, made once
 struct Names {
     PyObject *params, *lr, *betas, *eps, *weight_decay, *state_bits, *master_weights, *step, *exp_avg, *exp_avg_sq, *exp_avg_exponent,
-        *exp_avg_sq_exponent, *master;
+        *exp_avg_sq_exponent, *master, *maximize, *amsgrad, *differentiable, *decoupled_weight_decay;
 } names;
 
 const at::Tensor& state_tensor(PyObject* state, PyObject* key) {
@@ -175,6 +175,22 @@ PyObject* option(PyObject* group, PyObject* key) {
     PyObject* o = PyDict_GetItemWithError(group, key);
     if (!o) refuse(std::string("a parameter group has no ") + PyUnicode_AsUTF8(key));
     return o;
+}
+
+// truth of a group's option, `otherwise` where it has none
+bool is_set(PyObject* group, PyObject* key, bool otherwise) {
+    PyObject* o = PyDict_GetItemWithError(group, key);
+    const int set = o ? PyObject_IsTrue(o) : otherwise;
+    if (set < 0 || (!o && PyErr_Occurred())) throw PythonError();
+    return set;
+}
+
+// options of torch's Adams that a step cannot follow (adamw.py refuses them where groups are made and loaded)
+void refuse_options(PyObject* group) {
+    for (PyObject* name : {names.maximize, names.amsgrad, names.differentiable})
+        if (is_set(group, name, false)) refuse(std::string(PyUnicode_AsUTF8(name)) + " is not supported");
+    if (!is_set(group, names.decoupled_weight_decay, true) && number(option(group, names.weight_decay)) != 0.0)
+        refuse("weight decay is always decoupled: that of Adam (decoupled_weight_decay=False) is not supported");
 }
 
 fgs_adamw_hyper hyper_of(PyObject* group, int64_t step) {
@@ -251,6 +267,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                 PyErr_Clear();
                 refuse("state_bits must be 8 or 32");
             }
+            refuse_options(group);
             const int wants_master = PyObject_IsTrue(option(group, names.master_weights));
             for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); i++) {
                 PyObject* o = PyList_GET_ITEM(params, i);
@@ -570,6 +587,7 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fgs_host", "host side of the man
 PyMODINIT_FUNC PyInit__fgs_host() {
     const auto name = [](const char* s) { return PyUnicode_InternFromString(s); };
     names = {name("params"),  name("lr"),         name("betas"),            name("eps"),                 name("weight_decay"), name("state_bits"), name("master_weights"),
-             name("step"),    name("exp_avg"),    name("exp_avg_sq"),       name("exp_avg_exponent"),    name("exp_avg_sq_exponent"), name("master")};
+             name("step"),    name("exp_avg"),    name("exp_avg_sq"),       name("exp_avg_exponent"),    name("exp_avg_sq_exponent"), name("master"),
+             name("maximize"), name("amsgrad"), name("differentiable"), name("decoupled_weight_decay")};
     return PyModule_Create(&kModule);
 }

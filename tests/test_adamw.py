@@ -267,3 +267,48 @@ def test_lazily_negated_tensors_refused():
     p.grad = torch.ones(1)
     with pytest.raises(RuntimeError, match='parameter must not be a lazily negated view'):
         F.FusedAdamW([p]).step()
+
+
+@pytest.mark.parametrize('options,match', [({'maximize': True}, 'maximize'), ({'amsgrad': True}, 'amsgrad'), ({'differentiable': True}, 'differentiable'),
+                                           ({'decoupled_weight_decay': False, 'weight_decay': 0.1}, 'decoupled')])
+def test_options_of_other_optimizers_refused(options, match):
+    """A step that went on without them would turn around, or decay otherwise."""
+    import FasterGSVDACudaBackend as F
+    with pytest.raises(ValueError, match=match):
+        F.FusedAdamW([{'params': [_param()], **options}])
+    p = _param()
+    opt = F.FusedAdamW([p], lr=0.5)
+    opt.state[p] = {**opt._new_state(p, 32, False), 'step': 7}
+    state = copy.deepcopy(opt.state_dict())
+    state['param_groups'][0].update({'lr': 0.25, **options})
+    with pytest.raises(ValueError, match=match):
+        opt.load_state_dict(state)
+    assert opt.param_groups[0]['lr'] == 0.5 and opt.state[p]['step'] == 7
+    plain = {k: (False if v is True else v) for k, v in options.items()}
+    if match == 'decoupled':
+        plain['weight_decay'] = 0.0  # without a decay there is no difference
+    state['param_groups'][0].update(plain)
+    opt.load_state_dict(state)
+    assert opt.param_groups[0]['lr'] == 0.25
+
+
+@pytest.mark.parametrize('options', [{'maximize': True}, {'amsgrad': True}, {'decoupled_weight_decay': False, 'weight_decay': 0.1}])
+def test_checkpoints_that_cannot_be_followed_are_refused(options):
+    import FasterGSVDACudaBackend as F
+    p = _param(6)
+    make = torch.optim.Adam if 'decoupled_weight_decay' in options else torch.optim.AdamW
+    ref = make([p], **{k: v for k, v in options.items() if k != 'decoupled_weight_decay'})
+    ref.step()
+    with pytest.raises(ValueError):
+        F.FusedAdamW([p]).load_state_dict(ref.state_dict())
+
+
+@pytest.mark.parametrize('options,match', [({'maximize': True}, 'maximize'), ({'amsgrad': 1}, 'amsgrad'), ({'differentiable': True}, 'differentiable'),
+                                           ({'decoupled_weight_decay': False, 'weight_decay': 0.1}, 'decoupled')])
+def test_options_set_on_a_group_are_refused_by_the_step(options, match):
+    import FasterGSVDACudaBackend as F
+    opt = F.FusedAdamW([_param()])
+    opt.param_groups[0].update(options)
+    with pytest.raises(RuntimeError, match=match):
+        opt.step()
+    assert not opt.state

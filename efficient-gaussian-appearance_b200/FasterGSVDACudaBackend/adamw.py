@@ -4,6 +4,7 @@ FusedAdamW updates every parameter of every group in one kernel launch per 384 t
 bfloat16 or float16 parameters, moments in float32 or in 8 bits, an optional float32 copy of half-precision parameters,
 and clipping by the global gradient norm without a host round trip.
 """
+import copy
 import sys
 
 import torch
@@ -118,17 +119,42 @@ class FusedAdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """As torch's, but the state keeps its own types (torch's casts it to the parameters' type). Groups saved by another
         AdamW take this one's options where they lack them (its moments are float32: state_bits=32); what this one cannot
-        follow (maximize, amsgrad, differentiable, weight decay that is not decoupled) is refused, and nothing is changed."""
-        for group in state_dict['param_groups']:
-            self._check_options({**self.defaults, **group})
-        saved = state_dict['state']
-        super().load_state_dict({**state_dict, 'state': {}})
-        for group in self.param_groups:
-            for name, value in self.defaults.items():
-                group.setdefault(name, value)
-        self.state.clear()
-        for group, mine in zip(state_dict['param_groups'], self.param_groups):
-            for key, p in zip(group['params'], mine['params']):
-                if key in saved:
-                    self.state[p] = {sys.intern(k): v.detach().to(p.device, copy=True).contiguous() if torch.is_tensor(v) and k != 'step' else int(v)
-                                     for k, v in saved[key].items()}
+        follow (maximize, amsgrad, differentiable, weight decay that is not decoupled) is refused, and nothing is changed. Hooks
+        around the loading see the whole state."""
+        loaded = {}
+
+        def take(_, state_dict: dict) -> dict:  # behind all other pre-hooks; torch's loading sees no state of a parameter
+            for group in state_dict['param_groups']:
+                self._check_options({**self.defaults, **group})
+            rest = dict(state_dict['state'])
+            for group, mine in zip(state_dict['param_groups'], self.param_groups):
+                for key, p in zip(group['params'], mine['params']):
+                    if key in rest:
+                        loaded[p] = self._loaded_state(p, rest.pop(key))
+            return {**state_dict, 'state': rest}
+
+        def put(_) -> None:  # before all other post-hooks
+            for group in self.param_groups:
+                for name, value in self.defaults.items():
+                    group.setdefault(name, value)
+            self.state.update(loaded)
+
+        hooks = [self.register_load_state_dict_pre_hook(take), self.register_load_state_dict_post_hook(put, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    @staticmethod
+    def _loaded_state(p: torch.Tensor, saved: dict) -> dict:
+        state = {}
+        for name, value in saved.items():
+            if name == 'step':
+                value = int(value)
+            elif torch.is_tensor(value):
+                value = value.detach().to(p.device, copy=True).contiguous()
+            else:
+                value = copy.deepcopy(value)
+            state[sys.intern(name)] = value
+        return state

@@ -312,3 +312,83 @@ def test_options_set_on_a_group_are_refused_by_the_step(options, match):
     with pytest.raises(RuntimeError, match=match):
         opt.step()
     assert not opt.state
+
+
+def _stepped(n=300, step=7):
+    import FasterGSVDACudaBackend as F
+    p = _param(n, torch.bfloat16)
+    opt = F.FusedAdamW([p], state_bits=8, master_weights=True)
+    opt.state[p] = {**opt._new_state(p, 8, True), 'step': step}
+    opt.state[p]['exp_avg'].random_(0, 256)
+    opt.state[p]['master'] += 1e-4  # no bfloat16
+    return p, opt
+
+
+def test_hooks_around_loading():
+    """Pre-hooks see the saved state and may change it, post-hooks see the loaded one; both before and after the call of
+    this class's own."""
+    _, saved = _stepped()
+    p, opt = _stepped(step=3)
+    seen = []
+
+    def before(o, state_dict):
+        assert o is opt
+        seen.append((opt.state[p]['step'], state_dict['state'][0]['step']))
+        state = {k: {**v, 'step': 99} for k, v in state_dict['state'].items()}
+        return {**state_dict, 'state': state}
+
+    def after(o):
+        seen.append((opt.state[p]['step'], opt.state[p]['exp_avg'].dtype, dict(opt.param_groups[0])['state_bits']))
+
+    opt.register_load_state_dict_pre_hook(before)
+    opt.register_load_state_dict_post_hook(after, prepend=True)
+    source = saved.state_dict()
+    kept = copy.deepcopy(source)
+    opt.load_state_dict(source)
+    assert seen == [(3, 7), (99, torch.uint8, 8)] and opt.state[p]['step'] == 99
+    for name in ('exp_avg', 'master'):
+        assert torch.equal(opt.state[p][name], kept['state'][0][name]) and opt.state[p][name].dtype == kept['state'][0][name].dtype
+    assert source['state'][0]['step'] == 7  # the caller's dict is as it was
+    opt.load_state_dict(source)
+    assert len(seen) == 4
+
+
+def test_post_hooks_see_the_options_of_this_class():
+    import FasterGSVDACudaBackend as F
+    p = _param(6)
+    ref = torch.optim.AdamW([p])
+    ref.step()
+    opt = F.FusedAdamW([p])
+    seen = []
+    opt.register_load_state_dict_post_hook(lambda o: seen.append((o.param_groups[0]['state_bits'], o.state[p]['step'])))
+    opt.load_state_dict(ref.state_dict())
+    assert seen == [(32, 1)]
+
+
+@pytest.mark.parametrize('spoil', [lambda s: s['state'][0].update(step=None), lambda s: s['state'][0].update(step='x'),
+                                   lambda s: s['param_groups'].append(copy.deepcopy(s['param_groups'][0])),
+                                   lambda s: s['param_groups'][0]['params'].append(1), lambda s: s.pop('state')])
+def test_a_checkpoint_that_does_not_load_changes_nothing(spoil):
+    p, opt = _stepped(step=3)
+    opt.param_groups[0]['lr'] = 0.5
+    before = copy.deepcopy(opt.state[p])
+    _, saved = _stepped()
+    bad = copy.deepcopy(saved.state_dict())
+    spoil(bad)
+    with pytest.raises((TypeError, ValueError, KeyError)):
+        opt.load_state_dict(bad)
+    assert opt.param_groups[0]['lr'] == 0.5 and list(opt.state) == [p] and opt.state[p].keys() == before.keys()
+    assert all(torch.equal(opt.state[p][k], v) if torch.is_tensor(v) else opt.state[p][k] == v for k, v in before.items())
+    opt.load_state_dict(saved.state_dict())  # and no hook is left behind
+    assert opt.state[p]['step'] == 7 and opt.param_groups[0]['lr'] == 1e-3
+
+
+def test_state_beside_the_moments_is_kept():
+    """Entries of a user's own, of a parameter and of none, come back as they were."""
+    p, saved = _stepped()
+    saved.state[p]['note'] = {'a': [1, 2]}
+    state = copy.deepcopy(saved.state_dict())
+    state['state']['epoch'] = {'n': 5}
+    q, opt = _stepped(step=3)
+    opt.load_state_dict(state)
+    assert opt.state[q]['note'] == {'a': [1, 2]} and opt.state['epoch'] == {'n': 5} and opt.state[q]['step'] == 7

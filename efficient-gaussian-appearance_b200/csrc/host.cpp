@@ -210,6 +210,9 @@ fgs_adamw_hyper hyper_of(PyObject* group, int64_t step) {
     h.beta2 = number(b2.p);
     h.eps = number(option(group, names.eps));
     h.weight_decay = number(option(group, names.weight_decay));
+    // as fgs_adamw_step, which would come to it behind the launches of the norm and of other types
+    if (!(h.beta1 >= 0.0 && h.beta1 < 1.0 && h.beta2 >= 0.0 && h.beta2 < 1.0)) refuse("betas must be in [0, 1)");
+    if (!(h.eps >= 0.0) || (h.eps > 0.0 && h.eps < 1.2e-38)) refuse("eps must be zero or a normal float (at least 1.2e-38)");
     h.step = step;
     return h;
 }
@@ -223,6 +226,29 @@ struct Job {
     std::vector<int64_t> count;
     std::vector<int32_t> hyper;
 };
+
+// a parameter without state, which is made once nothing can be refused any more
+struct Fresh {
+    Job* job;
+    size_t at;
+    PyObject* param;  // borrowed
+    int bits;
+    bool master;
+};
+
+// places the addresses of a parameter's state as tensor `at` of a job
+void place_state(Job& job, size_t at, PyObject* state, int bits, bool master, int& device) {
+    const int64_t n = job.count[at], blocks = (n + kBlock - 1) / kBlock;
+    const int kind = bits == 8 ? kU8 : FGS_DTYPE_F32;
+    job.exp_avg[at] = address(state_tensor(state, names.exp_avg), "exp_avg", kind, n, device);
+    job.exp_avg_sq[at] = address(state_tensor(state, names.exp_avg_sq), "exp_avg_sq", kind, n, device);
+    if (bits == 8) {
+        job.exp_avg_exponent[at] = static_cast<uint8_t*>(address(state_tensor(state, names.exp_avg_exponent), "exp_avg_exponent", kU8, blocks, device));
+        job.exp_avg_sq_exponent[at] =
+            static_cast<uint8_t*>(address(state_tensor(state, names.exp_avg_sq_exponent), "exp_avg_sq_exponent", kU8, blocks, device));
+    }
+    if (master) job.master[at] = static_cast<float*>(address(state_tensor(state, names.master), "master", FGS_DTYPE_F32, n, device));
+}
 
 // Address ranges that a kernel writes by different threads: refused if two overlap. 300 of them are sorted in some 5 us, of
 // a step whose kernels take 100 and more.
@@ -254,7 +280,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
         std::vector<std::pair<PyObject*, int64_t>> counted;  // states and their new step counts (borrowed)
         std::vector<PyObject*> updated;                      // borrowed
         Written params_written;
-        Ref fresh(must(PyList_New(0)));                      // parameter, state, parameter, state ...
+        std::vector<Fresh> fresh;
         int device = -1;
         bool any = false;
         for (Py_ssize_t gi = 0; gi < PyList_GET_SIZE(groups); gi++) {
@@ -282,33 +308,32 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                 const int64_t n = p.numel();
                 job.param.push_back(address(p, "a parameter", code, n, device));
                 job.grad.push_back(address(g, "a gradient", code, n, device));
-                PyObject* state = states.find(o);
-                if (!state || (PyDict_Check(state) && PyDict_GET_SIZE(state) == 0)) {
-                    Ref made(must(PyObject_CallFunction(new_state, "Oii", o, static_cast<int>(bits), static_cast<int>(master))));
-                    if (PyList_Append(fresh.p, o) || PyList_Append(fresh.p, made.p)) throw PythonError();
-                    state = made.p;  // the list keeps it
-                }
-                if (!PyDict_Check(state)) refuse("the optimizer state of a parameter must be a dict");
-                PyObject* was = PyDict_GetItemWithError(state, names.step);
-                if (!was) refuse("the optimizer state has no step");
-                Ref whole(must(PyNumber_Long(was)));
-                const int64_t t = PyLong_AsLongLong(whole.p) + 1;
-                if (t < 1) {
-                    PyErr_Clear();
-                    refuse("step must not be negative");
-                }
-                const int kind = eight ? kU8 : FGS_DTYPE_F32;
-                job.exp_avg.push_back(address(state_tensor(state, names.exp_avg), "exp_avg", kind, n, device));
-                job.exp_avg_sq.push_back(address(state_tensor(state, names.exp_avg_sq), "exp_avg_sq", kind, n, device));
-                if (eight) {
-                    const int64_t blocks = (n + kBlock - 1) / kBlock;
-                    job.exp_avg_exponent.push_back(
-                        static_cast<uint8_t*>(address(state_tensor(state, names.exp_avg_exponent), "exp_avg_exponent", kU8, blocks, device)));
-                    job.exp_avg_sq_exponent.push_back(
-                        static_cast<uint8_t*>(address(state_tensor(state, names.exp_avg_sq_exponent), "exp_avg_sq_exponent", kU8, blocks, device)));
-                }
-                if (master) job.master.push_back(static_cast<float*>(address(state_tensor(state, names.master), "master", FGS_DTYPE_F32, n, device)));
                 job.count.push_back(n);
+                const size_t at = job.count.size() - 1;
+                job.exp_avg.push_back(nullptr);
+                job.exp_avg_sq.push_back(nullptr);
+                if (eight) {
+                    job.exp_avg_exponent.push_back(nullptr);
+                    job.exp_avg_sq_exponent.push_back(nullptr);
+                }
+                if (master) job.master.push_back(nullptr);
+                PyObject* state = states.find(o);
+                int64_t t = 1;
+                if (!state || (PyDict_Check(state) && PyDict_GET_SIZE(state) == 0)) {
+                    fresh.push_back({&job, at, o, static_cast<int>(bits), master});
+                } else {
+                    if (!PyDict_Check(state)) refuse("the optimizer state of a parameter must be a dict");
+                    PyObject* was = PyDict_GetItemWithError(state, names.step);
+                    if (!was) refuse("the optimizer state has no step");
+                    Ref whole(must(PyNumber_Long(was)));
+                    t = PyLong_AsLongLong(whole.p) + 1;
+                    if (t < 1) {
+                        PyErr_Clear();
+                        refuse("step must not be negative");
+                    }
+                    place_state(job, at, state, static_cast<int>(bits), master, device);
+                    counted.emplace_back(state, t);
+                }
                 updated.push_back(o);
                 params_written.add(job.param.back(), n, code);
                 size_t h = hypers.size();
@@ -319,7 +344,6 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                     h = hypers.size();
                 }
                 job.hyper.push_back(static_cast<int32_t>(h - 1));
-                counted.emplace_back(state, t);
             }
         }
         if (!any) Py_RETURN_NONE;
@@ -327,6 +351,14 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
         const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
         if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
             refuse("FusedAdamW.step cannot be captured into a CUDA graph: its step count is a host value");
+        Ref made(must(PyList_New(0)));  // the states of `fresh`
+        for (const Fresh& f : fresh) {
+            Ref state(must(PyObject_CallFunction(new_state, "Oii", f.param, f.bits, static_cast<int>(f.master))));
+            if (PyList_Append(made.p, state.p)) throw PythonError();  // the list keeps it
+            if (!PyDict_Check(state.p)) refuse("the optimizer state of a parameter must be a dict");
+            place_state(*f.job, f.at, state.p, f.bits, f.master, device);
+            counted.emplace_back(state.p, 1);
+        }
         const cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
         at::Tensor norm, partials;
         int n_partials = 0;
@@ -368,8 +400,8 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                                          n_partials ? norm.data_ptr<float>() : nullptr, stream));
                 }
         for (PyObject* o : updated) changed(THPVariable_Unpack(o));
-        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(fresh.p); i += 2)
-            if (PyDict_SetItem(all_state, PyList_GET_ITEM(fresh.p, i), PyList_GET_ITEM(fresh.p, i + 1))) throw PythonError();
+        for (size_t i = 0; i < fresh.size(); i++)
+            if (PyDict_SetItem(all_state, fresh[i].param, PyList_GET_ITEM(made.p, static_cast<Py_ssize_t>(i)))) throw PythonError();
         Ref count;  // most parameters have the same step count
         int64_t counts = -1;
         for (const auto& c : counted) {

@@ -511,3 +511,46 @@ def test_lazily_negated_gradients_are_refused(cuda):
     assert (p > 1 - 1e-2).all() and not (p == 1).any()
     with pytest.raises(RuntimeError, match='an output must not be a lazily negated view'):
         opt.read_moments([torch._neg_view(torch.empty(300, device=cuda))], [torch.empty(300, device=cuda)])
+
+
+def test_a_refused_first_step_makes_no_state(cuda, monkeypatch):
+    """Refusals come before the state of new parameters is made and filled: on the device, or into a graph under capture."""
+    import FasterGSVDACudaBackend as F
+    made = []
+    new_state = F.FusedAdamW._new_state
+    monkeypatch.setattr(F.FusedAdamW, '_new_state', staticmethod(lambda *a: made.append(1) or new_state(*a)))
+    p, q = _params([(40, 6), (8, 4)], torch.bfloat16, cuda)
+    flat = torch.ones(600, device=cuda)
+    a, b = torch.nn.Parameter(flat[:400]), torch.nn.Parameter(flat[200:])
+    good = [torch.ones_like(x) for x in (p, q, a, b)]
+
+    def refused(params, match, grads=good, **options):
+        for x, g in zip((p, q, a, b), grads):
+            x.grad = g
+        opt = F.FusedAdamW(params, state_bits=8, master_weights=True)
+        opt.param_groups[-1].update(options)
+        opt.max_grad_norm = 1.0
+        with pytest.raises((RuntimeError, TypeError), match=match):
+            opt.step()
+        assert not opt.state and not made
+        return opt
+
+    refused([p, q], 'contiguous', [good[0], torch.ones(4, 8, dtype=torch.bfloat16, device=cuda).t()] + good[2:])
+    refused([p, a, b], 'share memory')
+    refused([{'params': [p]}, {'params': [q]}], 'betas', betas=(0.9, 1.0))
+    refused([{'params': [p]}, {'params': [q]}], 'betas', betas=(float('nan'), 0.9))
+    refused([{'params': [p]}, {'params': [q]}], 'eps', eps=-1.0)
+    refused([{'params': [p]}, {'params': [q]}], 'eps', eps=1e-40)
+    refused([{'params': [p]}, {'params': [q]}], 'learning rates', lr=[])
+    refused([{'params': [p]}, {'params': [q]}], 'real number', lr='x')
+    opt = F.FusedAdamW([p, q], state_bits=8)
+    graph = torch.cuda.CUDAGraph()
+    x = torch.ones(3, device=cuda)
+    with pytest.raises(RuntimeError, match='captured'):
+        with torch.cuda.graph(graph):
+            x += 1
+            opt.step()
+    torch.cuda.synchronize()
+    assert not opt.state and not made
+    opt.step()
+    assert len(made) == 2 and opt.state[p]['step'] == opt.state[q]['step'] == 1

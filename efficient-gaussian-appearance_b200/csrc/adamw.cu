@@ -496,8 +496,7 @@ __device__ inline float clip_factor(double norm, double max_norm) {
 }
 
 // the norm and the clip factor from the partial sums, for steps of so many CTAs that not each should add them up
-__global__ void __launch_bounds__(kThreads) clip_kernel(const double* __restrict__ partials, int n_partials, double max_norm, float* __restrict__ factor,
-                                                        float* __restrict__ norm_out) {
+__global__ void __launch_bounds__(kThreads) clip_kernel(const double* partials, int n_partials, double max_norm, float* factor, float* norm_out) {
     __shared__ double scratch[kWarps];
     allow_dependent();
     wait_dependency();

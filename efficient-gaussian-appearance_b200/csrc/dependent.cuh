@@ -10,6 +10,9 @@ namespace fgs {
 __device__ inline void allow_dependent() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ inline void wait_dependency() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// What a dependent kernel reads of its predecessor's writes is not const and __restrict__: that promises that nobody writes it
+// while the kernel runs, and the read could be moved in front of the wait.
+
 // Launches a kernel as the programmatic dependent of the one before it in the stream: it may start before that one has
 // ended, and has to call wait_dependency() before it touches what that one, or any kernel before it, reads or writes.
 template <typename... Params, typename... Args>

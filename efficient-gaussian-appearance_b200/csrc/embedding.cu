@@ -531,7 +531,7 @@ __device__ inline void clear_rows(P* grad, const SumArgs& a, uint32_t cta, uint8
 // Within a group a row's sum stays in registers; rows that cross chunk borders are put together in shared memory, by
 // doubling along the groups that lie whole within the row.
 template <typename P, int N>
-__global__ void __launch_bounds__(kThreads, N * sizeof(P) == 4 ? 6 : 4) sum_kernel(const P* __restrict__ g, P* __restrict__ grad, const SumArgs a) {
+__global__ void __launch_bounds__(kThreads, N * sizeof(P) == 4 ? 6 : 4) sum_kernel(const P* g, P* grad, const SumArgs a) {
     using A = typename Pack<P, N>::A;
     extern __shared__ uint32_t staged[];  // the span's keys with one more on either side, and its tokens
     __shared__ float part[kThreads * N];
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, N * sizeof(P) == 4 ? 6 : 4) sum_kern
 // memory). A CTA looks at one span for a row that begins in it and
 // goes on; slots of `lanes` lanes take the row's spans in turn, and the slots' sums are added pairwise.
 template <typename P, int N>
-__global__ void __launch_bounds__(kThreads) join_kernel(P* __restrict__ grad, const SumArgs a) {
+__global__ void __launch_bounds__(kThreads) join_kernel(P* grad, const SumArgs a) {
     __shared__ float part[kThreads * N];
     wait_dependency();
     const uint32_t span = blockIdx.x;

@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kSortThreads) radix_upsweep(const S src, uint3
 }
 
 // row d of hist: exclusive offsets over the tiles; totals[d] = the row sum
-__global__ void __launch_bounds__(kSortThreads) radix_row_scan(uint32_t* __restrict__ hist, uint32_t n_tiles, uint32_t* __restrict__ totals) {
+__global__ void __launch_bounds__(kSortThreads) radix_row_scan(uint32_t* hist, uint32_t n_tiles, uint32_t* totals) {
     __shared__ uint32_t warp_tot[kSortWarps];
     allow_dependent();
     wait_dependency();
@@ -136,7 +136,7 @@ __device__ inline uint32_t digit_peers(uint32_t d, int bits, bool valid) {
 template <typename S, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads, 3) radix_downsweep(const S src, typename S::Key* __restrict__ kout, uint32_t* __restrict__ vout,
                                                                 uint32_t n, int shift, int bits, uint32_t mask,
-                                                                const uint32_t* __restrict__ hist, const uint32_t* __restrict__ totals,
+                                                                const uint32_t* hist, const uint32_t* totals,
                                                                 uint32_t n_tiles) {
     using K = typename S::Key;
     constexpr int kTile = kSortThreads * ITEMS;

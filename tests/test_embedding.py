@@ -67,3 +67,21 @@ def test_tensors_without_memory_refused():
                  lambda: torch.func.functionalize(lambda t: F.embedding_lookup(t, idx))(table)):
         with pytest.raises(RuntimeError, match='plain tensor'):
             call()
+
+
+def test_dependent_kernels_promise_nothing_about_what_they_read():
+    """A kernel that may start before its predecessor has ended must not declare what it reads const and __restrict__: that
+    lets the compiler move the read in front of the wait."""
+    import re
+    from pathlib import Path
+    csrc = Path(__file__).resolve().parent.parent / 'efficient-gaussian-appearance_b200' / 'csrc'
+    dependent = {}
+    for source in csrc.glob('*.cu'):
+        for kernel in source.read_text().split('__global__')[1:]:
+            head, _, body = kernel.partition(') {')
+            body = body.split('\n}\n')[0]
+            if 'wait_dependency()' in body:
+                name = re.search(r'(\w+_kernel|radix_\w+)\(', head).group(1)
+                dependent[name] = re.findall(r'const [\w: <>]+\*\s*__restrict__\s+(\w+)', head)
+    assert {'radix_downsweep', 'radix_row_scan', 'clip_kernel', 'sum_kernel', 'join_kernel', 'clear_kernel', 'adamw_kernel'} <= set(dependent)
+    assert not any(dependent.values()), dependent

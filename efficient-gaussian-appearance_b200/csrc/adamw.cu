@@ -14,10 +14,11 @@
 // octaves), the second eight bits (top = 255: 32 octaves, so that their ratio m / sqrt(v) has the same range). Float
 // bits order like the values, so coding is integer arithmetic on them: no division, no table.
 // Rounding: b2 = 0.999 changes v by far less than half a code step, so rounding to nearest would leave v where it is
-// (simulated: -74 % after 1000 steps). A threshold u is added under the third mantissa bit instead, from the additive
+// (tests/test_adamw.py simulates it: mean of v -71 % after 1000 steps of noisy gradients, updates off by 87 % rms). A threshold u is added under the third mantissa bit instead, from the additive
 // recurrence u = frac(i a + t b) of the element index i and the step t (a from the golden ratio; b = 1/r or 1/r^2 with
 // r the plastic number, r^3 = r + 1): over the steps an element's thresholds are evenly spread, so its rounding errors
-// cancel instead of adding up (simulated bias of v -0.4 %, update off by 11 % rms; independent random thresholds 24 %).
+// cancel instead of adding up (same simulation: -0.7 %, updates 11 %; independent random thresholds 0.2 %, 13 %). 1500 steps
+// behind a drop of the gradients to a tenth, v lags by 10 % and the updates are off by 14 % (random ones 0.2 %, 24 %).
 // Deterministic in (i, t). Values under the smallest code: m becomes that code or zero by its own threshold (unbiased);
 // a nonzero v becomes the smallest code, never zero, since it divides. A block with an infinity or NaN has E = 255 and
 // decodes to NaN throughout.

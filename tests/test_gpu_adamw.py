@@ -554,3 +554,27 @@ def test_a_refused_first_step_makes_no_state(cuda, monkeypatch):
     assert not opt.state and not made
     opt.step()
     assert len(made) == 2 and opt.state[p]['step'] == opt.state[q]['step'] == 1
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('limit', [0.7, 1e9], ids=['clipped', 'below the limit'])
+@pytest.mark.parametrize('shapes,dtypes', [
+    ([(10_500_000 + 77,)], (torch.float32,)),                                        # one launch of many CTAs: the factor is made once
+    ([(26_000 + i % 5,) for i in range(770)], (torch.float32,)),                     # two such launches and a short one behind them
+    ([(10_100_000,), (9_900_000 + 3,), (300,), (7, 5)], (torch.bfloat16, torch.float32)),  # two types, one norm
+    ([(1 + (977 * i) % 5000,) for i in range(60)], (torch.float32, torch.float16)),  # tables of the middle size
+], ids=['long', 'many', 'two types', '60 tensors'])
+def test_long_clipped_steps(cuda, shapes, dtypes, limit, bits):
+    import FasterGSVDACudaBackend as F
+    params = []
+    for i, s in enumerate(shapes):
+        p = torch.nn.Parameter(torch.randn(s, device=cuda, generator=torch.Generator(cuda).manual_seed(i)).to(dtypes[i % len(dtypes)]))
+        p.grad = (torch.randn(s, device=cuda, generator=torch.Generator(cuda).manual_seed(10_000 + i)) * 10.0 ** (i % 3 - 1)).to(p.dtype)
+        params.append(p)
+    opt = F.FusedAdamW(params, state_bits=bits, master_weights=True, max_grad_norm=limit)
+    norm = np.sqrt(sum((_np(p.grad).astype(np.float64) ** 2).sum() for p in params))
+    for _ in range(2):
+        before = _snapshot(opt)
+        opt.step()
+        assert abs(float(opt.grad_norm) - norm) <= 18 * 2.0 ** -24 * norm
+        _check(opt, before, min(1.0, limit / (norm + 1e-6)), True)

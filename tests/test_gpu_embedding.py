@@ -401,3 +401,19 @@ def test_lazily_negated_tensors(cuda):
     _check_rows(out, -table, -idx, 2.0)
     out.backward(torch._neg_view(g))
     _check_grad(leaf.grad, g, -idx, 2.0)  # negated twice: by the view of the table and by that of the gradient
+
+
+@pytest.mark.parametrize('index_type', [torch.int64, torch.int32], ids=['int64', 'int32'])
+@pytest.mark.parametrize('rows,width', [(200, 4), (4096, 3), (70_001, 1), (300_000, 2)], ids=['one pass', 'two passes', 'three passes', 'three passes, sparse'])
+@pytest.mark.parametrize('tokens', [454_656, 454_657, 1_300_001, 2_000_003])
+def test_gradients_of_long_lists(cuda, tokens, rows, width, index_type):
+    """Lists sorted in tiles of 4, 10, 16 and again 10 keys per thread, by one to three digits, in an even and in a skewed
+    order."""
+    import FasterGSVDACudaBackend as F
+    for kind in ('even', 'skewed'):
+        table, idx, g = _inputs(cuda, rows, width, tokens, torch.float32, kind, index_type)
+        table.requires_grad_(True)
+        out = F.embedding_lookup(table, idx, scale=0.5)
+        _check_rows(out, table, idx, 0.5)
+        out.backward(g)
+        _check_grad(table.grad, g, idx, 0.5)

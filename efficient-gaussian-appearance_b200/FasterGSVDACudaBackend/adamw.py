@@ -99,7 +99,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        self.grad_norm = host().adamw_step(self.state, self.param_groups, self._new_state, self.max_grad_norm)
+        host().adamw_step(self.state, self.param_groups, self._new_state, self.max_grad_norm, self)
         return loss
 
     def read_moments(self, exp_avgs: list | None = None, exp_avg_sqs: list | None = None, dtype: torch.dtype = torch.float32) -> tuple[list, list]:

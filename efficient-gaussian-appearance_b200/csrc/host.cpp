@@ -155,7 +155,7 @@ void changed(const at::Tensor& t) {
 // names of the state and of the group options, made once
 struct Names {
     PyObject *params, *lr, *betas, *eps, *weight_decay, *state_bits, *master_weights, *step, *exp_avg, *exp_avg_sq, *exp_avg_exponent,
-        *exp_avg_sq_exponent, *master, *maximize, *amsgrad, *differentiable, *decoupled_weight_decay;
+        *exp_avg_sq_exponent, *master, *maximize, *amsgrad, *differentiable, *decoupled_weight_decay, *grad_norm;
 } names;
 
 const at::Tensor& state_tensor(PyObject* state, PyObject* key) {
@@ -265,10 +265,18 @@ struct Written {
     }
 };
 
-// adamw_step(state dict, parameter groups, new_state(parameter, bits, master), max_grad_norm or None) -> the norm or None
+// adamw_step(state dict, parameter groups, new_state(parameter, bits, master), max_grad_norm or None[, optimizer]) -> the norm
+// or None; it also becomes the optimizer's grad_norm. (Set from here: torch.compile, which leaves this call out of its graphs,
+// fails on an attribute of an optimizer that is set between them.)
 PyObject* adamw_step(PyObject*, PyObject* args) {
-    PyObject *all_state, *groups, *new_state, *limit;
-    if (!PyArg_ParseTuple(args, "O!O!OO", &PyDict_Type, &all_state, &PyList_Type, &groups, &new_state, &limit)) return nullptr;
+    PyObject *all_state, *groups, *new_state, *limit, *optimizer = nullptr;
+    if (!PyArg_ParseTuple(args, "O!O!OO|O", &PyDict_Type, &all_state, &PyList_Type, &groups, &new_state, &limit, &optimizer)) return nullptr;
+    const auto done = [&](PyObject* norm) {
+        Ref n(must(norm));
+        if (optimizer && PyObject_SetAttr(optimizer, names.grad_norm, n.p)) throw PythonError();
+        Py_INCREF(n.p);
+        return n.p;
+    };
     return guarded([&]() -> PyObject* {
         refuse_recorded("FusedAdamW.step");
         const double max_norm = limit == Py_None ? 0.0 : number(limit);
@@ -346,7 +354,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                 job.hyper.push_back(static_cast<int32_t>(h - 1));
             }
         }
-        if (!any) Py_RETURN_NONE;
+        if (!any) return done(Py_NewRef(Py_None));
         params_written.refuse_shared("two parameters share memory (or one is in the groups twice)");
         const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
         if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
@@ -412,8 +420,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
             }
             if (PyDict_SetItem(c.first, names.step, count.p)) throw PythonError();
         }
-        if (!norm.defined()) Py_RETURN_NONE;
-        return THPVariable_Wrap(norm);
+        return done(norm.defined() ? THPVariable_Wrap(norm) : Py_NewRef(Py_None));
     });
 }
 
@@ -620,6 +627,6 @@ PyMODINIT_FUNC PyInit__fgs_host() {
     const auto name = [](const char* s) { return PyUnicode_InternFromString(s); };
     names = {name("params"),  name("lr"),         name("betas"),            name("eps"),                 name("weight_decay"), name("state_bits"), name("master_weights"),
              name("step"),    name("exp_avg"),    name("exp_avg_sq"),       name("exp_avg_exponent"),    name("exp_avg_sq_exponent"), name("master"),
-             name("maximize"), name("amsgrad"), name("differentiable"), name("decoupled_weight_decay")};
+             name("maximize"), name("amsgrad"), name("differentiable"), name("decoupled_weight_decay"), name("grad_norm")};
     return PyModule_Create(&kModule);
 }

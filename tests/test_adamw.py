@@ -445,3 +445,24 @@ def test_moments_in_8_bits_follow_those_in_64(monkeypatch):
     assert abs(bias) <= 2.0 ** -3 and off <= 1.5 * 2.0 ** -3, (bias, off)
     monkeypatch.setattr(O, 'thresholds', lambda count, step, signed: np.full(count, 2 ** 31, np.int64))
     assert _run_coded(1000)[0] < -0.5
+
+
+@pytest.mark.parametrize('backend', ['eager', 'aot_eager'])
+def test_step_within_a_compiled_function(backend):
+    """torch.compile runs the step between its graphs."""
+    import FasterGSVDACudaBackend as F
+    p = _param(grad=False)
+    opt = F.FusedAdamW([p], max_grad_norm=1.0)
+    opt.grad_norm = 'old'
+    torch._dynamo.reset()
+
+    @torch.compile(backend=backend)
+    def step(x):
+        y = x * 2.0
+        opt.step()
+        return y + 1.0
+
+    assert torch.equal(step(torch.ones(2)), torch.full((2,), 3.0)) and opt.grad_norm is None
+    p.grad = torch.ones(5)
+    with pytest.raises(RuntimeError, match='CUDA'):
+        step(torch.ones(2))

@@ -103,3 +103,35 @@ def test_morton_ordering_gathers_rows(cuda):
         assert torch.equal(t.view(t.params, g.name).reshape(t.n, -1), prims[g.name].reshape(t.n, -1)[order])
         assert torch.equal(t.shard_view(t.exp_avg, g.name)[:t.n], moments[g.name][0][order])
         assert torch.equal(t.shard_view(t.exp_avg_sq, g.name)[:t.n], moments[g.name][1][order])
+
+
+@pytest.mark.parametrize('backend', ['eager', 'aot_eager'])
+def test_training_step_within_compiled_functions(cuda, backend):
+    """torch.compile leaves the lookup, its gradient, the step and the reading of moments out of its graphs: the bits of the
+    calls outside."""
+    import FasterGSVDACudaBackend as F
+    r = torch.Generator().manual_seed(1)
+    start = torch.randn(30, 16, generator=r).to(cuda)
+    idx = torch.randint(0, 30, (100,), generator=r).to(cuda)
+    results = []
+    for wrap in (lambda f: f, torch.compile(backend=backend)):
+        torch._dynamo.reset()
+        table = torch.nn.Parameter(start.clone())
+        opt = F.FusedAdamW([table], state_bits=8, max_grad_norm=0.5)
+
+        @wrap
+        def loss_of(t, i):
+            return (F.embedding_lookup(t * 2.0, i, scale=2.0) + 1.0).square().sum()
+
+        @wrap
+        def step():
+            opt.step()
+            return opt.read_moments()
+
+        for _ in range(2):
+            opt.zero_grad()
+            loss = loss_of(table, idx)
+            loss.backward()
+            moments = step()
+        results.append([loss.detach(), table.detach(), table.grad, opt.grad_norm, *moments[0], *moments[1]])
+    assert all(torch.equal(a, b) for a, b in zip(*results))

@@ -77,21 +77,18 @@ PyObject* must(PyObject* o) {
     return o;
 }
 
-// Runs f() for Python: every C++ exception becomes a Python one.
+// Runs f() for Python: every C++ exception becomes a Python one, as torch translates its own (out of memory, and what a
+// Python hook raised below, which torch.utils.checkpoint needs back as it was).
 template <typename F>
 PyObject* guarded(F&& f) {
     try {
         return f();
     } catch (const PythonError&) {
         return nullptr;
-    } catch (const c10::Error& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
     } catch (const std::length_error& e) {
         PyErr_SetString(PyExc_ValueError, e.what());
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
     } catch (...) {
-        PyErr_SetString(PyExc_RuntimeError, "unknown error in _fgs_host");
+        torch::translate_exception_to_python(std::current_exception());
     }
     return nullptr;
 }

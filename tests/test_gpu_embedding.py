@@ -417,3 +417,33 @@ def test_gradients_of_long_lists(cuda, tokens, rows, width, index_type):
         _check_rows(out, table, idx, 0.5)
         out.backward(g)
         _check_grad(table.grad, g, idx, 0.5)
+
+
+def test_errors_keep_their_kind(cuda):
+    """Out of memory is torch's error for it, and what a hook raises comes through (activation checkpoints stop their second
+    forward that way)."""
+    import FasterGSVDACudaBackend as F
+    table, idx, g = _inputs(cuda, 30, 16, 100, torch.float32, 'even', torch.int64)
+    wide = torch.zeros(1, 2 ** 28, device=cuda)
+    with pytest.raises(torch.OutOfMemoryError):
+        F.embedding_lookup(wide, torch.zeros(4096, dtype=torch.int32, device=cuda))
+    table.requires_grad_(True)
+
+    class Stop(Exception):
+        pass
+
+    def stop(x):
+        raise Stop
+
+    with torch.autograd.graph.saved_tensors_hooks(stop, lambda x: x):
+        with pytest.raises(Stop):
+            F.embedding_lookup(table, idx)
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x, stop):
+        out = F.embedding_lookup(table, idx)
+    with pytest.raises(Stop):
+        torch.autograd.grad(out, table, g)
+    for reentrant in (False, True):
+        out = torch.utils.checkpoint.checkpoint(lambda t: F.embedding_lookup(t, idx, scale=2.0), table, use_reentrant=reentrant)
+        table.grad = None
+        out.backward(g)
+        _check_grad(table.grad, g, idx, 2.0)

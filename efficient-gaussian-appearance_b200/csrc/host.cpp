@@ -509,6 +509,8 @@ struct LookupBackward : torch::autograd::Node {
     torch::autograd::SavedVariable indices;
     std::vector<int64_t> shape;
     at::ScalarType type;
+    at::Device device{at::kCUDA};
+    int64_t tokens;
     double scale;
     int64_t padding;
 
@@ -530,6 +532,15 @@ struct LookupBackward : torch::autograd::Node {
         refuse_recorded("the backward of embedding_lookup");
         refuse_uncapturable();
         const at::Tensor idx = indices.unpack();
+        // direct calls of the node and hooks on saved tensors may hand over anything
+        int64_t width = 1;
+        for (size_t d = 1; d < shape.size(); d++) width *= shape[d];
+        refuse_wrapped(idx, "saved indices");
+        if (idx.layout() != at::kStrided || idx.is_neg() || (idx.scalar_type() != at::kLong && idx.scalar_type() != at::kInt) || !idx.is_contiguous() ||
+            idx.device() != device || idx.numel() != tokens)
+            refuse("the saved indices of embedding_lookup came back with another type, size, order or device");
+        if (grads[0].layout() != at::kStrided || grads[0].device() != device || grads[0].numel() != tokens * width)
+            refuse("embedding_lookup was given a gradient of another size or device than its output");
         at::Tensor grad;
         {
             const at::AutoGradMode no_graph(false);
@@ -538,8 +549,6 @@ struct LookupBackward : torch::autograd::Node {
             grad = at::empty(shape, g.options());
             refuse_wrapped(g, "the gradient of a lookup");
             refuse_wrapped(grad, "the table's gradient");
-            int64_t width = 1;
-            for (size_t d = 1; d < shape.size(); d++) width *= shape[d];
             size_t bytes = 0;
             check(lib.workspace_bytes(idx.numel(), shape[0], width, &bytes));
             const at::Tensor space = at::empty({static_cast<int64_t>(bytes)}, g.options().dtype(at::kByte));
@@ -561,6 +570,8 @@ at::Tensor lookup_with_grad(const at::Tensor& table, const at::Tensor& indices, 
     node->indices = torch::autograd::SavedVariable(indices, false);
     node->shape = table.sizes().vec();
     node->type = table.scalar_type();
+    node->device = table.device();
+    node->tokens = indices.numel();
     node->scale = scale;
     node->padding = padding;
     at::Tensor out = lookup(table, indices, scale, padding);

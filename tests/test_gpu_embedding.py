@@ -447,3 +447,33 @@ def test_errors_keep_their_kind(cuda):
         table.grad = None
         out.backward(g)
         _check_grad(table.grad, g, idx, 2.0)
+
+
+def test_hooks_on_the_node_and_on_saved_indices(cuda):
+    """What hooks and direct calls hand to the backward is checked before a kernel reads it: sizes, types, devices, orders."""
+    import FasterGSVDACudaBackend as F
+    table, idx, g = _inputs(cuda, 30, 16, 100, torch.float32, 'even', torch.int64)
+    table.requires_grad_(True)
+    for spoil in (lambda x: x[:50], lambda x: x[:, :8], lambda x: x.cpu(), lambda x: x.new_empty(0), lambda x: x.to_sparse()):
+        out = F.embedding_lookup(table, idx)
+        with pytest.raises(RuntimeError, match='gradient of another size or device'):  # torch checks nothing of a direct call
+            out.grad_fn(spoil(g))
+        out.grad_fn.register_prehook(lambda grads: (spoil(grads[0]),))  # noqa: B023
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(out, table, g)
+    for spoil in (lambda x: x[:50], lambda x: x.short(), lambda x: x.cpu(), lambda x: torch.stack([x, x], 1)[:, 0], lambda x: x.float()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, spoil):
+            out = F.embedding_lookup(table, idx)
+        with pytest.raises(RuntimeError, match='saved indices of embedding_lookup'):
+            torch.autograd.grad(out, table, g)
+    # and what stays within bounds goes through
+    _check_grad(F.embedding_lookup(table, idx).grad_fn(g), g, idx, 1.0)
+    out = F.embedding_lookup(table, idx, scale=2.0)
+    out.grad_fn.register_prehook(lambda grads: (2.0 * grads[0],))
+    _check_grad(torch.autograd.grad(out, table, g)[0], g, idx, 4.0)
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x.int(), lambda x: x):
+        out = F.embedding_lookup(table, idx)
+    _check_grad(torch.autograd.grad(out, table, g)[0], g, idx, 1.0)
+    with torch.autograd.graph.save_on_cpu():
+        out = F.embedding_lookup(table, idx)
+    _check_grad(torch.autograd.grad(out, table, g)[0], g, idx, 1.0)

@@ -125,12 +125,25 @@ void refuse_wrapped(const at::Tensor& t, const char* name) {
     if (t.key_set().has_any(wrappers)) refuse(std::string(name) + " must be a plain tensor: fake tensors and tensors of function transforms have no memory");
 }
 
+// Refuses tensors whose storage has been freed or shrunk beneath them (resize_, as sharded training does between its uses):
+// their address would be no null pointer, but their place within nothing.
+void refuse_unbacked(const at::Tensor& t, const char* name) {
+    int64_t last = t.storage_offset() + t.numel() - 1;
+    if (!t.is_contiguous()) {
+        last = t.storage_offset();
+        for (int64_t d = 0; d < t.dim(); d++) last += (t.size(d) - 1) * t.stride(d);
+    }
+    if (t.numel() > 0 && t.storage().nbytes() < static_cast<size_t>(last + 1) * t.element_size())
+        refuse(std::string(name) + " has less memory than elements: its storage was resized");
+}
+
 // data address of a contiguous CUDA tensor of the given type and element count on `device` (-1: any, and sets it)
 void* address(const at::Tensor& t, const char* name, int code, int64_t count, int& device) {
     refuse_wrapped(t, name);
     if (t.is_neg()) refuse(std::string(name) + " must not be a lazily negated view: its memory holds the negative");
     if (t.layout() != at::kStrided || type_code(t) != code || !t.is_contiguous())
         refuse(std::string(name) + " must be a contiguous " + kTypeNames[code] + " tensor");
+    refuse_unbacked(t, name);
     if (!t.is_cuda()) refuse(std::string(name) + " must be a CUDA tensor");
     if (device < 0) device = t.get_device();
     if (t.get_device() != device) refuse(std::string(name) + " must be on device cuda:" + std::to_string(device) + " like the others");
@@ -539,15 +552,17 @@ struct LookupBackward : torch::autograd::Node {
         if (idx.layout() != at::kStrided || idx.is_neg() || (idx.scalar_type() != at::kLong && idx.scalar_type() != at::kInt) || !idx.is_contiguous() ||
             idx.device() != device || idx.numel() != tokens)
             refuse("the saved indices of embedding_lookup came back with another type, size, order or device");
+        refuse_unbacked(idx, "saved indices");
         if (grads[0].layout() != at::kStrided || grads[0].device() != device || grads[0].numel() != tokens * width)
             refuse("embedding_lookup was given a gradient of another size or device than its output");
+        refuse_wrapped(grads[0], "the gradient of a lookup");
+        refuse_unbacked(grads[0], "the gradient of a lookup");
         at::Tensor grad;
         {
             const at::AutoGradMode no_graph(false);
             const at::Tensor g = grads[0].to(type).contiguous().resolve_neg();
             const c10::cuda::CUDAGuard guard(g.device());
             grad = at::empty(shape, g.options());
-            refuse_wrapped(g, "the gradient of a lookup");
             refuse_wrapped(grad, "the table's gradient");
             size_t bytes = 0;
             check(lib.workspace_bytes(idx.numel(), shape[0], width, &bytes));
@@ -605,6 +620,8 @@ PyObject* embedding_lookup(PyObject*, PyObject* args) {
                 throw PythonError();
             }
         }
+        refuse_unbacked(table, "table");
+        refuse_unbacked(given, "indices");
         const at::Tensor indices = given.contiguous().resolve_neg();
         return THPVariable_Wrap(table.requires_grad() && at::GradMode::is_enabled() ? lookup_with_grad(table, indices, scale, padding)
                                                                                    : lookup(table, indices, scale, padding));

@@ -466,3 +466,16 @@ def test_step_within_a_compiled_function(backend):
     p.grad = torch.ones(5)
     with pytest.raises(RuntimeError, match='CUDA'):
         step(torch.ones(2))
+
+
+def test_freed_storages_refused():
+    """Storages that were resized beneath their tensors: views within them keep an address."""
+    import FasterGSVDACudaBackend as F
+    flat = torch.ones(20)
+    p = torch.nn.Parameter(flat[10:15])
+    p.grad = torch.ones(5)
+    flat.untyped_storage().resize_(14 * 4)
+    with pytest.raises(RuntimeError, match='a parameter has less memory'):
+        F.FusedAdamW([p]).step()
+    with pytest.raises(RuntimeError, match='an output has less memory'):
+        F.FusedAdamW([_param()]).read_moments([p.detach()], [torch.zeros(5)])

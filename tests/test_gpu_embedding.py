@@ -477,3 +477,42 @@ def test_hooks_on_the_node_and_on_saved_indices(cuda):
     with torch.autograd.graph.save_on_cpu():
         out = F.embedding_lookup(table, idx)
     _check_grad(torch.autograd.grad(out, table, g)[0], g, idx, 1.0)
+
+
+def test_freed_storages_are_refused(cuda):
+    """Tensors whose storage was resized beneath them keep an address and a place within nothing."""
+    import FasterGSVDACudaBackend as F
+    table, idx, g = _inputs(cuda, 30, 16, 100, torch.float32, 'even', torch.int64)
+    table.requires_grad_(True)
+
+    def freed(x, of=lambda x: x):
+        flat = torch.cat([x.detach().reshape(-1)] * 2)
+        view = of(flat[x.numel():].view(x.shape))
+        flat.untyped_storage().resize_((flat.numel() - 1) * x.element_size())
+        return view
+
+    with pytest.raises(RuntimeError, match='table has less memory'):
+        F.embedding_lookup(freed(table), idx)
+    with pytest.raises(RuntimeError, match='indices has less memory'):
+        F.embedding_lookup(table, freed(idx))
+    with pytest.raises(RuntimeError, match='indices has less memory'):
+        F.embedding_lookup(table, freed(torch.stack([idx, idx], 1), lambda x: x[:, 1]))
+    out = F.embedding_lookup(table, idx)
+    for bad in (freed(g), freed(g.t().contiguous(), torch.t)):
+        with pytest.raises(RuntimeError, match='gradient of a lookup has less memory'):
+            torch.autograd.grad(out, table, bad, retain_graph=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x, freed):
+        out = F.embedding_lookup(table, idx)
+    with pytest.raises(RuntimeError, match='saved indices has less memory'):
+        torch.autograd.grad(out, table, g)
+    p = torch.nn.Parameter(torch.ones(8, device=cuda))
+    for name in ('grad', 'exp_avg', 'exp_avg_sq'):
+        opt = F.FusedAdamW([p])
+        p.grad = torch.ones(8, device=cuda)
+        opt.step()
+        if name == 'grad':
+            p.grad = freed(p.grad)
+        else:
+            opt.state[p][name] = freed(opt.state[p][name])
+        with pytest.raises(RuntimeError, match='has less memory'):
+            opt.step()

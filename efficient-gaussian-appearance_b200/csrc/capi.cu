@@ -733,6 +733,10 @@ int fgs_adam_step(const fgs_adam_segment* segs, int n, void* stream) {
     return FGS_OK;
 }
 
+// whether a device address can be read as elements of `bytes` bytes (kernels fault on others)
+static bool placed(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+static uintptr_t dtype_bytes(int dtype) { return dtype == FGS_DTYPE_F32 ? 4 : 2; }
+
 int fgs_adamw_step(const fgs_adamw_tensors* t, const fgs_adamw_hyper* hypers, int n_hypers, int dtype, int state_bits, double* partials,
                    int n_partials, double max_norm, float* grad_norm, void* stream) {
     static_assert(FGS_ADAMW_BLOCK == fgs::kAdamwBlock && FGS_DTYPE_F32 == int(fgs::kDtypeF32) && FGS_DTYPE_BF16 == int(fgs::kDtypeBf16) &&
@@ -747,6 +751,7 @@ int fgs_adamw_step(const fgs_adamw_tensors* t, const fgs_adamw_hyper* hypers, in
         return fail(FGS_ERR_INVALID_ARGUMENT, "NULL argument");
     if (eight && (!t->exp_avg_exponent || !t->exp_avg_sq_exponent)) return fail(FGS_ERR_INVALID_ARGUMENT, "8-bit moments need their exponents");
     if (master && dtype == FGS_DTYPE_F32) return fail(FGS_ERR_INVALID_ARGUMENT, "master weights are for half-precision parameters");
+    if (!placed(partials, 8) || !placed(grad_norm, 4)) return fail(FGS_ERR_INVALID_ARGUMENT, "partials or grad_norm is not aligned to its elements");
     if (partials && (n_partials < 0 || !grad_norm || !(max_norm > 0.0))) return fail(FGS_ERR_INVALID_ARGUMENT, "clipping needs max_norm > 0 and grad_norm");
     try {
         std::vector<fgs::AdamwHyper> H(static_cast<size_t>(n_hypers));
@@ -778,6 +783,9 @@ int fgs_adamw_step(const fgs_adamw_tensors* t, const fgs_adamw_hyper* hypers, in
             if (!t->param[i] || !t->grad[i] || !t->exp_avg[i] || !t->exp_avg_sq[i] || (master && !t->master[i]) ||
                 (eight && (!t->exp_avg_exponent[i] || !t->exp_avg_sq_exponent[i])))
                 return fail(FGS_ERR_INVALID_ARGUMENT, "tensor pointer is NULL");
+            if (!placed(t->param[i], dtype_bytes(dtype)) || !placed(t->grad[i], dtype_bytes(dtype)) || (master && !placed(t->master[i], 4)) ||
+                (!eight && (!placed(t->exp_avg[i], 4) || !placed(t->exp_avg_sq[i], 4))))
+                return fail(FGS_ERR_INVALID_ARGUMENT, "tensor pointer is not aligned to its elements");
             if (t->hyper[i] < 0 || t->hyper[i] >= n_hypers) return fail(FGS_ERR_INVALID_ARGUMENT, "hyperparameter index out of range");
         }
         const fgs::AdamwTensors A{static_cast<int>(t->count), t->param, t->grad, t->exp_avg, t->exp_avg_sq, t->exp_avg_exponent,
@@ -804,9 +812,12 @@ int fgs_grad_squares(const void* const* grads, const int64_t* n_elements, const 
     if (rc != FGS_OK) return rc;
     if (!n_partials || (count > 0 && (!grads || !n_elements || !dtypes || !partials))) return fail(FGS_ERR_INVALID_ARGUMENT, "NULL argument");
     if (capacity < need) return fail(FGS_ERR_WORKSPACE, "too few partial sums");
+    if (!placed(partials, 8)) return fail(FGS_ERR_INVALID_ARGUMENT, "partials is not aligned to its elements");
     for (int64_t i = 0; i < count; i++) {
         if (dtypes[i] > FGS_DTYPE_F16) return fail(FGS_ERR_INVALID_ARGUMENT, "unknown dtype");
         if (n_elements[i] > 0 && !grads[i]) return fail(FGS_ERR_INVALID_ARGUMENT, "gradient pointer is NULL");
+        if (n_elements[i] > 0 && !placed(grads[i], dtype_bytes(dtypes[i])))
+            return fail(FGS_ERR_INVALID_ARGUMENT, "gradient pointer is not aligned to its elements");
     }
     ProfScope p_("grad_norm", static_cast<cudaStream_t>(stream));
     FGS_CUDA(fgs::launch_grad_squares(grads, n_elements, dtypes, static_cast<int>(count), partials, n_partials, static_cast<cudaStream_t>(stream)),
@@ -819,8 +830,10 @@ int fgs_adamw_read_moments(const uint8_t* const* codes, const uint8_t* const* ex
     if (count < 0 || count > 0x7FFFFFFF) return fail(FGS_ERR_INVALID_ARGUMENT, "bad tensor list");
     if (dtype != FGS_DTYPE_F32 && dtype != FGS_DTYPE_BF16) return fail(FGS_ERR_INVALID_ARGUMENT, "moments are read as fp32 or bf16");
     if (count > 0 && (!codes || !exponents || !is_signed || !n_elements || !out)) return fail(FGS_ERR_INVALID_ARGUMENT, "NULL argument");
-    for (int64_t i = 0; i < count; i++)
+    for (int64_t i = 0; i < count; i++) {
         if (n_elements[i] > 0 && (!codes[i] || !exponents[i] || !out[i])) return fail(FGS_ERR_INVALID_ARGUMENT, "tensor pointer is NULL");
+        if (n_elements[i] > 0 && !placed(out[i], dtype_bytes(dtype))) return fail(FGS_ERR_INVALID_ARGUMENT, "output pointer is not aligned to its elements");
+    }
     FGS_CUDA(fgs::launch_read_moments(codes, exponents, is_signed, n_elements, static_cast<int>(count), out, dtype, static_cast<cudaStream_t>(stream)),
              "read moments");
     return FGS_OK;
@@ -848,6 +861,8 @@ int fgs_embedding_lookup(const void* table, int64_t rows, int64_t width, int dty
     const int rc = embedding_args(rows, width, n_indices, dtype, index_bytes, scale, padding_index, &a);
     if (rc != FGS_OK) return rc;
     if (n_indices > 0 && width > 0 && (!indices || !out || (rows > 0 && !table))) return fail(FGS_ERR_INVALID_ARGUMENT, "NULL argument");
+    if (!placed(table, dtype_bytes(dtype)) || !placed(out, dtype_bytes(dtype)) || !placed(indices, static_cast<uintptr_t>(index_bytes)))
+        return fail(FGS_ERR_INVALID_ARGUMENT, "pointer is not aligned to its elements");
     ProfScope p_("embedding", static_cast<cudaStream_t>(stream));
     FGS_CUDA(fgs::launch_embedding_lookup(a, table, indices, out, static_cast<cudaStream_t>(stream)), "embedding lookup");
     return FGS_OK;
@@ -869,6 +884,9 @@ int fgs_embedding_grad(const void* indices, int64_t n_indices, int index_bytes, 
     if (rc != FGS_OK) return rc;
     if (rows > 0 && width > 0 && (!grad_table || (n_indices > 0 && (!indices || !grad_out || !workspace))))
         return fail(FGS_ERR_INVALID_ARGUMENT, "NULL argument");
+    if (!placed(grad_out, dtype_bytes(dtype)) || !placed(grad_table, dtype_bytes(dtype)) || !placed(indices, static_cast<uintptr_t>(index_bytes)))
+        return fail(FGS_ERR_INVALID_ARGUMENT, "pointer is not aligned to its elements");
+    if (!placed(workspace, 16)) return fail(FGS_ERR_WORKSPACE, "embedding workspace must be aligned to 16 bytes");
     if (n_indices > 0 && workspace_bytes < fgs::embedding_workspace_bytes(n_indices, rows, width))
         return fail(FGS_ERR_WORKSPACE, "embedding workspace too small");
     ProfScope p_("embedding_grad", static_cast<cudaStream_t>(stream));

@@ -199,7 +199,7 @@ int fgs_adam_step(const fgs_adam_segment* segments, int n_segments, void* stream
  *   g <- c g;  m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g g;
  *   p <- p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
  * in fp32; c = min(1, max_norm / (norm + 1e-6)) with the norm from fgs_grad_squares, or 1. The arrays of the struct
- * hold one entry per tensor. */
+ * hold one entry per tensor. Pointers that are not aligned to their elements are refused. */
 enum { FGS_DTYPE_F32 = 0, FGS_DTYPE_BF16 = 1, FGS_DTYPE_F16 = 2 };
 #define FGS_ADAMW_BLOCK 256 /* elements that share one exponent byte where the moments are held in 8 bits */
 typedef struct {
@@ -243,7 +243,8 @@ int fgs_embedding_lookup(const void* table, int64_t rows, int64_t width, int dty
                          double scale, int64_t padding_index, void* out, void* stream);
 /* Its gradient: grad_table[v] = scale * sum of grad_out[t] over the t with indices[t] = v, in fp32, rounded once; rows
  * without an index get zeros (grad_table is written whole). The indices are sorted, so the order of the sums, and with
- * it every bit of the result, depends only on the inputs. */
+ * it every bit of the result, depends only on the inputs and on the alignment of grad_out and grad_table (the width of the
+ * accesses follows it). All pointers are aligned to their elements, the workspace to 16 bytes; others are refused. */
 int fgs_embedding_workspace_bytes(int64_t n_indices, int64_t rows, int64_t width, size_t* out);
 int fgs_embedding_grad(const void* indices, int64_t n_indices, int index_bytes, const void* grad_out, int dtype, int64_t rows, int64_t width,
                        double scale, int64_t padding_index, void* grad_table, void* workspace, size_t workspace_bytes, void* stream);

@@ -479,3 +479,27 @@ def test_freed_storages_refused():
         F.FusedAdamW([p]).step()
     with pytest.raises(RuntimeError, match='an output has less memory'):
         F.FusedAdamW([_param()]).read_moments([p.detach()], [torch.zeros(5)])
+
+
+@pytest.mark.parametrize('change', [
+    {'tensors': {'param': (ctypes.c_uint64 * 1)(66)}}, {'tensors': {'grad': (ctypes.c_uint64 * 1)(65)}}, {'tensors': {'exp_avg': (ctypes.c_uint64 * 1)(66)}},
+    {'tensors': {'exp_avg_sq': (ctypes.c_uint64 * 1)(67)}}, {'dtype': 1, 'tensors': {'param': (ctypes.c_uint64 * 1)(65)}},
+    {'dtype': 1, 'tensors': {'master': (ctypes.c_uint64 * 1)(66)}}, {'partials': 68, 'norm': 64, 'max_norm': 1.0}, {'partials': 64, 'norm': 66, 'max_norm': 1.0}])
+def test_c_entry_refuses_misaligned_pointers(change):
+    """A kernel would fault on an address that is no multiple of its elements' size."""
+    with pytest.raises(RuntimeError, match='aligned'):
+        _abi_call(**change)
+
+
+def test_c_entries_of_the_norm_and_the_moments_refuse_misaligned_pointers():
+    from FasterGSVDACudaBackend import _lib
+    lib, check = _lib.lib, _lib.check
+    room, used = ctypes.c_int(0), ctypes.c_int(0)
+    check(lib.fgs_grad_squares_capacity(1, ctypes.byref(room)))
+    ptr, odd, n, kind, a = (ctypes.c_uint64 * 1)(64), (ctypes.c_uint64 * 1)(66), (ctypes.c_int64 * 1)(4), (ctypes.c_uint8 * 1)(0), ctypes.addressof
+    with pytest.raises(RuntimeError, match='gradient pointer is not aligned'):
+        check(lib.fgs_grad_squares(a(odd), a(n), a(kind), 1, 64, room.value, ctypes.byref(used), None))
+    with pytest.raises(RuntimeError, match='partials is not aligned'):
+        check(lib.fgs_grad_squares(a(ptr), a(n), a(kind), 1, 68, room.value, ctypes.byref(used), None))
+    with pytest.raises(RuntimeError, match='output pointer is not aligned'):
+        check(lib.fgs_adamw_read_moments(a(ptr), a(ptr), a(kind), a(n), 1, a(odd), 0, None))

@@ -85,3 +85,15 @@ def test_dependent_kernels_promise_nothing_about_what_they_read():
                 dependent[name] = re.findall(r'const [\w: <>]+\*\s*__restrict__\s+(\w+)', head)
     assert {'radix_downsweep', 'radix_row_scan', 'clip_kernel', 'sum_kernel', 'join_kernel', 'clear_kernel', 'adamw_kernel'} <= set(dependent)
     assert not any(dependent.values()), dependent
+
+
+@pytest.mark.parametrize('place', [{'table': 66}, {'out': 65}, {'indices': 68}, {'workspace': 72}])
+def test_c_entries_refuse_misaligned_pointers(place):
+    """A kernel would fault on an address that is no multiple of its elements' size."""
+    from FasterGSVDACudaBackend._lib import lib, check
+    a = {'table': 64, 'out': 64, 'indices': 64, 'workspace': 64, **place}
+    with pytest.raises(RuntimeError, match='aligned'):
+        check(lib.fgs_embedding_grad(a['indices'], 5, 8, a['table'], 0, 4, 4, 1.0, -1, a['out'], a['workspace'], 1 << 40, None))
+    if 'workspace' not in place:
+        with pytest.raises(RuntimeError, match='aligned'):
+            check(lib.fgs_embedding_lookup(a['table'], 4, 4, 0, a['indices'], 5, 8, 1.0, -1, a['out'], None))

@@ -666,7 +666,8 @@ cudaError_t launch_all(const AdamwTensors& A, const AdamwHyper* hypers, int dtyp
 
 // ---------------------------------------------------------------------------------------------------
 // Sum of squared gradients: per-thread fp32 sums over 32 elements, added up in fp64; one partial sum per CTA, added in a
-// fixed order by the step (or clip_kernel). Bound by HBM: 80 MB of bf16 in 17 us (4.7 TB/s; with one load in flight per
+// fixed order by the step (or clip_kernel). A thread whose fp32 sum overflows (gradients from 1.8e19 on, whose norm is finite)
+// takes its share again in fp64. Bound by HBM: 80 MB of bf16 in 17 us (4.7 TB/s; with one load in flight per
 // thread 31 us).
 
 constexpr int kNormTensors = 1024;
@@ -691,8 +692,27 @@ __device__ inline uint4 load16(const void* a) {
     return r;
 }
 
+// this thread's share of a chunk in fp64: `units` accesses of EACH elements, then single ones
+template <typename P, int EACH>
+__device__ __noinline__ double share_squares(const P* g, uint32_t units, uint32_t n) {
+    double s = 0.0;
+#pragma unroll 1
+    for (uint32_t u = threadIdx.x; u < units; u += kThreads)
+#pragma unroll 1
+        for (int j = 0; j < EACH; j++) {
+            const double y = to_float(g[u * EACH + j]);
+            s = fma(y, y, s);
+        }
+#pragma unroll 1
+    for (uint32_t j = units * EACH + threadIdx.x; j < n; j += kThreads) {
+        const double y = to_float(g[j]);
+        s = fma(y, y, s);
+    }
+    return s;
+}
+
 template <typename P>
-__device__ inline float chunk_squares(const P* g, uint64_t left, bool vec) {
+__device__ inline double chunk_squares(const P* g, uint64_t left, bool vec) {
     constexpr int kEach = 16 / sizeof(P), kLoads = kNormChunk / kEach / kThreads;
     float s = 0.0f;
     const uint32_t n = left < kNormChunk ? static_cast<uint32_t>(left) : kNormChunk;
@@ -714,7 +734,7 @@ __device__ inline float chunk_squares(const P* g, uint64_t left, bool vec) {
         const float y = to_float(g[j]);
         s = fmaf(y, y, s);
     }
-    return s;
+    return s <= 3.4028234663852886e38f ? static_cast<double>(s) : share_squares<P, kEach>(g, units, n);
 }
 
 template <int CAP>
@@ -730,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, 5) grad_squares_kernel(const __grid_
         const uint64_t left = T.n[t] - start;
         const bool vec = T.kind[t] & 128;
         const int dtype = T.kind[t] & 127;
-        float s;
+        double s;
         if (dtype == kDtypeF32) s = chunk_squares(static_cast<const float*>(T.grad[t]) + start, left, vec);
         else if (dtype == kDtypeBf16) s = chunk_squares(static_cast<const __nv_bfloat16*>(T.grad[t]) + start, left, vec);
         else s = chunk_squares(static_cast<const __half*>(T.grad[t]) + start, left, vec);

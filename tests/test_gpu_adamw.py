@@ -578,3 +578,26 @@ def test_long_clipped_steps(cuda, shapes, dtypes, limit, bits):
         opt.step()
         assert abs(float(opt.grad_norm) - norm) <= 18 * 2.0 ** -24 * norm
         _check(opt, before, min(1.0, limit / (norm + 1e-6)), True)
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
+def test_clipping_of_gradients_whose_squares_overflow(cuda, dtype, bits):
+    """Finite gradients up to 1e30, whose squares are no float32 but whose norm is: clipped like others. In whole accesses,
+    in the rest behind them, and in tensors at odd addresses."""
+    import FasterGSVDACudaBackend as F
+    for misalign in (False, True):
+        params = _params([(5000,), (7, 3), (8192 * 3 + 5,)], dtype, cuda, misalign=misalign)
+        opt = F.FusedAdamW(params, state_bits=bits, max_grad_norm=1.0)
+        _grads(params, 1)
+        params[0].grad[17], params[0].grad[4999], params[1].grad[6, 2], params[2].grad[8192 * 3 + 1] = 1e30, 3e29, -1e25, 2e19
+        norm = np.sqrt(sum((_np(p.grad).astype(np.float64) ** 2).sum() for p in params))
+        before = _snapshot(opt)
+        opt.step()
+        assert abs(float(opt.grad_norm) - norm) <= 18 * 2.0 ** -24 * norm
+        assert all(torch.isfinite(p).all() for p in params)
+        if bits == 32:
+            _check(opt, before, 1.0 / (norm + 1e-6), True)
+    params[0].grad[18] = float('inf')
+    opt.step()
+    assert torch.isinf(opt.grad_norm)

@@ -733,8 +733,8 @@ int fgs_adam_step(const fgs_adam_segment* segs, int n, void* stream) {
     return FGS_OK;
 }
 
-// whether a device address can be read as elements of `bytes` bytes (kernels fault on others)
-static bool placed(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+// whether a device address can be read as elements of `bytes` bytes, a power of two (kernels fault on others)
+static bool placed(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 static uintptr_t dtype_bytes(int dtype) { return dtype == FGS_DTYPE_F32 ? 4 : 2; }
 
 int fgs_adamw_step(const fgs_adamw_tensors* t, const fgs_adamw_hyper* hypers, int n_hypers, int dtype, int state_bits, double* partials,

@@ -32,13 +32,16 @@ class FusedAdamW(torch.optim.Optimizer):
         parameter is its rounding. Float32 parameters need none.
     `max_grad_norm` (for all groups together; inf only measures): gradients are scaled by min(1, max_grad_norm /
     (norm + 1e-6)) as they are read, p.grad stays as it is, and `grad_norm` then holds the norm (a 0-dim device tensor, a
-    new one at each step; None after a step without clipping or gradients). An infinite or NaN gradient makes the norm infinite or NaN: the step is then not skipped, what it scales by 0 or NaN
-    becomes so.
+    new one at each step; None after a step without clipping or gradients). An infinite or NaN gradient makes the norm
+    infinite or NaN: the step is then not skipped, what it scales by 0 or NaN becomes so. With 8-bit moments an infinite or
+    NaN moment makes those of its block of 256 elements NaN.
 
     Parameters, gradients and state must be contiguous CUDA tensors on one device, and no two parameters may share
-    memory. The step count is a host value, so a
-    step cannot be captured into a CUDA graph, nor recorded by a tracer (RuntimeError). Anything refused is refused before a kernel is launched
-    and leaves parameters, state and step counts as they were. For autograd a step is a change in place.
+    memory. The step count is a host value, so a step cannot be captured into a CUDA graph, nor recorded by a tracer
+    (RuntimeError); torch.compile runs it between its graphs. Options of other AdamWs that a step does not follow (maximize,
+    amsgrad, differentiable, weight decay that is not decoupled) are refused. Anything refused is refused before state is
+    made or a kernel launched, and leaves parameters, state and step counts as they were. For autograd a step is a change
+    in place.
     """
 
     grad_norm = None

@@ -6,7 +6,8 @@
 // Bound by HBM: every parameter, gradient and moment is read once and written once (28 bytes per fp32 element, 16 with
 // 8-bit moments, 10 in bf16 with them). Measured on a B200 (6.56 TB/s copy): 59M fp32 elements 244 us (6.8 TB/s), with
 // 8-bit moments 159 us (5.9 TB/s); 40M bf16 elements in 300 tensors with fp32 copies 171 us (6.6 TB/s), with 8-bit moments
-// and no copies 102 us (3.9 TB/s: 63 instructions per element at 76 % of the issue slots).
+// and no copies 99 us (4.0 TB/s: 63 instructions per element at 77 % of the issue slots; of 9.1 cycles per issue a warp waits
+// 2.8 for loads, 2.0 ready but not picked, 1.3 for the half-rate pipes).
 //
 // Moments in 8 bits. 256 consecutive elements of a tensor (one warp's share) have one exponent byte E, the largest
 // exponent among them. A code q != 0 stands for the float with the bits (q + 8 (E + 1) - top) << 20: three mantissa
@@ -218,7 +219,8 @@ __device__ inline uint32_t encode1(float x, uint32_t u, int high) {
 
 // Values of two codes, as bf16 (which holds them exactly), from the halves of x: (q + base) << 4, zero for q = 0. Two
 // codes per instruction, and products in the place of shifts and selections, which run at half the rate: the 8-bit step
-// is bound by them. For blocks with base >= 0, where every nonzero code is a normal float.
+// is mostly bound by them. For blocks with base >= 0, where every nonzero code has nonzero bits (subnormal ones at base 1 and
+// 2, where no arithmetic touches them).
 template <bool SIGNED>
 __device__ inline uint32_t decode2(uint32_t x, uint32_t base) {
     const uint32_t q = SIGNED ? x & 0x007f007fu : x;

@@ -6,7 +6,8 @@
 //
 // Forward: one pass, bound by HBM (rows in, rows out). A CTA takes tiles of whole rows (or a part of a long one) in the
 // widest accesses that the row length and the addresses allow. Measured on a B200 (6.56 TB/s copy): 32,768 skewed rows of
-// 2048 bf16 34 us (7.9 TB/s of rows in and out; frequent ones come from L2), 2M rows of 32 floats out of 4096 45 us (6.0 TB/s).
+// 2048 bf16 34 us (7.9 TB/s of rows in and out; frequent ones come from L2), 2M rows of 32 floats out of 4096 52 us
+// (4.4 TB/s of DRAM writes as counted; two thirds of the warps active, waiting for loads).
 //
 // Backward: no atomics, the same sums at every run. The tokens are sorted by index (stably: tokens of one row keep their
 // order; one cluster up to 65536 tokens, sort.cu beyond), and the sorted list is cut into spans, one CTA each, and those
@@ -196,7 +197,7 @@ uint32_t lanes_for(uint64_t units, uint32_t most) {
     return best;
 }
 
-// An output larger than half the L2 is written past it: 2M rows of 32 floats take 51 instead of 68 us, and a short one
+// An output larger than half the L2 is written past it: 2M rows of 32 floats take 52 instead of 68 us, and a short one
 // stays there for its reader.
 constexpr uint64_t kStreamBytes = 64ull << 20;
 
@@ -527,7 +528,8 @@ __device__ inline void clear_rows(P* grad, const SumArgs& a, uint32_t cta, uint8
 
 // A CTA takes a span of sorted positions and a part of the columns; its groups of lanes take a chunk of the span each.
 // Bound by HBM: 32,768 rows of 1024 bf16 in 20 us (97 MB, 4.9 TB/s), 2M rows of 32 floats, gathered 128 bytes at a time, in
-// 54 us (4.8 TB/s). Four accesses in flight per lane and four CTAs per SM; eight and three took 6 us longer there.
+// 54 us (4.8 TB/s). Four accesses in flight per lane and four CTAs per SM; eight and three took 6 us longer there. Eight
+// narrower accesses, and six CTAs where they have 4 bytes (700k rows of 45 floats 99 -> 92 us with six).
 // Within a group a row's sum stays in registers; rows that cross chunk borders are put together in shared memory, by
 // doubling along the groups that lie whole within the row.
 template <typename P, int N>
@@ -778,7 +780,8 @@ size_t carve(void* ws, uint64_t tokens, uint64_t rows, uint64_t width, int size,
     b.vals_b = reinterpret_cast<uint32_t*>(take(small ? 0 : 4 * tokens));
     b.sort_bytes = small ? 0 : row_sort_temp_bytes(tokens);
     b.sort_temp = take(b.sort_bytes);
-    // narrower accesses (misaligned addresses) make more units and longer chunks, never more spans
+    // Narrower accesses (misaligned addresses) widen the groups of lanes, so a CTA has fewer of them and there are more spans
+    // as a rule: room for the most that any width makes.
     uint64_t spans = 1;
     for (int n = row_elements(width, size); n >= 1; n /= 2) {
         SumArgs S{};

@@ -122,7 +122,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict: dict) -> None:
         """As torch's, but the state keeps its own types (torch's casts it to the parameters' type). Groups saved by another
-        AdamW take this one's options where they lack them (its moments are float32: state_bits=32); what this one cannot
+        AdamW take this one's options where they lack them (its moments become float32: state_bits=32); what this one cannot
         follow (maximize, amsgrad, differentiable, weight decay that is not decoupled) is refused, and nothing is changed. Hooks
         around the loading see the whole state."""
         loaded = {}
@@ -157,7 +157,8 @@ class FusedAdamW(torch.optim.Optimizer):
             if name == 'step':
                 value = int(value)
             elif torch.is_tensor(value):
-                value = value.detach().to(p.device, copy=True).contiguous()
+                floats = name in ('exp_avg', 'exp_avg_sq') and value.is_floating_point()  # those of half-precision AdamWs, exactly
+                value = value.detach().to(p.device, torch.float32 if floats else None, copy=True).contiguous()
             else:
                 value = copy.deepcopy(value)
             state[sys.intern(name)] = value

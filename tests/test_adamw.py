@@ -503,3 +503,17 @@ def test_c_entries_of_the_norm_and_the_moments_refuse_misaligned_pointers():
         check(lib.fgs_grad_squares(a(ptr), a(n), a(kind), 1, 68, room.value, ctypes.byref(used), None))
     with pytest.raises(RuntimeError, match='output pointer is not aligned'):
         check(lib.fgs_adamw_read_moments(a(ptr), a(ptr), a(kind), a(n), 1, a(odd), 0, None))
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_half_precision_moments_of_another_adamw_load(dtype):
+    """torch's AdamW keeps its moments in the parameters' type; here they are float32, with the same values."""
+    import FasterGSVDACudaBackend as F
+    p = _param(6, dtype)
+    ref = torch.optim.AdamW([p])
+    ref.step()
+    opt = F.FusedAdamW([p])
+    opt.load_state_dict(ref.state_dict())
+    for name in ('exp_avg', 'exp_avg_sq'):
+        assert opt.state[p][name].dtype == torch.float32 and torch.equal(opt.state[p][name], ref.state[p][name].float())
+        assert ref.state[p][name].dtype == dtype

@@ -601,3 +601,19 @@ def test_clipping_of_gradients_whose_squares_overflow(cuda, dtype, bits):
     params[0].grad[18] = float('inf')
     opt.step()
     assert torch.isinf(opt.grad_norm)
+
+
+def test_goes_on_from_a_checkpoint_of_another_adamw(cuda):
+    import FasterGSVDACudaBackend as F
+    params = _params([(300,), (8, 5)], torch.bfloat16, cuda)
+    ref = torch.optim.AdamW(params, lr=0.02, weight_decay=0.1)
+    for step in (1, 2):
+        _grads(params, step)
+        ref.step()
+    opt = F.FusedAdamW(params)
+    opt.load_state_dict(ref.state_dict())
+    _grads(params, 3)
+    before = _snapshot(opt)
+    assert all(b['step'] == 2 and b['m'].any() for b in before)
+    opt.step()
+    _check(opt, before)
